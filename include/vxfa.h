@@ -287,6 +287,115 @@ int vxfa_flash_attn_ext_noalloc(const vxfa_tensor* q, const vxfa_tensor* k,
                                 vxfa_tensor* dst, float scale, float max_bias,
                                 float logit_softcap, void* stream);
 
+/* ---- Paged K/V cache ---------------------------------------------------------
+ *
+ * Serving many streams from one pool of cache pages. No counterpart in the
+ * reference, whose one stream owns a contiguous cache (src/voxtral.cpp:
+ * 1126-1136) and drops its oldest row when that is full (:1237-1266).
+ *
+ * The pool is two descriptors, k and v [D, page_size, Hkv, n_pages] F16 (rows
+ * contiguous; any 16-byte multiples as nb[1..3], so [page][row][head] and
+ * [page][head][row] both do), page_size a power of two from 16 to 65536. Row r
+ * of stream s lies in row r % page_size of the page that entry
+ * r / page_size of line s of the table names. An entry outside [0, n_pages)
+ * (-1, say) is an absent page: nothing is read there, its rows take no part,
+ * and rows appended there are dropped. So pages that a window has left behind
+ * can be freed at once.
+ *
+ * A call takes all streams of the batch with their chunks of new tokens, one
+ * or many each, packed along q's ne[1]: stream s has the tokens q_start[s] ..
+ * q_start[s + 1] - 1, and they are its last rows, n_kv[s] in all: token i of
+ * t lies in row p = n_kv[s] - t + i. The tables and sizes are device memory,
+ * read when the kernels run, so a captured call follows them from replay to
+ * replay; the host gives bounds. Values out of range do no harm: n_kv is
+ * taken as at most max_nkv, q_start as within the call's tokens and not
+ * decreasing, a row p below 0 takes no part, and tokens past max_nq of a
+ * stream are left out. Rows of q and dst behind the last stream's are neither
+ * read nor written. */
+typedef struct vxfa_paged {
+    const int32_t* pages;    /* device [n_streams][max_pages]                        */
+    const int32_t* n_kv;     /* device [n_streams]: rows in use, the new ones included */
+    const int32_t* q_start;  /* device [n_streams + 1], from 0 up                    */
+    int32_t n_streams;
+    int32_t max_pages;       /* entries of a line of the table                       */
+    int32_t max_nq;          /* no stream has more new tokens                        */
+    int32_t max_nkv;         /* no stream has more rows (0: max_pages * page_size)   */
+    int32_t window;          /* W > 0: a token sees the last W rows up to its own    */
+    int32_t pad_;            /* 0 */
+} vxfa_paged;
+
+/* Store the new rows of all streams in their pages: k_new, v_new F32
+ * [Hkv * D, T, 1, 1] with contiguous rows, rounded to f16 as by
+ * vxfa_kv_append. With rope (positions: one per packed token; they need not
+ * be the rows' numbers) K is rotated first as by vxfa_flash_attn_ext_rope,
+ * and, with q (F32 [D, T, Hq, 1]) and q_out (F16, same ne), so are the
+ * queries, rounded to f16 into q_out; q and q_out come together and need rope.
+ * Two tokens of one row (streams that share a page) leave one of them.
+ * One launch; asynchronous on `stream`. */
+int vxfa_paged_append(vxfa_ctx* ctx, const vxfa_tensor* k_new,
+                      const vxfa_tensor* v_new, const vxfa_paged* batch,
+                      vxfa_tensor* k, vxfa_tensor* v, const vxfa_rope* rope,
+                      const vxfa_tensor* q, vxfa_tensor* q_out, void* stream);
+
+/* Attention of the new tokens over their streams' rows, a token in row p over
+ * the rows j <= p (and j > p - window): q [D, T, Hq, 1] F16 or F32 (rounded
+ * to f16), dst [D, Hq, T, 1] F16 or F32, contiguous, D 64 or 128, any
+ * Hq % Hkv == 0. The score of query head h is
+ *   x = scale q.k;  logit_softcap > 0: x = logit_softcap tanh(x / logit_softcap);
+ *   x += slope_h (j - p), with ggml's slopes for max_bias > 0: n the largest
+ *   power of two in Hq, slope_h = 2^(-max_bias (h + 1) / n) for h < n, else
+ *   2^(-max_bias (2 (h - n) + 1) / (2 n)); 0 for max_bias = 0.
+ * Sums and statistics are F32, the products f16 MFMA; a token that sees no row
+ * gets zeros. Rows that a window removes may still be read where a block of
+ * 32 rows holds one that a token sees, and have to be finite there.
+ *
+ * weights (nullable) collects what each row is worth to the tokens:
+ * F32 [page_size, Hkv, n_pages, 1], elements contiguous along ne[0];
+ * element (row, kv head, page) of every row of a stream becomes that of
+ * weights_in plus the sum, over the tokens and the head's query heads, of the
+ * softmax's weights. weights_in may be weights itself, another tensor of that
+ * shape, or NULL (zeros). Streams that share a page leave one stream's sum
+ * there. Rows of no stream are left as they were. Needs 4 * Hq * T bytes of
+ * the workspace (else VXFA_NO_WORKSPACE).
+ *
+ * The output is deterministic; asynchronous on `stream`. */
+int vxfa_flash_attn_ext_paged(vxfa_ctx* ctx, const vxfa_tensor* q,
+                              const vxfa_tensor* k, const vxfa_tensor* v,
+                              const vxfa_paged* batch, vxfa_tensor* dst,
+                              float scale, float max_bias, float logit_softcap,
+                              const vxfa_tensor* weights_in,
+                              vxfa_tensor* weights, void* stream);
+
+/* What an eviction keeps of every stream and kv head: all rows if there are no
+ * more than `budget`; else the first n_sink, the last n_recent, and of the
+ * others the budget - n_sink - n_recent with the largest weights (of equal
+ * ones the first; a NaN counts as less than any number). */
+typedef struct vxfa_evict {
+    const int32_t* pages;   /* device [n_streams][max_pages]: where the kept rows go */
+    int32_t max_pages;
+    int32_t budget;         /* rows kept of a stream, > 0                            */
+    int32_t n_sink;         /* >= 0; n_sink + n_recent <= budget                     */
+    int32_t n_recent;
+    int32_t* kept;          /* device [n_streams][Hkv][budget]: row numbers kept,
+                               ascending, then -1; or NULL                           */
+    int32_t* n_kv;          /* device [n_streams]: rows left, min(n_kv, budget); or
+                               NULL; not batch->n_kv                                 */
+} vxfa_evict;
+
+/* Keep the best rows of every stream, for each kv head its own: the kept rows
+ * of k, v and weights move, in their order, to rows 0, 1, .. of the pages that
+ * evict->pages names, pages of the same pool that no stream of the call lies
+ * in (streams may share pages, which an eviction in place would spoil for the
+ * others). The old pages are left as they were. batch->q_start, max_nq and
+ * window are not looked at. Rows that lie in absent pages count as rows of
+ * weight NaN and of zeros. Afterwards row numbers are no longer token
+ * positions: the distances and windows of further calls go by rows. Needs
+ * 4 * Hkv * n_streams * min(budget, max_nkv) bytes of the workspace where kept is NULL (else
+ * VXFA_NO_WORKSPACE). Asynchronous on `stream`. */
+int vxfa_paged_evict(vxfa_ctx* ctx, vxfa_tensor* k, vxfa_tensor* v,
+                     vxfa_tensor* weights, const vxfa_paged* batch,
+                     const vxfa_evict* evict, void* stream);
+
 /* Human-readable name of a status code (static storage). */
 const char* vxfa_status_str(int status);
 

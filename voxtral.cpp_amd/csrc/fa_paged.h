@@ -1,0 +1,124 @@
+// fa_paged.h — what the kernels over a paged K/V cache share: the launch
+// descriptors, a stream's sizes and pages as the kernels read them, scores.
+//
+// Tables and sizes lie on the device and may hold anything: every number
+// read there is brought into its range before it is used as an index.
+#pragma once
+
+#include "fa_common.h"
+
+namespace vxfa {
+
+constexpr int kPagedMinLog2 = 4, kPagedMaxLog2 = 16;   // page sizes 16 .. 65536
+
+// The batch: streams, their tables, the pool's pages.
+struct PagedBatch {
+    const int32_t* pages;     // [n_streams][max_pages]
+    const int32_t* n_kv;      // [n_streams]
+    const int32_t* q_start;   // [n_streams + 1]
+    int32_t n_streams, max_pages, n_pages;
+    int32_t ps_log2;          // log2 of a page's rows
+    int32_t tokens;           // packed tokens of the call
+    int32_t max_nq;           // tokens of a stream that are looked at
+    int32_t max_nkv;          // rows of a stream at most (within max_pages pages)
+};
+
+// A stream's sizes: t tokens from packed token q0 on, the last of n rows.
+struct PagedStream {
+    int q0, t, n;
+};
+__device__ __forceinline__ PagedStream paged_stream(const PagedBatch& b, int s) {
+    PagedStream r;
+    r.q0 = min(max(b.q_start[s], 0), b.tokens);
+    r.t = min(max(b.q_start[s + 1], r.q0), b.tokens) - r.q0;
+    r.n = min(max(b.n_kv[s], 0), b.max_nkv);
+    return r;
+}
+
+// The page of entry i of stream s, or -1 (absent).
+__device__ __forceinline__ int paged_page(const PagedBatch& b, int s, int i) {
+    const int p = b.pages[(int64_t)s * b.max_pages + i];
+    return (uint32_t)p < (uint32_t)b.n_pages ? p : -1;
+}
+
+// One matrix of the pool: row r of head h in page p at
+// base + p * nb3 + h * nb2 + r * nb1.
+struct PagedPool {
+    char* base;
+    int64_t nb1, nb2, nb3;
+};
+
+struct PagedAttn {
+    PagedBatch b;
+    const void* q;            // [token][head][D], F16 or F32
+    int64_t q_nb1, q_nb2;     // bytes between tokens, heads
+    PagedPool k, v;
+    void* dst;                // [token][head][D], F16 or F32
+    uint8_t q_f16, dst_f16;
+    int32_t hq, hkv, window;
+    // scores in log2 units: c s; with a cap, cap tanh of it, as
+    // cap - 2 cap / (1 + 2^(c s)) with c = 2 log2(e) scale / softcap
+    float c;                  // scale * log2(e), or the factor above
+    float cap;                // softcap * log2(e); 0: none
+    // distance slopes (bias1 != 0): head h of hq, n2 the largest power of two
+    // in hq: 2^(bias1 (h + 1)) for h < n2, else 2^(bias1 (h - n2 + 1/2))
+    float bias1;              // -max_bias / n2
+    int32_t n2;
+    // accumulated weights
+    const float* w_in;        // null: zeros
+    float* w_out;             // null: none
+    int64_t wi_nb2, wi_nb3, wo_nb2, wo_nb3;
+    float* lse;               // [token][head] log2 of the sum of the row's 2^x (+inf: no row seen); null: not wanted
+    char* ws;                 // scratch
+    size_t ws_bytes;
+};
+
+// slope_h * log2(e)
+__device__ __forceinline__ float paged_slope(const PagedAttn& a, int h) {
+    if (a.bias1 == 0.f) return 0.f;
+    return kLog2e * exp2f(a.bias1 * (h < a.n2 ? (float)(h + 1) : (float)(h - a.n2) + 0.5f));
+}
+// log2-domain score of a product s, without the distance term. (The cap's
+// subtraction near s = 0 leaves 2^-24 of the cap, an absolute error in an
+// exponent.)
+__device__ __forceinline__ float paged_score(float s, float c, float cap) {
+    if (cap == 0.f) return c * s;
+    return fmaf(-2.f * cap, __builtin_amdgcn_rcpf(1.f + exp2_fast(c * s)), cap);
+}
+
+struct PagedAppend {
+    PagedBatch b;
+    const float* k_new;       // [token][Hkv D]
+    const float* v_new;
+    int64_t kn_nb1, vn_nb1;
+    PagedPool k, v;
+    int32_t d, hq, hkv;
+    const int32_t* rope_pos;  // [token]; null: no rotation
+    float rope_ts;
+    int32_t rope_dims;
+    const float* q;           // null: keys and values only
+    int64_t q_nb1, q_nb2;
+    _Float16* q_out;
+    int64_t qo_nb1, qo_nb2;
+};
+
+struct PagedEvict {
+    PagedBatch b;
+    PagedPool k, v;
+    char* w;                  // weights [row of the page] at w + page nb3 + head nb2
+    int64_t w_nb2, w_nb3;
+    int32_t d, hkv;
+    const int32_t* to;        // [n_streams][max_to]
+    int32_t max_to;
+    int32_t budget, n_sink, n_recent;
+    int32_t* kept;            // [n_streams][hkv][kept_row]
+    int32_t kept_row;         // entries of a row (>= min(budget, max_nkv))
+    int32_t* n_out;           // null: not wanted
+};
+
+hipError_t launch_paged_append(const PagedAppend& a, hipStream_t st);
+hipError_t launch_paged_attn(const PagedAttn& a, int head_dim, hipStream_t st);
+hipError_t launch_paged_weights(const PagedAttn& a, int head_dim, hipStream_t st);
+hipError_t launch_paged_evict(const PagedEvict& a, hipStream_t st);
+
+}  // namespace vxfa

@@ -49,9 +49,27 @@ def mask(n_kv: int, rows: int, planes: int = 1, batch: int = 1, row_stride: int 
     return ne, nb
 
 
-def dst(hd: int, heads: int, n_tokens: int, batch: int = 1):
+def kv_pages(n_pages: int, page_size: int, kv_heads: int, hd: int, elt: int = F16_SIZE):
+    """K or V of one layer as a pool of pages for the paged entry points:
+    [hd, page_size, kv_heads, n_pages], each page laid out like the token-major
+    cache. Backing buffer: [n_pages][page_size][kv_heads][hd]."""
+    ne = (hd, page_size, kv_heads, n_pages)
+    nb = (elt, kv_heads * hd * elt, hd * elt, page_size * kv_heads * hd * elt)
+    return ne, nb
+
+
+def weight_pages(n_pages: int, page_size: int, kv_heads: int):
+    """Accumulated attention weights beside a page pool, F32 [page_size,
+    kv_heads, n_pages, 1]. Backing buffer: [n_pages][kv_heads][page_size]."""
+    ne = (page_size, kv_heads, n_pages, 1)
+    nb = (F32_SIZE, page_size * F32_SIZE, kv_heads * page_size * F32_SIZE, n_pages * kv_heads * page_size * F32_SIZE)
+    return ne, nb
+
+
+def dst(hd: int, heads: int, n_tokens: int, batch: int = 1, elt: int = F32_SIZE):
     """Output of flash_attn_ext: F32 [hd, heads, n_tokens, batch], contiguous
-    (already permuted; voxtral then applies cont + reshape, :1612, :1804)."""
+    (already permuted; voxtral then applies cont + reshape, :1612, :1804).
+    The paged entry point writes F16 too (elt 2)."""
     ne = (hd, heads, n_tokens, batch)
-    nb = (F32_SIZE, hd * F32_SIZE, hd * heads * F32_SIZE, hd * heads * n_tokens * F32_SIZE)
+    nb = (elt, hd * elt, hd * heads * elt, hd * heads * n_tokens * elt)
     return ne, nb

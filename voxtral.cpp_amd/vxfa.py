@@ -32,6 +32,9 @@ EXPORTS = (
     "vxfa_flash_attn_ext_ring",
     "vxfa_flash_attn_ext_rope",
     "vxfa_flash_attn_ext_noalloc",
+    "vxfa_paged_append",
+    "vxfa_flash_attn_ext_paged",
+    "vxfa_paged_evict",
     "vxfa_status_str",
     "vxfa_last_error",
     "vxfa_version",
@@ -95,6 +98,50 @@ def rope(positions_ptr: int, n_dims: int, freq_base: float, mode: int = 0, freq_
     return r
 
 
+class VxfaPaged(ctypes.Structure):
+    """vxfa_paged: the streams of a batch over a pool of cache pages (device int32 pointers)."""
+    _fields_ = [
+        ("pages", ctypes.c_void_p),
+        ("n_kv", ctypes.c_void_p),
+        ("q_start", ctypes.c_void_p),
+        ("n_streams", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32),
+        ("max_nq", ctypes.c_int32),
+        ("max_nkv", ctypes.c_int32),
+        ("window", ctypes.c_int32),
+        ("pad_", ctypes.c_int32),
+    ]
+
+
+def paged(pages_ptr: int, n_kv_ptr: int, q_start_ptr: int, n_streams: int, max_pages: int, max_nq: int,
+          max_nkv: int = 0, window: int = 0) -> VxfaPaged:
+    p = VxfaPaged()
+    p.pages, p.n_kv, p.q_start = pages_ptr, n_kv_ptr, q_start_ptr
+    p.n_streams, p.max_pages, p.max_nq, p.max_nkv, p.window = n_streams, max_pages, max_nq, max_nkv, window
+    return p
+
+
+class VxfaEvict(ctypes.Structure):
+    """vxfa_evict: what an eviction keeps, and the pages it goes to (device int32 pointers)."""
+    _fields_ = [
+        ("pages", ctypes.c_void_p),
+        ("max_pages", ctypes.c_int32),
+        ("budget", ctypes.c_int32),
+        ("n_sink", ctypes.c_int32),
+        ("n_recent", ctypes.c_int32),
+        ("kept", ctypes.c_void_p),
+        ("n_kv", ctypes.c_void_p),
+    ]
+
+
+def evict(pages_ptr: int, max_pages: int, budget: int, n_sink: int = 0, n_recent: int = 0, kept: int = 0,
+          n_kv: int = 0) -> VxfaEvict:
+    e = VxfaEvict()
+    e.pages, e.max_pages, e.budget, e.n_sink, e.n_recent = pages_ptr, max_pages, budget, n_sink, n_recent
+    e.kept, e.n_kv = kept, n_kv
+    return e
+
+
 class VxfaError(RuntimeError):
     def __init__(self, status: int, msg: str):
         super().__init__(f"vxfa status {status} ({status_str(status)}): {msg}")
@@ -147,6 +194,14 @@ def load() -> ctypes.CDLL:
     L.vxfa_flash_attn_ext_noalloc.argtypes = [P, P, P, P, P, ctypes.c_float, ctypes.c_float, ctypes.c_float,
                                               ctypes.c_void_p]
     L.vxfa_flash_attn_ext_noalloc.restype = ctypes.c_int
+    B = ctypes.POINTER(VxfaPaged)
+    L.vxfa_paged_append.argtypes = [ctypes.c_void_p, P, P, B, P, P, ctypes.POINTER(VxfaRope), P, P, ctypes.c_void_p]
+    L.vxfa_paged_append.restype = ctypes.c_int
+    L.vxfa_flash_attn_ext_paged.argtypes = [ctypes.c_void_p, P, P, P, B, P, ctypes.c_float, ctypes.c_float,
+                                            ctypes.c_float, P, P, ctypes.c_void_p]
+    L.vxfa_flash_attn_ext_paged.restype = ctypes.c_int
+    L.vxfa_paged_evict.argtypes = [ctypes.c_void_p, P, P, P, B, ctypes.POINTER(VxfaEvict), ctypes.c_void_p]
+    L.vxfa_paged_evict.restype = ctypes.c_int
     L.vxfa_status_str.argtypes = [ctypes.c_int]
     L.vxfa_status_str.restype = ctypes.c_char_p
     L.vxfa_last_error.argtypes = [ctypes.c_void_p]
@@ -257,6 +312,32 @@ class Context:
         rc = self._lib.vxfa_flash_attn_ext_rope(self._h, q, k, v, k_new, v_new,
                                                 rope_desc, mask, dst, scale, max_bias,
                                                 logit_softcap, stream)
+        if check and rc != OK:
+            raise VxfaError(rc, self.last_error())
+        return rc
+
+    def paged_append(self, k_new, v_new, batch, k, v, rope=None, q=None, q_out=None, stream: int = 0,
+                     check: bool = True) -> int:
+        """New rows of all streams into their pages; with rope, K (and q, into q_out as F16) rotated first."""
+        rc = self._lib.vxfa_paged_append(self._h, k_new, v_new, batch, k, v, rope, q, q_out, stream)
+        if check and rc != OK:
+            raise VxfaError(rc, self.last_error())
+        return rc
+
+    def flash_attn_ext_paged(self, q, k, v, batch, dst, scale: float, max_bias: float = 0.0,
+                             logit_softcap: float = 0.0, weights_in=None, weights=None, stream: int = 0,
+                             check: bool = True) -> int:
+        """The new tokens of all streams over their paged rows (batch: VxfaPaged), causal within each stream;
+        weights: accumulated attention weight of each row and kv head, on top of weights_in."""
+        rc = self._lib.vxfa_flash_attn_ext_paged(self._h, q, k, v, batch, dst, scale, max_bias, logit_softcap,
+                                                 weights_in, weights, stream)
+        if check and rc != OK:
+            raise VxfaError(rc, self.last_error())
+        return rc
+
+    def paged_evict(self, k, v, weights, batch, evict_desc, stream: int = 0, check: bool = True) -> int:
+        """Each stream's rows of the largest weights (VxfaEvict), per kv head, moved to other pages."""
+        rc = self._lib.vxfa_paged_evict(self._h, k, v, weights, batch, evict_desc, stream)
         if check and rc != OK:
             raise VxfaError(rc, self.last_error())
         return rc
