@@ -96,6 +96,7 @@ PagedBatch batch_of(const vxfa_paged* b, const vxfa_tensor* k, int64_t tokens) {
     int64_t rows = (int64_t)b->max_pages << r.ps_log2;
     if (rows > 0x7fff0000) rows = 0x7fff0000;
     r.max_nkv = (int32_t)(b->max_nkv > 0 && b->max_nkv < rows ? b->max_nkv : rows);
+    if (r.n_pages == 0) r.max_nkv = 0;   // (an absent page's rows may be loaded from page 0)
     return r;
 }
 
