@@ -117,6 +117,9 @@ struct PagedEvict {
 };
 
 hipError_t launch_paged_append(const PagedAppend& a, hipStream_t st);
+// single tokens, and a few at once (paged_rows_takes)
+bool paged_rows_takes(const PagedAttn& a);
+hipError_t launch_paged_rows(const PagedAttn& a, int head_dim, hipStream_t st);
 hipError_t launch_paged_attn(const PagedAttn& a, int head_dim, hipStream_t st);
 hipError_t launch_paged_weights(const PagedAttn& a, int head_dim, hipStream_t st);
 hipError_t launch_paged_evict(const PagedEvict& a, hipStream_t st);

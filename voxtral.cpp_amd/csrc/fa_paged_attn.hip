@@ -97,6 +97,7 @@ __global__ __launch_bounds__(64) void paged_weights_kernel(PagedAttn a) {
 
 hipError_t launch_paged_attn(const PagedAttn& a, int head_dim, hipStream_t st) {
     if (a.b.tokens <= 0 || a.b.n_streams <= 0) return hipSuccess;
+    if (paged_rows_takes(a)) return launch_paged_rows(a, head_dim, st);
     const dim3 grid((unsigned)a.b.tokens, (unsigned)a.hq);
     if (head_dim == 128) hipLaunchKernelGGL((paged_attn_kernel<128>), grid, dim3(64), 0, st, a);
     else if (head_dim == 64) hipLaunchKernelGGL((paged_attn_kernel<64>), grid, dim3(64), 0, st, a);

@@ -253,7 +253,7 @@ int vxfa_flash_attn_ext_paged(vxfa_ctx* c, const vxfa_tensor* q, const vxfa_tens
     a.dst_f16 = dst->type == VXFA_TYPE_F16;
     a.hq = (int32_t)Hq;
     a.hkv = (int32_t)Hkv;
-    a.window = batch->window;
+    a.window = batch->window < a.b.max_nkv ? batch->window : 0;   // (a window of all rows is none)
     a.c = scale * vxfa::kLog2e;
     if (logit_softcap > 0) {
         a.c = 2.0f * vxfa::kLog2e * (scale / logit_softcap);
