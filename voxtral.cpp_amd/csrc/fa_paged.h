@@ -86,6 +86,18 @@ __device__ __forceinline__ float paged_score(float s, float c, float cap) {
     return fmaf(-2.f * cap, __builtin_amdgcn_rcpf(1.f + exp2_fast(c * s)), cap);
 }
 
+// four output values at element `at`, 16-byte (F16: 8-byte) aligned
+__device__ __forceinline__ void paged_store4(const PagedAttn& a, int64_t at, floatx4 x) {
+    if (a.dst_f16) {
+        half4 y;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = (_Float16)x[i];
+        *(half4*)((_Float16*)a.dst + at) = y;
+    } else {
+        *(floatx4*)((float*)a.dst + at) = x;
+    }
+}
+
 struct PagedAppend {
     PagedBatch b;
     const float* k_new;       // [token][Hkv D]
@@ -120,7 +132,8 @@ hipError_t launch_paged_append(const PagedAppend& a, hipStream_t st);
 // single tokens, and a few at once (paged_rows_takes)
 bool paged_rows_takes(const PagedAttn& a);
 hipError_t launch_paged_rows(const PagedAttn& a, int head_dim, hipStream_t st);
-hipError_t launch_paged_attn(const PagedAttn& a, int head_dim, hipStream_t st);
+// any chunks
+hipError_t launch_paged_chunk(const PagedAttn& a, int head_dim, hipStream_t st);
 hipError_t launch_paged_weights(const PagedAttn& a, int head_dim, hipStream_t st);
 hipError_t launch_paged_evict(const PagedEvict& a, hipStream_t st);
 

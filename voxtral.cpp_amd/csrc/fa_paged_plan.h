@@ -137,4 +137,144 @@ __device__ __forceinline__ Part rows_locate(const PagedBatch& b, const RowsPlan&
 }
 #endif
 
+// ---- chunks -------------------------------------------------------------------
+// A stream's tokens in tiles (bm positions), the rows that a tile walks in
+// pieces; all tiles of a stream have as many pieces. The pieces' length `lp`
+// (blocks of 32 rows) is one of 64 that the lanes weigh.
+
+struct ChunkPlan {
+    uint32_t hpw_log2;        // log2 of the query heads per workgroup
+    int32_t cuts;             // 0: a piece per tile
+    int32_t items;            // pieces in the grid per head group
+    int32_t tiles;            // tiles of all streams at most (sizes that break the bounds: the rest is left out)
+    int32_t room;             // records (of a workgroup's piece) per head group
+    int32_t nhg;
+};
+struct ChunkTile {
+    int32_t s, tile, n, slot; // stream, tile, its pieces, its first record
+};
+struct ChunkBounds {
+    int64_t tiles;            // tiles of all streams at most
+    size_t table;             // bytes of their ChunkTiles
+};
+constexpr int kChunkStreams = 64;   // more streams are not cut
+
+inline ChunkBounds chunk_plan(const PagedBatch& b, int nhg, int bm, size_t record, size_t ws_bytes, ChunkPlan& p) {
+    ChunkBounds r;
+    // sum of ceil(t / bm) over streams of `tokens` tokens in all, max_nq at most each
+    const int64_t per = ((int64_t)b.max_nq + bm - 1) / bm;
+    r.tiles = (int64_t)b.tokens / bm + b.n_streams;
+    if (b.n_streams == 1) r.tiles = ((int64_t)b.tokens + bm - 1) / bm;
+    if (r.tiles > per * b.n_streams) r.tiles = per * b.n_streams;
+    if (r.tiles > b.tokens) r.tiles = b.tokens;
+    r.table = ((size_t)(1 + r.tiles) * sizeof(ChunkTile) + 255) & ~(size_t)255;
+    p.nhg = nhg;
+    p.tiles = (int32_t)r.tiles;
+    const int64_t room = r.table < ws_bytes ? (int64_t)((ws_bytes - r.table) / (record * (size_t)nhg)) : 0;
+    p.room = (int32_t)(room < 4096 ? room : 4096);
+    // tiles for four rounds of the chip's 256 CUs, or too few rows: not cut
+    p.cuts = r.tiles * nhg < 1024 && b.max_nkv >= 128 && b.n_streams <= kChunkStreams && p.room >= 2;
+    int64_t items = r.tiles;
+    if (p.cuts) items = r.tiles > 512 / nhg ? r.tiles : (512 / nhg > 1 ? 512 / nhg : 1);
+    if (p.cuts && items < 2) items = 2;
+    p.items = (int32_t)items;
+    return r;
+}
+
+// piece `piece` of the n of tile `tile` of stream s (-1: none); slot: the tile's
+// first record; tile_no: its number among all tiles, of which there are `tiles`
+struct ChunkItem {
+    int s, tile, piece, n, slot, tile_no, tiles;
+    PagedStream st;
+};
+
+#ifdef __HIPCC__
+__device__ __forceinline__ int wave_scan(int x, int lane) {   // inclusive
+#pragma unroll
+    for (int w = 1; w < 64; w <<= 1) {
+        const int y = __shfl_up(x, w, 64);
+        if (lane >= w) x += y;
+    }
+    return x;
+}
+// ceil(n / d) of small numbers, the same on every lane
+__device__ __forceinline__ int chunk_pieces(int n, int d) { return (n + d - 1) / d; }
+
+__device__ __forceinline__ ChunkItem chunk_locate(const PagedBatch& b, const ChunkPlan& p, int window, int bm, int item) {
+    const int lane = (int)threadIdx.x & 63;
+    ChunkItem r;
+    r.s = -1;
+    r.tiles = 0;
+    int before = 0;
+    for (int s0 = 0; s0 < b.n_streams; s0 += 64) {
+        PagedStream st{0, 0, 0};
+        if (s0 + lane < b.n_streams) st = paged_stream(b, s0 + lane);
+        const int nq = min(st.t, b.max_nq);
+        const int tiles = (nq + bm - 1) / bm;
+        int np = 1;
+        if (p.cuts) {   // (64 streams at most)
+            // blocks that the last tile walks, which is the longest
+            int lo = 0;
+            if (window > 0) lo = max(st.n - st.t + (tiles - 1) * bm - window + 1, 0) / 32;
+            const int nb = tiles > 0 ? max((st.n + 31) / 32 - lo, 1) : 0;
+            // all blocks: a tile before it walks bm / 32 less
+            float work = (float)tiles * (float)nb;
+            if (window <= 0) work = fmaxf(work - (float)(bm / 32) * 0.5f * (float)tiles * (float)(tiles - 1), (float)tiles);
+            float total = work;
+            int longest = nb;
+#pragma unroll
+            for (int w = 1; w < 64; w <<= 1) {
+                longest = max(longest, __shfl_xor(longest, w, 64));
+                total += __shfl_xor(total, w, 64);
+            }
+            // this lane's length: the longest walk in lane + 1 pieces, whole steps
+            const int lp = max((((longest + lane) / (lane + 1)) + 1) & ~1, 2);
+            int items = 0, recs = 0;
+            for (int s = 0; s < b.n_streams; ++s) {
+                const int n = chunk_pieces(__builtin_amdgcn_readlane(nb, s), lp), ts = __builtin_amdgcn_readlane(tiles, s);
+                items += n * ts;
+                recs += n > 1 ? n * ts : 0;
+            }
+            // time in blocks: a workgroup costs its blocks and kWg, 256 run at once;
+            // a record its traffic
+            constexpr float kWg = 4.f, kRecord = 0.05f;
+            const float count = (float)(items * p.nhg), rounds = ceilf(count * (1.f / 256.f));
+            float cost = fmaxf(rounds * (total * (float)p.nhg / fmaxf(count, 1.f) + kWg), (float)lp + kWg) + kRecord * (float)(recs * p.nhg);
+            if (items > p.items || recs > p.room) cost = 3.0e38f;
+            if (lane == 0) cost = fminf(cost, 1.0e38f);   // (one piece a tile always fits)
+            float best = cost;
+#pragma unroll
+            for (int w = 1; w < 64; w <<= 1) best = fminf(best, __shfl_xor(best, w, 64));
+            const int pick = (int)__builtin_ctzll(__ballot(cost == best));
+            np = chunk_pieces(nb, __builtin_amdgcn_readlane(lp, pick));
+            if (pick == 0 || np < 1) np = 1;
+        }
+        const int n = tiles * np;
+        const int incl = wave_scan(n, lane), tincl = wave_scan(tiles, lane);
+        const int rincl = p.cuts ? wave_scan(np > 1 ? n : 0, lane) : 0;
+        const uint64_t hit = r.s < 0 ? __ballot(before + incl > item) : 0;
+        if (hit) {
+            const int w = (int)__builtin_ctzll(hit);
+            r.s = s0 + w;
+            r.n = __builtin_amdgcn_readlane(np, w);
+            const int ts = __builtin_amdgcn_readlane(tiles, w);
+            const int i = item - (before + __builtin_amdgcn_readlane(incl, w) - ts * r.n);
+            r.tile = ts - 1 - i / r.n;              // the longest first
+            r.piece = i % r.n;
+            r.slot = r.n > 1 ? __builtin_amdgcn_readlane(rincl, w) - ts * r.n + (ts - 1 - r.tile) * r.n : 0;
+            r.tile_no = r.tiles + __builtin_amdgcn_readlane(tincl, w) - ts + r.tile;
+            if (r.tile_no >= p.tiles) r.s = -1;
+            r.st.q0 = __builtin_amdgcn_readlane(st.q0, w);
+            r.st.t = __builtin_amdgcn_readlane(st.t, w);
+            r.st.n = __builtin_amdgcn_readlane(st.n, w);
+        }
+        before += __builtin_amdgcn_readlane(incl, 63);
+        r.tiles += __builtin_amdgcn_readlane(tincl, 63);
+        if (hit && item > 0) return r;              // (the first one goes on to count the tiles)
+    }
+    r.tiles = min(r.tiles, p.tiles);
+    return r;
+}
+#endif
+
 }  // namespace vxfa

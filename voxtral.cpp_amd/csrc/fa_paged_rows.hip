@@ -62,17 +62,6 @@ __device__ __forceinline__ float quad_sum(float x) {
     return pair32_sum(__builtin_bit_cast(float, (int)r[0]) + __builtin_bit_cast(float, (int)r[1]));
 }
 
-__device__ __forceinline__ void store4(const PagedAttn& a, int64_t at, floatx4 x) {
-    if (a.dst_f16) {
-        half4 y;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] = (_Float16)x[i];
-        *(half4*)((_Float16*)a.dst + at) = y;
-    } else {
-        *(floatx4*)((float*)a.dst + at) = x;
-    }
-}
-
 template <int D>
 __global__ __launch_bounds__(64 * PR_WAVES, 2) void paged_rows_kernel(RowsArgs ra) {
     constexpr int KS = D / 32;                 // k steps of the first product
@@ -258,7 +247,7 @@ __global__ __launch_bounds__(64 * PR_WAVES, 2) void paged_rows_kernel(RowsArgs r
             if (sub * (int)ra.hpw.d + hh < G) {
                 const int64_t at = (int64_t)(st.q0 + tk) * a.hq + hk * G + sub * (int)ra.hpw.d + hh;
                 const float inv = L == 0.f ? 0.f : 1.f / L;
-                store4(a, at * D + 4 * c, x * inv);
+                paged_store4(a, at * D + 4 * c, x * inv);
                 if (a.lse && c == 0) a.lse[at] = L == 0.f ? INFINITY : M + log2f(L);
             }
         } else {
@@ -326,7 +315,7 @@ __global__ __launch_bounds__(64) void paged_rows_combine(RowsArgs ra) {
     if (grp == 0) {
         const int64_t at = (int64_t)(st.q0 + i) * a.hq + hk * (a.hq / a.hkv) + g;
         const float inv = L == 0.f ? 0.f : 1.f / L;
-        store4(a, at * D + 32 * sl + 4 * f, x * inv);
+        paged_store4(a, at * D + 32 * sl + 4 * f, x * inv);
         if (a.lse && sl == 0 && f == 0) a.lse[at] = L == 0.f ? INFINITY : mm + log2f(L);
     }
 }
