@@ -98,6 +98,12 @@ __device__ __forceinline__ void paged_store4(const PagedAttn& a, int64_t at, flo
     }
 }
 
+// what row r of a page has gathered from this call, on top of what it had
+__device__ __forceinline__ void paged_weight_add(const PagedAttn& a, int page, int hk, int r, float add) {
+    const float old = a.w_in ? *(const float*)((const char*)a.w_in + page * a.wi_nb3 + hk * a.wi_nb2 + 4 * (int64_t)r) : 0.f;
+    *(float*)((char*)a.w_out + page * a.wo_nb3 + hk * a.wo_nb2 + 4 * (int64_t)r) = old + add;
+}
+
 struct PagedAppend {
     PagedBatch b;
     const float* k_new;       // [token][Hkv D]
@@ -131,7 +137,8 @@ struct PagedEvict {
 hipError_t launch_paged_append(const PagedAppend& a, hipStream_t st);
 // single tokens, and a few at once (paged_rows_takes)
 bool paged_rows_takes(const PagedAttn& a);
-hipError_t launch_paged_rows(const PagedAttn& a, int head_dim, hipStream_t st);
+// weighed: the accumulated weights are done, too (else launch_paged_weights)
+hipError_t launch_paged_rows(const PagedAttn& a, int head_dim, hipStream_t st, bool& weighed);
 // any chunks
 hipError_t launch_paged_chunk(const PagedAttn& a, int head_dim, hipStream_t st);
 hipError_t launch_paged_weights(const PagedAttn& a, int head_dim, hipStream_t st);

@@ -1,24 +1,38 @@
 // fa_paged_evict.hip — the rows of each stream and kv head with the largest
 // accumulated weights, moved to other pages.
 //
-// Two launches. paged_select_kernel, a workgroup per (stream, kv head), finds
-// the smallest key that is kept by a radix selection over the weights (four
-// digits of 8 bits of an unsigned key that orders as the floats do, a
-// histogram in LDS each; counts do not depend on the order of the atomics),
-// then lists the kept rows in order: of the rows whose key is that very one the
-// first are taken, as many as are still wanted. paged_move_kernel copies the
-// listed rows, 16 bytes a lane.
+// Two launches.
+//   paged_select_kernel, a workgroup per (stream, kv head): a radix selection
+//   over the weights, as unsigned keys that order as the floats do. Digits of
+//   11, 11 and 10 bits: a histogram in LDS (counts do not depend on the order
+//   of the atomics), a scan of it from the top, and the digit that holds the
+//   last key to be kept. Then the kept rows are listed in order: those of larger
+//   keys, and of those with that very key the first, as many as are still
+//   wanted. A thread has 8 neighbouring rows, whose keys stay in registers from
+//   pass to pass (up to 8192 rows; a longer stream is read again, a segment at
+//   a time).
+//   paged_move_kernel: 8 kept rows a wavefront, K and V at once, 16 bytes a lane,
+//   the four loads of a lane in flight together.
 #include "fa_paged.h"
 
 namespace vxfa {
 
-constexpr int SEL_NT = 1024;
+constexpr int SEL_NT = 1024, SEL_PER = 8, SEL_SEG = SEL_NT * SEL_PER, SEL_BINS = 2048;
 
 // orders as the floats do, -0 as +0, NaN below all
 __device__ __forceinline__ uint32_t sel_key(float x) {
     if (x != x) return 0;
     const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.f);
     return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+
+__device__ __forceinline__ int sel_scan(int x, int lane) {   // inclusive, over a wavefront
+#pragma unroll
+    for (int w = 1; w < 64; w <<= 1) {
+        const int y = __shfl_up(x, w, 64);
+        if (lane >= w) x += y;
+    }
+    return x;
 }
 
 __global__ __launch_bounds__(SEL_NT) void paged_select_kernel(PagedEvict a) {
@@ -32,95 +46,141 @@ __global__ __launch_bounds__(SEL_NT) void paged_select_kernel(PagedEvict a) {
         return;
     }
     const int end = n - a.n_recent;   // rows [n_sink, end) compete
-    auto key_of = [&](int j) -> uint32_t {
-        const int page = paged_page(a.b, s, j >> a.b.ps_log2);
-        if (page < 0) return 0;
-        return sel_key(*(const float*)(a.w + page * a.w_nb3 + h * a.w_nb2 + 4 * (int64_t)(j & ((1 << a.b.ps_log2) - 1))));
+    const int lg = a.b.ps_log2;
+    uint32_t key[SEL_PER];
+    // (8 rows are half a page at most)
+    auto load = [&](int j0) {
+        const int j = j0 + SEL_PER * tid;
+        const int page = j < n ? paged_page(a.b, s, j >> lg) : -1;
+        const float* w = (const float*)(a.w + max(page, 0) * a.w_nb3 + h * a.w_nb2 + 4 * (int64_t)(j & ((1 << lg) - 1)));
+        float x[SEL_PER];
+#pragma unroll
+        for (int i = 0; i < SEL_PER; ++i) x[i] = page >= 0 ? w[i] : 0.f;
+#pragma unroll
+        for (int i = 0; i < SEL_PER; ++i) key[i] = page >= 0 ? sel_key(x[i]) : 0;
     };
-    __shared__ uint32_t hist[256];
+    __shared__ uint32_t hist[SEL_BINS];
+    __shared__ int wsum[2][SEL_NT / 64];
     __shared__ uint32_t pick[2];
-    uint32_t want = (uint32_t)(a.budget - a.n_sink - a.n_recent), prefix = 0;
-    // want > 0: the want-th largest key
-    if (want > 0) {
-        for (int sh = 24; sh >= 0; sh -= 8) {
-            for (int i = tid; i < 256; i += SEL_NT) hist[i] = 0;
+    const bool one = n <= SEL_SEG;
+    if (one) load(0);
+    int want = a.budget - a.n_sink - a.n_recent;   // of the competing rows
+    const bool any = want > 0;
+    uint32_t prefix = 0;
+    if (any) {
+        for (int pass = 0; pass < 3; ++pass) {
+            const int sh = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bits = pass == 2 ? 10 : 11;
+            for (int i = tid; i < SEL_BINS; i += SEL_NT) hist[i] = 0;
             __syncthreads();
-            for (int j = a.n_sink + tid; j < end; j += SEL_NT) {
-                const uint32_t k = key_of(j);
-                if (sh == 24 || (k >> (sh + 8)) == (prefix >> (sh + 8))) atomicAdd(&hist[(k >> sh) & 255], 1u);
+            for (int j0 = 0; j0 < n; j0 += SEL_SEG) {
+                if (!one) load(j0);
+#pragma unroll
+                for (int i = 0; i < SEL_PER; ++i) {
+                    const int j = j0 + SEL_PER * tid + i;
+                    if (j >= a.n_sink && j < end && (pass == 0 || (key[i] >> (sh + bits)) == (prefix >> (sh + bits))))
+                        atomicAdd(&hist[(key[i] >> sh) & ((1 << bits) - 1)], 1u);
+                }
             }
             __syncthreads();
-            if (tid == 0) {
-                uint32_t left = want;
-                int d = 255;
-                while (d > 0 && hist[d] < left) left -= hist[d--];
-                pick[0] = (uint32_t)d;
-                pick[1] = left;
+            // thread t: bins 2047 - 2 t and the one below, from the top
+            const int b1 = SEL_BINS - 1 - 2 * tid;
+            const int c1 = (int)hist[b1], c2 = (int)hist[b1 - 1];
+            const int incl = sel_scan(c1 + c2, lane);
+            if (lane == 63) wsum[0][wave] = incl;
+            __syncthreads();
+            int above = incl - c1 - c2;
+            for (int w = 0; w < wave; ++w) above += wsum[0][w];
+            if (above < want && above + c1 >= want) {
+                pick[0] = (uint32_t)b1;
+                pick[1] = (uint32_t)(want - above);
+            } else if (above + c1 < want && above + c1 + c2 >= want) {
+                pick[0] = (uint32_t)(b1 - 1);
+                pick[1] = (uint32_t)(want - above - c1);
             }
             __syncthreads();
             prefix |= pick[0] << sh;
-            want = pick[1];
-            __syncthreads();
+            want = (int)pick[1];
+            // (hist and pick are written again only after the next barrier but one)
         }
     }
-    // rows in order; `want` of the equal ones
-    __shared__ int wsum[SEL_NT / 64][2];
-    int done = 0, eq_done = 0;   // kept and equal rows before this step
-    const bool any = a.budget - a.n_sink - a.n_recent > 0;
-    for (int j0 = 0; j0 < n; j0 += SEL_NT) {
-        const int j = j0 + tid;
-        const bool in = j < n, always = in && (j < a.n_sink || j >= end);
-        const uint32_t k = in && !always && any ? key_of(j) : 0;
-        const bool eq = in && !always && any && k == prefix, gt = in && !always && any && k > prefix;
-        const uint64_t below = ((uint64_t)1 << lane) - 1, em = __ballot(eq);
-        if (lane == 0) wsum[wave][0] = __popcll(em);
+    // rows in order; `want` of those with the key `prefix`
+    int done = 0, eq_done = 0;   // kept and equal rows of the segments before
+    for (int j0 = 0; j0 < n; j0 += SEL_SEG) {
+        if (!one) load(j0);
+        const int jt = j0 + SEL_PER * tid;
+        int eq = 0;
+#pragma unroll
+        for (int i = 0; i < SEL_PER; ++i) eq += any && jt + i >= a.n_sink && jt + i < end && key[i] == prefix;
         __syncthreads();
-        int eb = eq_done + __popcll(em & below), et = 0;
+        const int ei = sel_scan(eq, lane);
+        if (lane == 63) wsum[0][wave] = ei;
+        __syncthreads();
+        int eb = eq_done + ei - eq;
         for (int w = 0; w < SEL_NT / 64; ++w) {
-            if (w < wave) eb += wsum[w][0];
-            et += wsum[w][0];
+            if (w < wave) eb += wsum[0][w];
+            eq_done += wsum[0][w];
         }
-        const bool keep = always || gt || (eq && eb < (int)want);
-        const uint64_t km = __ballot(keep);
-        if (lane == 0) wsum[wave][1] = __popcll(km);
+        uint32_t keep = 0;
+#pragma unroll
+        for (int i = 0; i < SEL_PER; ++i) {
+            const int j = jt + i;
+            if (j >= n) continue;
+            if (j < a.n_sink || j >= end) keep |= 1u << i;
+            else if (any && key[i] > prefix) keep |= 1u << i;
+            else if (any && key[i] == prefix && eb++ < want) keep |= 1u << i;
+        }
+        const int c = __popc(keep), ki = sel_scan(c, lane);
+        if (lane == 63) wsum[1][wave] = ki;
         __syncthreads();
-        int kb = done + __popcll(km & below), kt = 0;
+        int kb = done + ki - c;
         for (int w = 0; w < SEL_NT / 64; ++w) {
-            if (w < wave) kb += wsum[w][1];
-            kt += wsum[w][1];
+            if (w < wave) kb += wsum[1][w];
+            done += wsum[1][w];
         }
-        if (keep && kb < a.kept_row) kept[kb] = j;
-        done += kt;
-        eq_done += et;
-        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < SEL_PER; ++i)
+            if (((keep >> i) & 1) && kb < a.kept_row) kept[kb++] = jt + i;
     }
     for (int r = done + tid; r < a.kept_row; r += SEL_NT) kept[r] = -1;
 }
 
-// a wavefront per kept row: K, V and the weight
+template <int D>
 __global__ __launch_bounds__(256) void paged_move_kernel(PagedEvict a) {
-    const int lane = (int)threadIdx.x & 63, r = (int)blockIdx.x * 4 + ((int)threadIdx.x >> 6);
-    const int h = (int)blockIdx.y, s = (int)blockIdx.z;
-    if (r >= a.kept_row) return;
-    const int j = a.kept[((int64_t)s * a.hkv + h) * a.kept_row + r];
-    if (j < 0) return;
+    constexpr int CH = D / 8, RPW = 64 / (2 * CH);   // rows of one step: CH lanes of K, CH of V each
+    constexpr int U = 8 / RPW;
+    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+    const int h = (int)blockIdx.x % a.hkv, r0 = ((int)blockIdx.x / a.hkv * 4 + wave) * 8, s = (int)blockIdx.y;
     const int lg = a.b.ps_log2, mask = (1 << lg) - 1;
-    if ((r >> lg) >= a.max_to) return;
-    const int to = a.to[(int64_t)s * a.max_to + (r >> lg)];
-    if ((uint32_t)to >= (uint32_t)a.b.n_pages) return;
-    const int from = paged_page(a.b, s, j >> lg);
-    const int ch = a.d / 8;
-    if (lane < 2 * ch) {
-        const PagedPool& p = lane < ch ? a.k : a.v;
-        const int64_t o = 16 * (lane % ch) + h * p.nb2;
-        u32x4 x = {0, 0, 0, 0};
-        if (from >= 0) x = *(const u32x4*)(p.base + from * p.nb3 + (j & mask) * p.nb1 + o);
-        *(u32x4*)(p.base + to * p.nb3 + (r & mask) * p.nb1 + o) = x;
+    const int32_t* kept = a.kept + ((int64_t)s * a.hkv + h) * a.kept_row;
+    const PagedPool& pool = (lane / CH) & 1 ? a.v : a.k;
+    const int64_t col = 16 * (lane % CH) + h * pool.nb2;
+    int j[U], to[U], from[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int r = r0 + RPW * u + lane / (2 * CH);
+        j[u] = r < a.kept_row ? kept[r] : -1;
+        to[u] = (r >> lg) < a.max_to && r < a.kept_row ? a.to[(int64_t)s * a.max_to + (r >> lg)] : -1;
+        if ((uint32_t)to[u] >= (uint32_t)a.b.n_pages) to[u] = -1;
     }
-    if (lane == 63) {
-        float x = __builtin_nanf("");
-        if (from >= 0) x = *(const float*)(a.w + from * a.w_nb3 + h * a.w_nb2 + 4 * (j & mask));
-        *(float*)(a.w + to * a.w_nb3 + h * a.w_nb2 + 4 * (r & mask)) = x;
+#pragma unroll
+    for (int u = 0; u < U; ++u) from[u] = j[u] >= 0 && to[u] >= 0 ? paged_page(a.b, s, j[u] >> lg) : -1;
+    u32x4 x[U];
+    float w[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        x[u] = u32x4{0, 0, 0, 0};
+        w[u] = __builtin_nanf("");
+        if (from[u] >= 0) {
+            x[u] = __builtin_nontemporal_load((const u32x4*)(pool.base + from[u] * pool.nb3 + (j[u] & mask) * pool.nb1 + col));
+            if (lane % (2 * CH) == 0) w[u] = *(const float*)(a.w + from[u] * a.w_nb3 + h * a.w_nb2 + 4 * (j[u] & mask));
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int r = r0 + RPW * u + lane / (2 * CH);
+        if (j[u] < 0 || to[u] < 0) continue;
+        *(u32x4*)(pool.base + to[u] * pool.nb3 + (r & mask) * pool.nb1 + col) = x[u];
+        if (lane % (2 * CH) == 0) *(float*)(a.w + to[u] * a.w_nb3 + h * a.w_nb2 + 4 * (r & mask)) = w[u];
     }
 }
 
@@ -129,7 +189,12 @@ hipError_t launch_paged_evict(const PagedEvict& a, hipStream_t st) {
     hipLaunchKernelGGL(paged_select_kernel, dim3((unsigned)a.b.n_streams, (unsigned)a.hkv), dim3(SEL_NT), 0, st, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(paged_move_kernel, dim3((unsigned)((a.kept_row + 3) / 4), (unsigned)a.hkv, (unsigned)a.b.n_streams), dim3(256), 0, st, a);
+    const int64_t gx = ((int64_t)a.kept_row + 31) / 32 * a.hkv;
+    if (gx > kMaxGridX) return hipErrorInvalidValue;
+    const dim3 grid((unsigned)gx, (unsigned)a.b.n_streams);
+    if (a.d == 128) hipLaunchKernelGGL((paged_move_kernel<128>), grid, dim3(256), 0, st, a);
+    else if (a.d == 64) hipLaunchKernelGGL((paged_move_kernel<64>), grid, dim3(256), 0, st, a);
+    else return hipErrorInvalidValue;
     return hipGetLastError();
 }
 

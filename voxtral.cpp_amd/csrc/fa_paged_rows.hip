@@ -41,6 +41,10 @@ struct RowsArgs {
     int32_t items;            // parts in the grid per head group
     int2* cut;                // [n_streams] first part, parts of a stream
     float* recs;              // [head group][part][rec]
+    // the scores, for the weights that the rows gather: null, or
+    // [head group][stream][query row][xrow], -inf where a row is not seen
+    float* x;
+    int64_t xrow;
 };
 
 template <int N>
@@ -164,6 +168,7 @@ __global__ __launch_bounds__(64 * PR_WAVES, 2) void paged_rows_kernel(RowsArgs r
     const int vr = 4 * quad + (row >> 2);      // the row this lane addresses, 8 bytes 16 db + 4 (row % 4) of it
     const int vaddr = MAT + vr * ROW + (row & 1) * 8, vsw = swv(vr);
 
+    float* const xs = ra.x && valid ? ra.x + (((int64_t)hg * a.b.n_streams + part.s) * ra.rows + row) * ra.xrow : nullptr;
     for (int k = 0; k < nk; ++k) {
         pr_wait_lds();
         if (k + NS - 1 < nk) {
@@ -190,6 +195,7 @@ __global__ __launch_bounds__(64 * PR_WAVES, 2) void paged_rows_kernel(RowsArgs r
             x[i] = j >= first && j <= p ? x[i] : -INFINITY;
             mx = fmaxf(mx, x[i]);
         }
+        if (xs) *(floatx4*)(xs + j0) = floatx4{x[0], x[1], x[2], x[3]};
         mx = quad_max(mx);
         if (__any(mx > m)) {
             const float mn = fmaxf(m, mx), al = exp2_fast(m - (mn == -INFINITY ? 0.f : mn));
@@ -320,11 +326,36 @@ __global__ __launch_bounds__(64) void paged_rows_combine(RowsArgs ra) {
     }
 }
 
+// The weights that the rows gather from scores that paged_rows_kernel left: a
+// thread per row and kv head sums 2^(x - lse) over the query rows.
+__global__ __launch_bounds__(256) void paged_rows_weights(RowsArgs ra) {
+    const PagedAttn& a = ra.a;
+    const int s = (int)blockIdx.y, hk = (int)blockIdx.x % a.hkv, j = (int)blockIdx.x / a.hkv * 256 + (int)threadIdx.x;
+    const PagedStream st = paged_stream(a.b, s);
+    if (j >= st.n) return;
+    const int page = paged_page(a.b, s, j >> a.b.ps_log2);
+    if (page < 0) return;
+    float sum = 0.f;
+    const int G = a.hq / a.hkv, hpw = (int)ra.hpw.d;
+    if (j >= rows_first(st, a.window)) {
+        for (int sub = 0; sub < ra.groups; ++sub) {
+            const float* x = ra.x + ((int64_t)(hk * ra.groups + sub) * a.b.n_streams + s) * ra.rows * ra.xrow + j;
+            const int heads = min(hpw, G - sub * hpw);
+            for (int i = 0; i < min(st.t, a.b.max_nq); ++i) {
+                const float* lse = a.lse + (int64_t)(st.q0 + i) * a.hq + hk * G + sub * hpw;
+                for (int h = 0; h < heads; ++h) sum += exp2_fast(x[(int64_t)(i * hpw + h) * ra.xrow] - lse[h]);
+            }
+        }
+    }
+    paged_weight_add(a, page, hk, j & ((1 << a.b.ps_log2) - 1), sum);
+}
+
 bool paged_rows_takes(const PagedAttn& a) {
     return (int64_t)a.b.max_nq * rows_heads(a.hq / a.hkv) <= 16;
 }
 
-hipError_t launch_paged_rows(const PagedAttn& a, int head_dim, hipStream_t st) {
+hipError_t launch_paged_rows(const PagedAttn& a, int head_dim, hipStream_t st, bool& weighed) {
+    weighed = false;
     if (!paged_rows_takes(a)) return hipErrorInvalidValue;
     RowsArgs ra;
     ra.a = a;
@@ -337,8 +368,19 @@ hipError_t launch_paged_rows(const PagedAttn& a, int head_dim, hipStream_t st) {
     const size_t cut = ((size_t)a.b.n_streams * sizeof(int2) + 255) & ~(size_t)255;
     if (cut > a.ws_bytes) return hipErrorInvalidValue;   // (65535 streams at most: half a MiB)
     ra.cut = reinterpret_cast<int2*>(a.ws);
-    ra.recs = reinterpret_cast<float*>(a.ws + cut);
-    const int64_t room = (int64_t)((a.ws_bytes - cut) / ((size_t)ra.rec * sizeof(float))) / nhg;
+    size_t used = cut;
+    // scores, if they leave the records' usual room; else the weights form them again
+    ra.x = nullptr;
+    ra.xrow = ((int64_t)a.b.max_nkv + 15) & ~(int64_t)15;
+    const double xb = (double)nhg * a.b.n_streams * ra.rows * (double)ra.xrow * sizeof(float);
+    const size_t usual = (size_t)(512 + (size_t)a.b.n_streams * nhg) * ra.rec * sizeof(float);
+    if (a.w_out && xb + (double)used + (double)usual <= (double)a.ws_bytes) {
+        ra.x = reinterpret_cast<float*>(a.ws + used);
+        used += ((size_t)xb + 255) & ~(size_t)255;
+        weighed = true;
+    }
+    ra.recs = reinterpret_cast<float*>(a.ws + used);
+    const int64_t room = used < a.ws_bytes ? (int64_t)((a.ws_bytes - used) / ((size_t)ra.rec * sizeof(float))) / nhg : 0;
     ra.p = rows_plan(a.b, nhg, room, ra.items);
     const int64_t nwg = (int64_t)ra.items * nhg;
     if (nwg > 0x7fffffff / 256) return hipErrorInvalidValue;
@@ -346,10 +388,18 @@ hipError_t launch_paged_rows(const PagedAttn& a, int head_dim, hipStream_t st) {
     if (head_dim == 128) hipLaunchKernelGGL((paged_rows_kernel<128>), grid, block, 0, st, ra);
     else hipLaunchKernelGGL((paged_rows_kernel<64>), grid, block, 0, st, ra);
     hipError_t e = hipGetLastError();
-    if (e != hipSuccess || !ra.p.cuts) return e;
-    const dim3 cg((unsigned)(a.hq * (head_dim / 32)), (unsigned)a.b.max_nq, (unsigned)a.b.n_streams);
-    if (head_dim == 128) hipLaunchKernelGGL((paged_rows_combine<128>), cg, dim3(64), 0, st, ra);
-    else hipLaunchKernelGGL((paged_rows_combine<64>), cg, dim3(64), 0, st, ra);
+    if (e != hipSuccess) return e;
+    if (ra.p.cuts) {
+        const dim3 cg((unsigned)(a.hq * (head_dim / 32)), (unsigned)a.b.max_nq, (unsigned)a.b.n_streams);
+        if (head_dim == 128) hipLaunchKernelGGL((paged_rows_combine<128>), cg, dim3(64), 0, st, ra);
+        else hipLaunchKernelGGL((paged_rows_combine<64>), cg, dim3(64), 0, st, ra);
+        e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    if (!ra.x) return e;
+    const int64_t gx = ((int64_t)a.b.max_nkv + 255) / 256 * a.hkv;
+    if (gx > kMaxGridX) return hipErrorInvalidValue;
+    hipLaunchKernelGGL(paged_rows_weights, dim3((unsigned)gx, (unsigned)a.b.n_streams), dim3(256), 0, st, ra);
     return hipGetLastError();
 }
 

@@ -1,42 +1,194 @@
-// fa_paged_weights.hip — the weights that the rows of a paged cache gather.
+// fa_paged_weights.hip — the attention weight that each row of a paged cache
+// gathers from the tokens of a call, for gfx950.
+//
+// A row's weight is the sum, over tokens i and the kv head's query heads, of
+// P_ij = 2^(x_ij - lse_i), where lse_i (the logarithm of the row sum) is only
+// known when the attention is done: the scores are formed again, from K alone,
+// half the attention's products. (Single tokens: paged_rows_kernel has left its
+// scores, and paged_weights_rows sums them; see there.)
+//   Workgroup = 128 rows of a stream and kv head, 4 wavefronts: two halves of 64
+//   rows by two halves of the query rows. S^T = K Q^T by
+//   v_mfma_f32_32x32x16_f16: a lane has the scores of 16 rows for one query row,
+//   so lse, position and slope are one register each, and the sums over query rows
+//   stay in 16 registers a block until the end. K stays in registers; 64 query
+//   rows (tokens x heads, packed) a step go through LDS, loaded a step ahead, of
+//   those tokens only that see some of the 128 rows.
+// One workgroup owns a row's sum: no atomics, the same bits every time.
 #include "fa_paged.h"
 
 namespace vxfa {
 
-// One thread per (row of a stream, kv head): the scores again, now that the
-// tokens' sums are known.
-template <int D>
-__global__ __launch_bounds__(64) void paged_weights_kernel(PagedAttn a) {
-    const int s = (int)blockIdx.y, hk = (int)blockIdx.z, j = (int)blockIdx.x * 64 + (int)threadIdx.x;
+constexpr int PW_ROWS = 128;
+
+struct WeightsArgs {
+    PagedAttn a;
+    DivMod grp;               // query heads per kv head
+    int32_t ntiles;           // row tiles of a stream at most
+};
+
+template <int D, bool QF16>
+__global__ __launch_bounds__(256, 2) void paged_weights_kernel(WeightsArgs wa) {
+    constexpr int KS = D / 16, ROW = 2 * D, CH = D / 8;
+    constexpr int STEP = 64 * ROW;                  // bytes of 64 query rows
+    __shared__ __attribute__((aligned(16))) char smem[2 * STEP];
+    __shared__ float part[2][64];
+    const PagedAttn& a = wa.a;
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int nl = lane & 31, hh = lane >> 5;
+    const int ph = wave & 1, rh = wave >> 1;        // half of the rows, of the query rows
+    const int s = (int)blockIdx.y, hk = (int)blockIdx.x % a.hkv, kv0 = (int)blockIdx.x / a.hkv * PW_ROWS;
     const PagedStream st = paged_stream(a.b, s);
-    if (j >= st.n) return;
-    const int page = paged_page(a.b, s, j >> a.b.ps_log2), r = j & ((1 << a.b.ps_log2) - 1);
-    if (page < 0) return;
-    half8 k[D / 8];
-    for (int d = 0; d < D / 8; ++d) k[d] = ((const half8*)(a.k.base + page * a.k.nb3 + hk * a.k.nb2 + r * a.k.nb1))[d];
-    float sum = 0.f;
-    const int G = a.hq / a.hkv;
-    for (int i = 0; i < min(st.t, a.b.max_nq); ++i) {
-        const int p = st.n - st.t + i;
-        if (j > p || (a.window > 0 && j <= p - a.window)) continue;
-        for (int h = hk * G; h < (hk + 1) * G; ++h) {
-            float dot = 0.f;
-            for (int d = 0; d < D / 8; ++d) {
-                const half8 q = load_q8(a.q, (int64_t)(st.q0 + i) * a.q_nb1 + (int64_t)h * a.q_nb2 + 8 * d * (a.q_f16 ? 2 : 4), a.q_f16);
-                for (int e = 0; e < 8; ++e) dot = fmaf((float)k[d][e], (float)q[e], dot);
-            }
-            sum += exp2_fast(paged_score(dot, a.c, a.cap) + paged_slope(a, h) * (float)(j - p) - a.lse[(int64_t)(st.q0 + i) * a.hq + h]);
+    if (kv0 >= st.n) return;
+    const int lg = a.b.ps_log2, pmask = (1 << lg) - 1;
+    const int G = (int)wa.grp.d, nq = min(st.t, a.b.max_nq), past = st.n - st.t;
+
+    // ---- K: A operand, row nl of a block, dims 16 ks + 8 hh .. (rows that are not
+    // there: zeros) ------------------------------------------------------------------
+    half8 kr[2][KS];
+    int pos[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+        pos[b] = kv0 + 64 * ph + 32 * b;
+        const int j = pos[b] + nl;
+        const int page = j < st.n ? paged_page(a.b, s, j >> lg) : -1;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) kr[b][ks] = half8{};
+        if (page >= 0) {
+            const char* p = a.k.base + page * a.k.nb3 + (int64_t)hk * a.k.nb2 + (int64_t)(j & pmask) * a.k.nb1 + 16 * hh;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) kr[b][ks] = *(const half8*)(p + 32 * ks);
         }
     }
-    const float old = a.w_in ? *(const float*)((const char*)a.w_in + page * a.wi_nb3 + hk * a.wi_nb2 + 4 * r) : 0.f;
-    *(float*)((char*)a.w_out + page * a.wo_nb3 + hk * a.wo_nb2 + 4 * r) = old + sum;
+
+    // ---- query rows (token G + head) that see some of the rows -----------------
+    const int t0 = min(max(kv0 - past, 0), nq);
+    int t1 = nq;
+    if (a.window > 0) t1 = min((int)min((int64_t)kv0 + PW_ROWS - 1 + a.window - past, (int64_t)nq), nq);
+    const int r_begin = t0 * G, r_end = max(t1, t0) * G;
+    constexpr int QN = QF16 ? 64 * CH / 256 : 2 * 64 * CH / 256;   // 16-byte loads of a thread
+    constexpr int QC = QF16 ? CH : 2 * CH;                          // of a row
+    floatx4 qraw[QN];
+    auto load_q = [&](int r0) {
+#pragma unroll
+        for (int u = 0; u < QN; ++u) {
+            const int e = tid + 256 * u, r = min(r0 + e / QC, r_end - 1);
+            const int tk = (int)wa.grp.div((uint32_t)r), h = hk * G + r - tk * G;
+            qraw[u] = *((const floatx4*)((const char*)a.q + (int64_t)(st.q0 + tk) * a.q_nb1 + (int64_t)h * a.q_nb2) + e % QC);
+        }
+    };
+    // 16-byte chunk j of row r at j ^ (r % CH)
+    auto put_q = [&](int buf) {
+#pragma unroll
+        for (int u = 0; u < QN; ++u) {
+            const int e = tid + 256 * u, r = e / QC, j = e % QC;
+            char* row = smem + buf * STEP + r * ROW;
+            if constexpr (QF16) {
+                *(floatx4*)(row + ((j ^ (r % CH)) * 16)) = qraw[u];
+            } else {
+                half4 y;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) y[i] = (_Float16)qraw[u][i];
+                *(half4*)(row + (((j >> 1) ^ (r % CH)) * 16) + (j & 1) * 8) = y;
+            }
+        }
+    };
+    float sum[2][16];
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) sum[b][j] = 0.f;
+
+    const bool mod = a.cap != 0.f || a.bias1 != 0.f;
+    if (r_begin < r_end) load_q(r_begin);
+    for (int r0 = r_begin, buf = 0; r0 < r_end; r0 += 64, buf ^= 1) {
+        put_q(buf);
+        // this lane's query row
+        const int r = r0 + 32 * rh + nl, rc = min(r, r_end - 1);
+        const int tk = (int)wa.grp.div((uint32_t)rc), h = hk * G + rc - tk * G;
+        float lse = a.lse[(int64_t)(st.q0 + tk) * a.hq + h];
+        if (r >= r_end) lse = INFINITY;             // (weight 0)
+        if (r0 + 64 < r_end) load_q(r0 + 64);
+        __syncthreads();                            // (the other buffer is read until the next one)
+        const int p = past + tk, first = a.window > 0 ? p - a.window + 1 : INT32_MIN;
+        const float slope = mod ? paged_slope(a, h) : 0.f;
+        half8 qb[KS];
+        const char* row = smem + buf * STEP + (32 * rh + nl) * ROW;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) qb[ks] = *(const half8*)(row + (((2 * ks + hh) ^ (nl % CH)) * 16));
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            floatx16 x = {};
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) x = __builtin_amdgcn_mfma_f32_32x32x16_f16(kr[b][ks], qb[ks], x, 0, 0, 0);
+            // element j: row pos + 8 (j / 4) + 4 hh + j % 4
+            const int j0 = pos[b] + 4 * hh;
+            if (mod) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    x[j] = fmaf(slope, (float)(j0 + 8 * (j >> 2) + (j & 3) - p), paged_score(x[j], a.c, a.cap)) - lse;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) x[j] = fmaf(a.c, x[j], -lse);
+            }
+            // (a block that all the wavefront's query rows see whole needs no mask)
+            if (__any(pos[b] + 31 > p || pos[b] < first)) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const int k = j0 + 8 * (j >> 2) + (j & 3);
+                    x[j] = k > p || k < first ? -INFINITY : x[j];
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 16; ++j) sum[b][j] += exp2_fast(x[j]);
+        }
+    }
+    // ---- over the lanes of a half, then the wavefronts ----------------------------
+    float mine[2] = {0.f, 0.f};                     // lane nl: block b's row nl (both halves of lanes alike)
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            float y = row16_sum(sum[b][j]);
+            const int yi = __builtin_bit_cast(int, y);
+            const auto sw = __builtin_amdgcn_permlane16_swap(yi, yi, false, false);
+            y = __builtin_bit_cast(float, (int)sw[0]) + __builtin_bit_cast(float, (int)sw[1]);
+            // (lanes of half hh now hold row 8 (j / 4) + 4 hh + j % 4)
+            if (nl == 8 * (j >> 2) + 4 * hh + (j & 3)) mine[b] = y;
+        }
+    if (rh == 1) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+            if (((nl >> 2) & 1) == hh) part[ph][32 * b + nl] = mine[b];
+    }
+    __syncthreads();
+    if (rh == 0) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const int j = pos[b] + nl;
+            if (((nl >> 2) & 1) == hh && j < st.n) {
+                const int page = paged_page(a.b, s, j >> lg);
+                if (page >= 0) paged_weight_add(a, page, hk, j & pmask, mine[b] + part[ph][32 * b + nl]);
+            }
+        }
+    }
+}
+
+template <int D>
+static void launch_pw(const WeightsArgs& wa, const dim3& grid, hipStream_t st) {
+    if (wa.a.q_f16) hipLaunchKernelGGL((paged_weights_kernel<D, true>), grid, dim3(256), 0, st, wa);
+    else hipLaunchKernelGGL((paged_weights_kernel<D, false>), grid, dim3(256), 0, st, wa);
 }
 
 hipError_t launch_paged_weights(const PagedAttn& a, int head_dim, hipStream_t st) {
     if (a.b.max_nkv <= 0 || a.b.n_streams <= 0) return hipSuccess;
-    const dim3 grid((unsigned)((a.b.max_nkv + 63) / 64), (unsigned)a.b.n_streams, (unsigned)a.hkv);
-    if (head_dim == 128) hipLaunchKernelGGL((paged_weights_kernel<128>), grid, dim3(64), 0, st, a);
-    else if (head_dim == 64) hipLaunchKernelGGL((paged_weights_kernel<64>), grid, dim3(64), 0, st, a);
+    WeightsArgs wa;
+    wa.a = a;
+    wa.grp = DivMod::make((uint32_t)(a.hq / a.hkv > 0 ? a.hq / a.hkv : 1));
+    wa.ntiles = (int32_t)(((int64_t)a.b.max_nkv + PW_ROWS - 1) / PW_ROWS);
+    if ((int64_t)wa.ntiles * a.hkv > kMaxGridX) return hipErrorInvalidValue;
+    const dim3 grid((unsigned)(wa.ntiles * a.hkv), (unsigned)a.b.n_streams);
+    if (head_dim == 128) launch_pw<128>(wa, grid, st);
+    else if (head_dim == 64) launch_pw<64>(wa, grid, st);
     else return hipErrorInvalidValue;
     return hipGetLastError();
 }

@@ -287,9 +287,10 @@ int vxfa_flash_attn_ext_paged(vxfa_ctx* c, const vxfa_tensor* q, const vxfa_tens
     // few tokens: every row's K and V read by the workgroup of all its query rows
     // (up to 16); else tiles of 32 query rows
     hipError_t e = hipSuccess;
+    bool weighed = false;
     if (T * Hq > 0 && a.b.n_streams > 0)
-        e = vxfa::paged_rows_takes(a) ? vxfa::launch_paged_rows(a, (int)D, st) : vxfa::launch_paged_chunk(a, (int)D, st);
-    if (e == hipSuccess && weights) e = vxfa::launch_paged_weights(a, (int)D, st);
+        e = vxfa::paged_rows_takes(a) ? vxfa::launch_paged_rows(a, (int)D, st, weighed) : vxfa::launch_paged_chunk(a, (int)D, st);
+    if (e == hipSuccess && weights && !weighed) e = vxfa::launch_paged_weights(a, (int)D, st);
     if (e != hipSuccess) return fail(c, VXFA_HIP_ERROR, "paged attention: %s", hipGetErrorString(e));
     return VXFA_OK;
 }
