@@ -35,6 +35,19 @@ __device__ __forceinline__ PagedStream paged_stream(const PagedBatch& b, int s) 
     return r;
 }
 
+// Inclusive sums over the lanes of a wavefront, by DPP shifts within a row of 16
+// lanes and broadcasts of a row's last lane (no LDS round trips).
+__device__ __forceinline__ int wave_scan(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);   // row_shr 1, 2, 4, 8
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);   // row_bcast 15 into rows 1 and 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);   // row_bcast 31 into rows 2 and 3
+    return x;
+}
+__device__ __forceinline__ int wave_sum(int x) { return __builtin_amdgcn_readlane(wave_scan(x), 63); }
+
 // The page of entry i of stream s, or -1 (absent).
 __device__ __forceinline__ int paged_page(const PagedBatch& b, int s, int i) {
     const int p = b.pages[(int64_t)s * b.max_pages + i];
@@ -71,6 +84,7 @@ struct PagedAttn {
     float* lse;               // [token][head] log2 of the sum of the row's 2^x (+inf: no row seen); null: not wanted
     char* ws;                 // scratch
     size_t ws_bytes;
+    int32_t pieces;           // chunks: pieces of the longest walk (0: the plan's choice)
 };
 
 // slope_h * log2(e)
@@ -141,6 +155,7 @@ bool paged_rows_takes(const PagedAttn& a);
 hipError_t launch_paged_rows(const PagedAttn& a, int head_dim, hipStream_t st, bool& weighed);
 // any chunks
 hipError_t launch_paged_chunk(const PagedAttn& a, int head_dim, hipStream_t st);
+hipError_t launch_paged_chunk64(const PagedAttn& a, hipStream_t st);
 hipError_t launch_paged_weights(const PagedAttn& a, int head_dim, hipStream_t st);
 hipError_t launch_paged_evict(const PagedEvict& a, hipStream_t st);
 

@@ -26,18 +26,19 @@ __device__ __forceinline__ uint32_t sel_key(float x) {
     return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 
-__device__ __forceinline__ int sel_scan(int x, int lane) {   // inclusive, over a wavefront
-#pragma unroll
-    for (int w = 1; w < 64; w <<= 1) {
-        const int y = __shfl_up(x, w, 64);
-        if (lane >= w) x += y;
-    }
-    return x;
+// Sum over the wavefronts before this one, and over all, of each one's `total` (all
+// its lanes alike); w: 16 ints of LDS, not read by a slower wavefront any more.
+__device__ __forceinline__ int2 sel_before(int total, int* w, int wave, int lane) {
+    if (lane == 0) w[wave] = total;
+    __syncthreads();
+    const int incl = wave_scan(lane < SEL_NT / 64 ? w[lane] : 0);
+    const int all = __builtin_amdgcn_readlane(incl, SEL_NT / 64 - 1);
+    return int2{wave > 0 ? __builtin_amdgcn_readlane(incl, wave > 0 ? wave - 1 : 0) : 0, all};
 }
 
 __global__ __launch_bounds__(SEL_NT) void paged_select_kernel(PagedEvict a) {
     const int s = (int)blockIdx.x, h = (int)blockIdx.y, tid = (int)threadIdx.x;
-    const int lane = tid & 63, wave = tid >> 6;
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = min(max(a.b.n_kv[s], 0), a.b.max_nkv);
     int32_t* kept = a.kept + ((int64_t)s * a.hkv + h) * a.kept_row;
     if (h == 0 && tid == 0 && a.n_out) a.n_out[s] = min(n, a.budget);
@@ -85,11 +86,8 @@ __global__ __launch_bounds__(SEL_NT) void paged_select_kernel(PagedEvict a) {
             // thread t: bins 2047 - 2 t and the one below, from the top
             const int b1 = SEL_BINS - 1 - 2 * tid;
             const int c1 = (int)hist[b1], c2 = (int)hist[b1 - 1];
-            const int incl = sel_scan(c1 + c2, lane);
-            if (lane == 63) wsum[0][wave] = incl;
-            __syncthreads();
-            int above = incl - c1 - c2;
-            for (int w = 0; w < wave; ++w) above += wsum[0][w];
+            const int incl = wave_scan(c1 + c2);
+            const int above = sel_before(__builtin_amdgcn_readlane(incl, 63), wsum[0], wave, lane).x + incl - c1 - c2;
             if (above < want && above + c1 >= want) {
                 pick[0] = (uint32_t)b1;
                 pick[1] = (uint32_t)(want - above);
@@ -112,14 +110,10 @@ __global__ __launch_bounds__(SEL_NT) void paged_select_kernel(PagedEvict a) {
 #pragma unroll
         for (int i = 0; i < SEL_PER; ++i) eq += any && jt + i >= a.n_sink && jt + i < end && key[i] == prefix;
         __syncthreads();
-        const int ei = sel_scan(eq, lane);
-        if (lane == 63) wsum[0][wave] = ei;
-        __syncthreads();
-        int eb = eq_done + ei - eq;
-        for (int w = 0; w < SEL_NT / 64; ++w) {
-            if (w < wave) eb += wsum[0][w];
-            eq_done += wsum[0][w];
-        }
+        const int ei = wave_scan(eq);
+        const int2 es = sel_before(__builtin_amdgcn_readlane(ei, 63), wsum[0], wave, lane);
+        int eb = eq_done + es.x + ei - eq;
+        eq_done += es.y;
         uint32_t keep = 0;
 #pragma unroll
         for (int i = 0; i < SEL_PER; ++i) {
@@ -129,14 +123,10 @@ __global__ __launch_bounds__(SEL_NT) void paged_select_kernel(PagedEvict a) {
             else if (any && key[i] > prefix) keep |= 1u << i;
             else if (any && key[i] == prefix && eb++ < want) keep |= 1u << i;
         }
-        const int c = __popc(keep), ki = sel_scan(c, lane);
-        if (lane == 63) wsum[1][wave] = ki;
-        __syncthreads();
-        int kb = done + ki - c;
-        for (int w = 0; w < SEL_NT / 64; ++w) {
-            if (w < wave) kb += wsum[1][w];
-            done += wsum[1][w];
-        }
+        const int c = __popc(keep), ki = wave_scan(c);
+        const int2 ks = sel_before(__builtin_amdgcn_readlane(ki, 63), wsum[1], wave, lane);
+        int kb = done + ks.x + ki - c;
+        done += ks.y;
 #pragma unroll
         for (int i = 0; i < SEL_PER; ++i)
             if (((keep >> i) & 1) && kb < a.kept_row) kept[kb++] = jt + i;

@@ -54,12 +54,6 @@ struct Part {
 };
 
 #ifdef __HIPCC__
-__device__ __forceinline__ int wave_sum(int x) {
-#pragma unroll
-    for (int w = 1; w < 64; w <<= 1) x += __shfl_xor(x, w, 64);
-    return x;
-}
-
 // the first row that any of a stream's tokens sees, down to a whole tile
 __device__ __forceinline__ int rows_first(const PagedStream& s, int window) {
     return window > 0 ? max(s.n - s.t - window + 1, 0) & ~15 : 0;
@@ -112,12 +106,7 @@ __device__ __forceinline__ Part rows_locate(const PagedBatch& b, const RowsPlan&
             if (s0 + lane < b.n_streams) s = paged_stream(b, s0 + lane);
         }
         const int n = parts(s, chunk);
-        int incl = n;
-#pragma unroll
-        for (int w = 1; w < 64; w <<= 1) {
-            const int y = __shfl_up(incl, w, 64);
-            if (lane >= w) incl += y;
-        }
+        const int incl = wave_scan(n);
         const uint64_t hit = __ballot(before + incl > item);
         if (hit) {
             const int w = (int)__builtin_ctzll(hit);
@@ -145,6 +134,7 @@ __device__ __forceinline__ Part rows_locate(const PagedBatch& b, const RowsPlan&
 struct ChunkPlan {
     uint32_t hpw_log2;        // log2 of the query heads per workgroup
     int32_t cuts;             // 0: a piece per tile
+    int32_t pieces;           // > 0: pieces of the longest walk (else chunk_choose's)
     int32_t items;            // pieces in the grid per head group
     int32_t tiles;            // tiles of all streams at most (sizes that break the bounds: the rest is left out)
     int32_t room;             // records (of a workgroup's piece) per head group
@@ -159,7 +149,31 @@ struct ChunkBounds {
 };
 constexpr int kChunkStreams = 64;   // more streams are not cut
 
-inline ChunkBounds chunk_plan(const PagedBatch& b, int nhg, int bm, size_t record, size_t ws_bytes, ChunkPlan& p) {
+// A cut's time in blocks of 32 rows: `total` blocks of a head group, in `items`
+// workgroups (of each head group) of `lp` at most. A workgroup costs its blocks
+// and kWg, 256 run at once; a record costs its traffic, and the joining of a
+// walk's pieces goes one after another.
+__host__ __device__ inline float chunk_cost(float total, int items, int recs, int lp, int nhg, int pieces) {
+    constexpr float kWg = 4.f, kRecord = 0.05f, kPiece = 0.3f;
+    const float count = (float)(items * nhg), rounds = ceilf(count * (1.f / 256.f));
+    return fmaxf(rounds * (total * (float)nhg / fmaxf(count, 1.f) + kWg), (float)lp + kWg) + kRecord * (float)(recs * nhg) +
+           (recs ? kPiece * (float)pieces : 0.f);
+}
+// length of the pieces of a walk of nb blocks in n pieces: whole steps
+__host__ __device__ inline int chunk_length(int nb, int n) {
+    const int l = ((nb + n - 1) / n + 1) & ~1;
+    return l > 4 ? l : 4;
+}
+// all blocks of a stream's tiles, the last of which walks nb: one before it walks
+// bm / 32 less, but for a window
+__host__ __device__ inline float chunk_blocks(int tiles, int nb, int bm, int window) {
+    const float all = (float)tiles * (float)nb;
+    if (window > 0) return all;
+    const float less = all - (float)(bm / 32) * 0.5f * (float)tiles * (float)(tiles - 1);
+    return less > (float)tiles ? less : (float)tiles;
+}
+
+inline ChunkBounds chunk_plan(const PagedBatch& b, int nhg, int bm, int window, size_t record, size_t ws_bytes, ChunkPlan& p) {
     ChunkBounds r;
     // sum of ceil(t / bm) over streams of `tokens` tokens in all, max_nq at most each
     const int64_t per = ((int64_t)b.max_nq + bm - 1) / bm;
@@ -172,11 +186,33 @@ inline ChunkBounds chunk_plan(const PagedBatch& b, int nhg, int bm, size_t recor
     p.tiles = (int32_t)r.tiles;
     const int64_t room = r.table < ws_bytes ? (int64_t)((ws_bytes - r.table) / (record * (size_t)nhg)) : 0;
     p.room = (int32_t)(room < 4096 ? room : 4096);
-    // tiles for four rounds of the chip's 256 CUs, or too few rows: not cut
-    p.cuts = r.tiles * nhg < 1024 && b.max_nkv >= 128 && b.n_streams <= kChunkStreams && p.room >= 2;
+    // tiles for two rounds of the chip's 256 CUs (16 streams of up to 512 tokens on up
+    // to 4096 rows, 600 workgroups: uncut 169 us, in halves 172), or too few rows: not cut
+    p.cuts = r.tiles * nhg < 512 && b.max_nkv >= 128 && b.n_streams <= kChunkStreams && p.room >= 2;
     int64_t items = r.tiles;
     if (p.cuts) items = r.tiles > 512 / nhg ? r.tiles : (512 / nhg > 1 ? 512 / nhg : 1);
     if (p.cuts && items < 2) items = 2;
+    if (p.cuts && p.pieces == 0 && b.n_streams == 1) {
+        // one stream, whose sizes are near the bounds: the pieces are chosen here,
+        // and the grid holds no more
+        const int tiles = (int)r.tiles;
+        int64_t nb = ((int64_t)b.max_nkv + 31) / 32;
+        if (window > 0 && nb > ((int64_t)window + bm) / 32 + 1) nb = ((int64_t)window + bm) / 32 + 1;
+        float best = 3.0e38f;
+        p.pieces = 1;
+        for (int n = 1; n <= 64; ++n) {
+            const int lp = chunk_length((int)nb, n), k = n == 1 ? 1 : (int)((nb + lp - 1) / lp), all = k * tiles;
+            if (k > 1 && all > p.room) break;
+            const float cost = chunk_cost(chunk_blocks(tiles, (int)nb, bm, window), all, k > 1 ? all : 0, lp, nhg, k);
+            if (cost < best) {
+                best = cost;
+                p.pieces = k;
+            }
+        }
+    }
+    if (p.pieces > 64) p.pieces = 64;
+    if (p.pieces > 0) items = r.tiles * p.pieces;
+    if (p.pieces == 1) p.cuts = 0;
     p.items = (int32_t)items;
     return r;
 }
@@ -189,16 +225,55 @@ struct ChunkItem {
 };
 
 #ifdef __HIPCC__
-__device__ __forceinline__ int wave_scan(int x, int lane) {   // inclusive
-#pragma unroll
-    for (int w = 1; w < 64; w <<= 1) {
-        const int y = __shfl_up(x, w, 64);
-        if (lane >= w) x += y;
-    }
-    return x;
-}
 // ceil(n / d) of small numbers, the same on every lane
 __device__ __forceinline__ int chunk_pieces(int n, int d) { return (n + d - 1) / d; }
+
+// Up to 64 streams, a lane each: their tiles (none past the last stream), blocks
+// that the longest tile walks, and pieces per tile.
+__device__ __forceinline__ int chunk_choose(const PagedBatch& b, const ChunkPlan& p, int window, int bm, int lane,
+                                            const PagedStream& st, int tiles, int& nb) {
+    // blocks that the last tile walks, which is the longest
+    int lo = 0;
+    if (window > 0) lo = max(st.n - st.t + (tiles - 1) * bm - window + 1, 0) / 32;
+    nb = tiles > 0 ? max((st.n + 31) / 32 - lo, 1) : 0;
+    if (!p.cuts) return 1;
+    // all blocks: a tile before it walks bm / 32 less
+    float total = tiles > 0 ? chunk_blocks(tiles, nb, bm, window) : 0.f;
+    int longest = nb;
+    if (b.n_streams > 1) {
+#pragma unroll
+        for (int w = 1; w < 64; w <<= 1) {
+            longest = max(longest, __shfl_xor(longest, w, 64));
+            total += __shfl_xor(total, w, 64);
+        }
+    } else {
+        longest = __builtin_amdgcn_readfirstlane(longest);
+    }
+    if (p.pieces > 0) {
+        // (those of the longest walk, where their records fit)
+        const int lp = chunk_length(longest, p.pieces), n = max(chunk_pieces(nb, lp), 1);
+        int recs = n > 1 ? n * tiles : 0;
+        if (b.n_streams > 1) recs = wave_sum(recs);
+        else recs = __builtin_amdgcn_readfirstlane(recs);
+        return recs <= p.room ? n : 1;
+    }
+    // this lane's length: the longest walk in lane + 1 pieces
+    const int lp = chunk_length(longest, lane + 1);
+    int items = 0, recs = 0;
+    for (int s = 0; s < b.n_streams; ++s) {
+        const int n = chunk_pieces(__builtin_amdgcn_readlane(nb, s), lp), ts = __builtin_amdgcn_readlane(tiles, s);
+        items += n * ts;
+        recs += n > 1 ? n * ts : 0;
+    }
+    float cost = chunk_cost(total, items, recs, lp, p.nhg, lane + 1);
+    if (items > p.items || recs > p.room) cost = 3.0e38f;
+    if (lane == 0) cost = fminf(cost, 1.0e38f);   // (one piece a tile always fits)
+    float best = cost;
+#pragma unroll
+    for (int w = 1; w < 64; w <<= 1) best = fminf(best, __shfl_xor(best, w, 64));
+    const int pick = (int)__builtin_ctzll(__ballot(cost == best));
+    return pick == 0 ? 1 : max(chunk_pieces(nb, __builtin_amdgcn_readlane(lp, pick)), 1);
+}
 
 __device__ __forceinline__ ChunkItem chunk_locate(const PagedBatch& b, const ChunkPlan& p, int window, int bm, int item) {
     const int lane = (int)threadIdx.x & 63;
@@ -209,67 +284,41 @@ __device__ __forceinline__ ChunkItem chunk_locate(const PagedBatch& b, const Chu
     for (int s0 = 0; s0 < b.n_streams; s0 += 64) {
         PagedStream st{0, 0, 0};
         if (s0 + lane < b.n_streams) st = paged_stream(b, s0 + lane);
-        const int nq = min(st.t, b.max_nq);
-        const int tiles = (nq + bm - 1) / bm;
-        int np = 1;
-        if (p.cuts) {   // (64 streams at most)
-            // blocks that the last tile walks, which is the longest
-            int lo = 0;
-            if (window > 0) lo = max(st.n - st.t + (tiles - 1) * bm - window + 1, 0) / 32;
-            const int nb = tiles > 0 ? max((st.n + 31) / 32 - lo, 1) : 0;
-            // all blocks: a tile before it walks bm / 32 less
-            float work = (float)tiles * (float)nb;
-            if (window <= 0) work = fmaxf(work - (float)(bm / 32) * 0.5f * (float)tiles * (float)(tiles - 1), (float)tiles);
-            float total = work;
-            int longest = nb;
-#pragma unroll
-            for (int w = 1; w < 64; w <<= 1) {
-                longest = max(longest, __shfl_xor(longest, w, 64));
-                total += __shfl_xor(total, w, 64);
-            }
-            // this lane's length: the longest walk in lane + 1 pieces, whole steps
-            const int lp = max((((longest + lane) / (lane + 1)) + 1) & ~1, 2);
-            int items = 0, recs = 0;
-            for (int s = 0; s < b.n_streams; ++s) {
-                const int n = chunk_pieces(__builtin_amdgcn_readlane(nb, s), lp), ts = __builtin_amdgcn_readlane(tiles, s);
-                items += n * ts;
-                recs += n > 1 ? n * ts : 0;
-            }
-            // time in blocks: a workgroup costs its blocks and kWg, 256 run at once;
-            // a record its traffic
-            constexpr float kWg = 4.f, kRecord = 0.05f;
-            const float count = (float)(items * p.nhg), rounds = ceilf(count * (1.f / 256.f));
-            float cost = fmaxf(rounds * (total * (float)p.nhg / fmaxf(count, 1.f) + kWg), (float)lp + kWg) + kRecord * (float)(recs * p.nhg);
-            if (items > p.items || recs > p.room) cost = 3.0e38f;
-            if (lane == 0) cost = fminf(cost, 1.0e38f);   // (one piece a tile always fits)
-            float best = cost;
-#pragma unroll
-            for (int w = 1; w < 64; w <<= 1) best = fminf(best, __shfl_xor(best, w, 64));
-            const int pick = (int)__builtin_ctzll(__ballot(cost == best));
-            np = chunk_pieces(nb, __builtin_amdgcn_readlane(lp, pick));
-            if (pick == 0 || np < 1) np = 1;
+        const int tiles = (min(st.t, b.max_nq) + bm - 1) / bm;
+        int nb, np;
+        np = chunk_choose(b, p, window, bm, lane, st, tiles, nb);
+        // pieces, tiles and records of the streams ahead of the lane's: those of longer
+        // walks (and, of equal ones, the earlier)
+        const int n = tiles * np, rec = np > 1 ? n : 0;
+        int ahead = 0, tahead = 0, rahead = 0, all = 0, tall = 0;
+        for (int s = 0; s < min(b.n_streams - s0, 64); ++s) {
+            const int nbs = __builtin_amdgcn_readlane(nb, s), ns = __builtin_amdgcn_readlane(n, s);
+            const int ts = __builtin_amdgcn_readlane(tiles, s), rs = __builtin_amdgcn_readlane(rec, s);
+            const bool first = nbs > nb || (nbs == nb && s < lane);
+            ahead += first ? ns : 0;
+            tahead += first ? ts : 0;
+            rahead += first ? rs : 0;
+            all += ns;
+            tall += ts;
         }
-        const int n = tiles * np;
-        const int incl = wave_scan(n, lane), tincl = wave_scan(tiles, lane);
-        const int rincl = p.cuts ? wave_scan(np > 1 ? n : 0, lane) : 0;
-        const uint64_t hit = r.s < 0 ? __ballot(before + incl > item) : 0;
+        const int mine = item - before - ahead;
+        const uint64_t hit = r.s < 0 ? __ballot(mine >= 0 && mine < n) : 0;
         if (hit) {
             const int w = (int)__builtin_ctzll(hit);
             r.s = s0 + w;
             r.n = __builtin_amdgcn_readlane(np, w);
-            const int ts = __builtin_amdgcn_readlane(tiles, w);
-            const int i = item - (before + __builtin_amdgcn_readlane(incl, w) - ts * r.n);
+            const int ts = __builtin_amdgcn_readlane(tiles, w), i = __builtin_amdgcn_readlane(mine, w);
             r.tile = ts - 1 - i / r.n;              // the longest first
             r.piece = i % r.n;
-            r.slot = r.n > 1 ? __builtin_amdgcn_readlane(rincl, w) - ts * r.n + (ts - 1 - r.tile) * r.n : 0;
-            r.tile_no = r.tiles + __builtin_amdgcn_readlane(tincl, w) - ts + r.tile;
-            if (r.tile_no >= p.tiles) r.s = -1;
+            r.slot = r.n > 1 ? __builtin_amdgcn_readlane(rahead, w) + (i - r.piece) : 0;
+            r.tile_no = r.tiles + __builtin_amdgcn_readlane(tahead, w) + r.tile;
             r.st.q0 = __builtin_amdgcn_readlane(st.q0, w);
             r.st.t = __builtin_amdgcn_readlane(st.t, w);
             r.st.n = __builtin_amdgcn_readlane(st.n, w);
+            if (r.tile_no >= p.tiles) r.s = -1;
         }
-        before += __builtin_amdgcn_readlane(incl, 63);
-        r.tiles += __builtin_amdgcn_readlane(tincl, 63);
+        before += all;
+        r.tiles += tall;
         if (hit && item > 0) return r;              // (the first one goes on to count the tiles)
     }
     r.tiles = min(r.tiles, p.tiles);

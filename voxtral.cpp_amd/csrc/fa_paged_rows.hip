@@ -327,27 +327,42 @@ __global__ __launch_bounds__(64) void paged_rows_combine(RowsArgs ra) {
 }
 
 // The weights that the rows gather from scores that paged_rows_kernel left: a
-// thread per row and kv head sums 2^(x - lse) over the query rows.
+// thread per 4 rows (of one page) and kv head sums 2^(x - lse) over the query
+// rows.
 __global__ __launch_bounds__(256) void paged_rows_weights(RowsArgs ra) {
     const PagedAttn& a = ra.a;
-    const int s = (int)blockIdx.y, hk = (int)blockIdx.x % a.hkv, j = (int)blockIdx.x / a.hkv * 256 + (int)threadIdx.x;
+    const int s = (int)blockIdx.y, hk = (int)blockIdx.x % a.hkv, j = ((int)blockIdx.x / a.hkv * 256 + (int)threadIdx.x) * 4;
     const PagedStream st = paged_stream(a.b, s);
     if (j >= st.n) return;
     const int page = paged_page(a.b, s, j >> a.b.ps_log2);
     if (page < 0) return;
-    float sum = 0.f;
+    const int left = min(st.n - j, 4), r = j & ((1 << a.b.ps_log2) - 1);
     const int G = a.hq / a.hkv, hpw = (int)ra.hpw.d;
-    if (j >= rows_first(st, a.window)) {
+    const float* wi = a.w_in ? (const float*)((const char*)a.w_in + page * a.wi_nb3 + hk * a.wi_nb2) + r : nullptr;
+    float* wo = (float*)((char*)a.w_out + page * a.wo_nb3 + hk * a.wo_nb2) + r;
+    float old[4] = {0.f, 0.f, 0.f, 0.f};
+    if (wi) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) old[c] = c < left ? wi[c] : 0.f;
+    }
+    floatx4 sum = {0.f, 0.f, 0.f, 0.f};
+    if (j + 3 >= rows_first(st, a.window)) {       // (a multiple of 16, as the tiles are)
         for (int sub = 0; sub < ra.groups; ++sub) {
             const float* x = ra.x + ((int64_t)(hk * ra.groups + sub) * a.b.n_streams + s) * ra.rows * ra.xrow + j;
             const int heads = min(hpw, G - sub * hpw);
             for (int i = 0; i < min(st.t, a.b.max_nq); ++i) {
                 const float* lse = a.lse + (int64_t)(st.q0 + i) * a.hq + hk * G + sub * hpw;
-                for (int h = 0; h < heads; ++h) sum += exp2_fast(x[(int64_t)(i * hpw + h) * ra.xrow] - lse[h]);
+                for (int h = 0; h < heads; ++h) {
+                    const floatx4 y = *(const floatx4*)(x + (int64_t)(i * hpw + h) * ra.xrow);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) sum[c] += exp2_fast(y[c] - lse[h]);
+                }
             }
         }
     }
-    paged_weight_add(a, page, hk, j & ((1 << a.b.ps_log2) - 1), sum);
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+        if (c < left) wo[c] = old[c] + sum[c];
 }
 
 bool paged_rows_takes(const PagedAttn& a) {
@@ -397,7 +412,7 @@ hipError_t launch_paged_rows(const PagedAttn& a, int head_dim, hipStream_t st, b
         if (e != hipSuccess) return e;
     }
     if (!ra.x) return e;
-    const int64_t gx = ((int64_t)a.b.max_nkv + 255) / 256 * a.hkv;
+    const int64_t gx = ((int64_t)a.b.max_nkv + 1023) / 1024 * a.hkv;
     if (gx > kMaxGridX) return hipErrorInvalidValue;
     hipLaunchKernelGGL(paged_rows_weights, dim3((unsigned)gx, (unsigned)a.b.n_streams), dim3(256), 0, st, ra);
     return hipGetLastError();

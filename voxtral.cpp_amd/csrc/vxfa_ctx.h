@@ -35,6 +35,9 @@ struct Tuning {
     // VXFA_ROPE_Q=0: no scratch for rotated queries, as for a call whose rows do
     // not fit it
     bool rope_q = true;
+    // VXFA_PAGED_PIECES: pieces of the longest walk of a paged chunk call (0: the
+    // plan's choice)
+    int paged_pieces = 0;
     void read_env() {
         if (const char* e = getenv("VXFA_DECODE_SPLIT")) split_override = atoi(e);
         if (const char* e = getenv("VXFA_PREFILL_WAVES")) waves_override = atoi(e);
@@ -43,6 +46,7 @@ struct Tuning {
         if (const char* e = getenv("VXFA_PAIR_INTERVALS")) pair_intervals = atoi(e) != 0;
         if (const char* e = getenv("VXFA_ROPE_Q")) rope_q = atoi(e) != 0;
         if (const char* e = getenv("VXFA_PREFILL_GROUP")) group = atoi(e) != 0;
+        if (const char* e = getenv("VXFA_PAGED_PIECES")) paged_pieces = atoi(e);
         if (const char* e = getenv("VXFA_DECODE_ROWS")) decode_rows = atoi(e) != 0;
     }
 };

@@ -265,6 +265,7 @@ int vxfa_flash_attn_ext_paged(vxfa_ctx* c, const vxfa_tensor* q, const vxfa_tens
         a.n2 = (int32_t)n2;
         a.bias1 = -max_bias / (float)n2;
     }
+    a.pieces = c->tune.paged_pieces;
     a.ws = c->ws;
     a.ws_bytes = kWorkspaceBytes;
     if (weights) {
