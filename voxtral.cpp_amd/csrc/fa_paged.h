@@ -7,6 +7,8 @@
 
 #include "fa_common.h"
 
+#include <type_traits>
+
 namespace vxfa {
 
 constexpr int kPagedMinLog2 = 4, kPagedMaxLog2 = 16;   // page sizes 16 .. 65536
@@ -45,6 +47,28 @@ __device__ __forceinline__ int wave_scan(int x) {
     x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);   // row_bcast 15 into rows 1 and 3
     x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);   // row_bcast 31 into rows 2 and 3
     return x;
+}
+// (x >= 0)
+__device__ __forceinline__ float wave_sum(float x) {
+    auto add = [&](auto ctl, auto rows) {
+        x += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(ctl)::value, decltype(rows)::value, 0xF, false));
+    };
+    add(std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xF>{});
+    add(std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xF>{});
+    add(std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xF>{});
+    add(std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xF>{});
+    add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xA>{});
+    add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xC>{});
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
+}
+__device__ __forceinline__ int wave_max(int x) {
+    x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x111, 0xF, 0xF, false));
+    x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x112, 0xF, 0xF, false));
+    x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x114, 0xF, 0xF, false));
+    x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x118, 0xF, 0xF, false));
+    x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x142, 0xA, 0xF, false));
+    x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x143, 0xC, 0xF, false));
+    return __builtin_amdgcn_readlane(x, 63);
 }
 __device__ __forceinline__ int wave_sum(int x) { return __builtin_amdgcn_readlane(wave_scan(x), 63); }
 
@@ -110,12 +134,6 @@ __device__ __forceinline__ void paged_store4(const PagedAttn& a, int64_t at, flo
     } else {
         *(floatx4*)((float*)a.dst + at) = x;
     }
-}
-
-// what row r of a page has gathered from this call, on top of what it had
-__device__ __forceinline__ void paged_weight_add(const PagedAttn& a, int page, int hk, int r, float add) {
-    const float old = a.w_in ? *(const float*)((const char*)a.w_in + page * a.wi_nb3 + hk * a.wi_nb2 + 4 * (int64_t)r) : 0.f;
-    *(float*)((char*)a.w_out + page * a.wo_nb3 + hk * a.wo_nb2 + 4 * (int64_t)r) = old + add;
 }
 
 struct PagedAppend {

@@ -60,19 +60,22 @@ __global__ __launch_bounds__(SEL_NT) void paged_select_kernel(PagedEvict a) {
 #pragma unroll
         for (int i = 0; i < SEL_PER; ++i) key[i] = page >= 0 ? sel_key(x[i]) : 0;
     };
-    __shared__ uint32_t hist[SEL_BINS];
+    __shared__ uint32_t hists[3][SEL_BINS];
+    __shared__ int list[SEL_SEG];
     __shared__ int wsum[2][SEL_NT / 64];
     __shared__ uint32_t pick[2];
+    // (a histogram for each pass, cleared while the first keys are on their way)
+    for (int i = tid; i < 3 * SEL_BINS; i += SEL_NT) (&hists[0][0])[i] = 0;
     const bool one = n <= SEL_SEG;
     if (one) load(0);
+    __syncthreads();
     int want = a.budget - a.n_sink - a.n_recent;   // of the competing rows
     const bool any = want > 0;
     uint32_t prefix = 0;
     if (any) {
         for (int pass = 0; pass < 3; ++pass) {
             const int sh = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bits = pass == 2 ? 10 : 11;
-            for (int i = tid; i < SEL_BINS; i += SEL_NT) hist[i] = 0;
-            __syncthreads();
+            uint32_t* const hist = hists[pass];
             for (int j0 = 0; j0 < n; j0 += SEL_SEG) {
                 if (!one) load(j0);
 #pragma unroll
@@ -98,7 +101,7 @@ __global__ __launch_bounds__(SEL_NT) void paged_select_kernel(PagedEvict a) {
             __syncthreads();
             prefix |= pick[0] << sh;
             want = (int)pick[1];
-            // (hist and pick are written again only after the next barrier but one)
+            // (pick is written again only after the next barrier but one)
         }
     }
     // rows in order; `want` of those with the key `prefix`
@@ -125,11 +128,15 @@ __global__ __launch_bounds__(SEL_NT) void paged_select_kernel(PagedEvict a) {
         }
         const int c = __popc(keep), ki = wave_scan(c);
         const int2 ks = sel_before(__builtin_amdgcn_readlane(ki, 63), wsum[1], wave, lane);
-        int kb = done + ks.x + ki - c;
-        done += ks.y;
+        // through LDS, so that the list is written in whole lines
+        int kb = ks.x + ki - c;
 #pragma unroll
         for (int i = 0; i < SEL_PER; ++i)
-            if (((keep >> i) & 1) && kb < a.kept_row) kept[kb++] = jt + i;
+            if ((keep >> i) & 1) list[kb++] = jt + i;
+        __syncthreads();
+        for (int r = tid; r < ks.y; r += SEL_NT)
+            if (done + r < a.kept_row) kept[done + r] = list[r];
+        done += ks.y;
     }
     for (int r = done + tid; r < a.kept_row; r += SEL_NT) kept[r] = -1;
 }

@@ -27,11 +27,12 @@ inline RowsPlan rows_plan(const PagedBatch& b, int nhg, int64_t room, int32_t& i
     p.small = 512 / nhg > 0 ? 512 / nhg : 1;
     p.large = 2048 / nhg > 0 ? 2048 / nhg : 1;
     p.limit = 512;
-    // with n parts' worth of rows, streams of their own rounding: n + streams at most
+    // n parts' worth of rows are at most n parts of one stream, n + streams of more
+    const int64_t more = b.n_streams > 1 ? b.n_streams : 0;
     const int64_t all = (int64_t)b.n_streams * b.max_nkv;
     if (all <= (int64_t)p.small * p.limit) p.large = p.small;
     p.cuts = 1;
-    while (p.cuts && (int64_t)p.large + b.n_streams > room) {
+    while (p.cuts && (int64_t)p.large + more > room) {
         if (p.large > 64) p.large /= 2;
         else p.cuts = 0;
     }
@@ -40,7 +41,7 @@ inline RowsPlan rows_plan(const PagedBatch& b, int nhg, int64_t room, int32_t& i
     items = b.n_streams;
     if (p.cuts) {
         const int64_t by_rows = (int64_t)b.n_streams * ((b.max_nkv + 63) / 64);
-        const int64_t by_parts = (int64_t)p.large + b.n_streams;
+        const int64_t by_parts = (int64_t)p.large + more;
         items = (int32_t)(by_rows < by_parts ? by_rows : by_parts);
     }
     return p;
@@ -225,8 +226,10 @@ struct ChunkItem {
 };
 
 #ifdef __HIPCC__
-// ceil(n / d) of small numbers, the same on every lane
-__device__ __forceinline__ int chunk_pieces(int n, int d) { return (n + d - 1) / d; }
+// pieces of at most 1 / inv blocks of a walk of nb, nb > 0: ceil(nb / lp) (exact
+// for fewer than 2^20 blocks, the half keeping clear of the steps; beyond, one
+// more or less does no harm)
+__device__ __forceinline__ int chunk_pieces(int nb, int lp, float inv) { return (int)(((float)(nb + lp - 1) + 0.5f) * inv); }
 
 // Up to 64 streams, a lane each: their tiles (none past the last stream), blocks
 // that the longest tile walks, and pieces per tile.
@@ -241,38 +244,36 @@ __device__ __forceinline__ int chunk_choose(const PagedBatch& b, const ChunkPlan
     float total = tiles > 0 ? chunk_blocks(tiles, nb, bm, window) : 0.f;
     int longest = nb;
     if (b.n_streams > 1) {
-#pragma unroll
-        for (int w = 1; w < 64; w <<= 1) {
-            longest = max(longest, __shfl_xor(longest, w, 64));
-            total += __shfl_xor(total, w, 64);
-        }
+        longest = wave_max(longest);
+        total = wave_sum(total);
     } else {
         longest = __builtin_amdgcn_readfirstlane(longest);
     }
     if (p.pieces > 0) {
         // (those of the longest walk, where their records fit)
-        const int lp = chunk_length(longest, p.pieces), n = max(chunk_pieces(nb, lp), 1);
+        const int lp = chunk_length(longest, p.pieces), n = max((nb + lp - 1) / lp, 1);
         int recs = n > 1 ? n * tiles : 0;
         if (b.n_streams > 1) recs = wave_sum(recs);
         else recs = __builtin_amdgcn_readfirstlane(recs);
         return recs <= p.room ? n : 1;
     }
-    // this lane's length: the longest walk in lane + 1 pieces
-    const int lp = chunk_length(longest, lane + 1);
+    // this lane's length, from the longest walk down to a 64th of it
+    const int lp = lane == 0 ? longest : max((int)((uint32_t)longest * (uint32_t)(64 - lane) >> 6) & ~1, 4);
+    const float inv = __builtin_amdgcn_rcpf((float)max(lp, 1));
     int items = 0, recs = 0;
     for (int s = 0; s < b.n_streams; ++s) {
-        const int n = chunk_pieces(__builtin_amdgcn_readlane(nb, s), lp), ts = __builtin_amdgcn_readlane(tiles, s);
+        const int n = chunk_pieces(__builtin_amdgcn_readlane(nb, s), lp, inv), ts = __builtin_amdgcn_readlane(tiles, s);
         items += n * ts;
         recs += n > 1 ? n * ts : 0;
     }
-    float cost = chunk_cost(total, items, recs, lp, p.nhg, lane + 1);
+    float cost = chunk_cost(total, items, recs, lp, p.nhg, chunk_pieces(longest, lp, inv));
     if (items > p.items || recs > p.room) cost = 3.0e38f;
     if (lane == 0) cost = fminf(cost, 1.0e38f);   // (one piece a tile always fits)
-    float best = cost;
-#pragma unroll
-    for (int w = 1; w < 64; w <<= 1) best = fminf(best, __shfl_xor(best, w, 64));
+    // (costs are positive: they order as integers)
+    const float best = __builtin_bit_cast(float, -wave_max(-__builtin_bit_cast(int, cost)));
     const int pick = (int)__builtin_ctzll(__ballot(cost == best));
-    return pick == 0 ? 1 : max(chunk_pieces(nb, __builtin_amdgcn_readlane(lp, pick)), 1);
+    const float inv_pick = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, inv), pick));
+    return pick == 0 ? 1 : max(chunk_pieces(nb, __builtin_amdgcn_readlane(lp, pick), inv_pick), 1);
 }
 
 __device__ __forceinline__ ChunkItem chunk_locate(const PagedBatch& b, const ChunkPlan& p, int window, int bm, int item) {

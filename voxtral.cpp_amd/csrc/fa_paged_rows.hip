@@ -277,19 +277,22 @@ __global__ __launch_bounds__(64) void paged_rows_combine(RowsArgs ra) {
     const int g = rest / (D / 32), sl = rest % (D / 32);
     const int i = (int)blockIdx.y, s = (int)blockIdx.z;
     const PagedStream st = paged_stream(a.b, s);
-    if (i >= min(st.t, a.b.max_nq)) return;
+    // (one stream's parts begin at 0: its records are on their way before their number
+    // is known)
+    const bool one = a.b.n_streams == 1;
     const int2 cut = ra.cut[s];
-    if (cut.y <= 1) return;
+    if (!one && (i >= min(st.t, a.b.max_nq) || cut.y <= 1)) return;
+    const int first = one ? 0 : cut.x, nload = one ? ra.items : cut.y;
     const int sub = (int)ra.hpw.div((uint32_t)g), r = i * (int)ra.hpw.d + g - sub * (int)ra.hpw.d;
-    const float* rec = ra.recs + ((int64_t)(hk * ra.groups + sub) * ra.items + cut.x) * ra.rec;
+    const float* rec = ra.recs + ((int64_t)(hk * ra.groups + sub) * ra.items + first) * ra.rec;
     float M = -INFINITY, L = 0.f;
     floatx4 x = {0.f, 0.f, 0.f, 0.f};
-    for (int p0 = grp; p0 < cut.y; p0 += 64) {
+    for (int p0 = grp; p0 < nload; p0 += 64) {
         float m[8], l[8];
         floatx4 o[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
-            const float* q = rec + (int64_t)min(p0 + 8 * u, cut.y - 1) * ra.rec;
+            const float* q = rec + (int64_t)min(p0 + 8 * u, nload - 1) * ra.rec;
             o[u] = *(const floatx4*)(q + r * D + 32 * sl + 4 * f);
             m[u] = q[ra.rows * D + r];
             l[u] = q[ra.rows * (D + 1) + r];
@@ -297,7 +300,11 @@ __global__ __launch_bounds__(64) void paged_rows_combine(RowsArgs ra) {
         float mn = M;
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
-            if (p0 + 8 * u >= cut.y) m[u] = -INFINITY;
+            if (p0 + 8 * u >= cut.y) {   // (what is loaded there may be anything)
+                m[u] = -INFINITY;
+                l[u] = 0.f;
+                o[u] = floatx4{0.f, 0.f, 0.f, 0.f};
+            }
             mn = fmaxf(mn, m[u]);
         }
         const float ms = mn == -INFINITY ? 0.f : mn, al = exp2_fast(M - ms);
@@ -312,6 +319,7 @@ __global__ __launch_bounds__(64) void paged_rows_combine(RowsArgs ra) {
             for (int c = 0; c < 4; ++c) x[c] = fmaf(w, o[u][c], x[c]);
         }
     }
+    if (one && (i >= min(st.t, a.b.max_nq) || cut.y <= 1)) return;
     const float mm = quad_max(fmaxf(M, row_ror<8>(M))), ms = mm == -INFINITY ? 0.f : mm;
     const float w = exp2_fast(M - ms);
     auto all = [](float y) { return quad_sum(y + row_ror<8>(y)); };

@@ -26,8 +26,9 @@ struct WeightsArgs {
     int32_t ntiles;           // row tiles of a stream at most
 };
 
-template <int D, bool QF16>
-__global__ __launch_bounds__(256, 2) void paged_weights_kernel(WeightsArgs wa) {
+// MOD: the scores have a cap or a distance term
+template <int D, bool QF16, bool MOD>
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void paged_weights_kernel(WeightsArgs wa) {
     constexpr int KS = D / 16, ROW = 2 * D, CH = D / 8;
     constexpr int STEP = 64 * ROW;                  // bytes of 64 query rows
     __shared__ __attribute__((aligned(16))) char smem[2 * STEP];
@@ -42,29 +43,35 @@ __global__ __launch_bounds__(256, 2) void paged_weights_kernel(WeightsArgs wa) {
     const int lg = a.b.ps_log2, pmask = (1 << lg) - 1;
     const int G = (int)wa.grp.d, nq = min(st.t, a.b.max_nq), past = st.n - st.t;
 
-    // ---- K: A operand, row nl of a block, dims 16 ks + 8 hh .. (rows that are not
-    // there: zeros) ------------------------------------------------------------------
-    half8 kr[2][KS];
-    int pos[2];
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-        pos[b] = kv0 + 64 * ph + 32 * b;
-        const int j = pos[b] + nl;
-        const int page = j < st.n ? paged_page(a.b, s, j >> lg) : -1;
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) kr[b][ks] = half8{};
-        if (page >= 0) {
-            const char* p = a.k.base + page * a.k.nb3 + (int64_t)hk * a.k.nb2 + (int64_t)(j & pmask) * a.k.nb1 + 16 * hh;
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) kr[b][ks] = *(const half8*)(p + 32 * ks);
-        }
-    }
-
     // ---- query rows (token G + head) that see some of the rows -----------------
     const int t0 = min(max(kv0 - past, 0), nq);
     int t1 = nq;
     if (a.window > 0) t1 = min((int)min((int64_t)kv0 + PW_ROWS - 1 + a.window - past, (int64_t)nq), nq);
     const int r_begin = t0 * G, r_end = max(t1, t0) * G;
+
+    // ---- K: A operand, row nl of a block, dims 16 ks + 8 hh .. (rows that are not
+    // there: zeros) ------------------------------------------------------------------
+    half8 kr[2][KS];
+    int pos[2], pages[2];
+    float old[2] = {0.f, 0.f};                     // what the lane's rows have gathered so far
+    const bool writes = rh == 0 && ((nl >> 2) & 1) == hh;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+        pos[b] = kv0 + 64 * ph + 32 * b;
+        const int j = pos[b] + nl;
+        const int page = j < st.n ? paged_page(a.b, s, j >> lg) : -1;
+        pages[b] = page;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) kr[b][ks] = half8{};
+        if (page >= 0 && r_begin < r_end) {
+            const char* p = a.k.base + page * a.k.nb3 + (int64_t)hk * a.k.nb2 + (int64_t)(j & pmask) * a.k.nb1 + 16 * hh;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) kr[b][ks] = *(const half8*)(p + 32 * ks);
+        }
+        if (page >= 0 && writes && a.w_in)
+            old[b] = *(const float*)((const char*)a.w_in + page * a.wi_nb3 + hk * a.wi_nb2 + 4 * (int64_t)(j & pmask));
+    }
+
     constexpr int QN = QF16 ? 64 * CH / 256 : 2 * 64 * CH / 256;   // 16-byte loads of a thread
     constexpr int QC = QF16 ? CH : 2 * CH;                          // of a row
     floatx4 qraw[QN];
@@ -98,19 +105,31 @@ __global__ __launch_bounds__(256, 2) void paged_weights_kernel(WeightsArgs wa) {
 #pragma unroll
         for (int j = 0; j < 16; ++j) sum[b][j] = 0.f;
 
-    const bool mod = a.cap != 0.f || a.bias1 != 0.f;
-    if (r_begin < r_end) load_q(r_begin);
+    // a step's query row of the lane: its token, head and lse
+    auto row_of = [&](int r0, int& tk, int& h) -> float {
+        const int r = r0 + 32 * rh + nl, rc = min(r, r_end - 1);
+        tk = (int)wa.grp.div((uint32_t)rc);
+        h = hk * G + rc - tk * G;
+        const float lse = a.lse[(int64_t)(st.q0 + tk) * a.hq + h];
+        return r < r_end ? lse : INFINITY;          // (weight 0)
+    };
+    int tk = 0, h = 0;
+    float lse = 0.f;
+    if (r_begin < r_end) {
+        load_q(r_begin);
+        lse = row_of(r_begin, tk, h);
+    }
     for (int r0 = r_begin, buf = 0; r0 < r_end; r0 += 64, buf ^= 1) {
         put_q(buf);
-        // this lane's query row
-        const int r = r0 + 32 * rh + nl, rc = min(r, r_end - 1);
-        const int tk = (int)wa.grp.div((uint32_t)rc), h = hk * G + rc - tk * G;
-        float lse = a.lse[(int64_t)(st.q0 + tk) * a.hq + h];
-        if (r >= r_end) lse = INFINITY;             // (weight 0)
-        if (r0 + 64 < r_end) load_q(r0 + 64);
+        const int tk_now = tk, h_now = h;
+        const float lse_now = lse;
+        if (r0 + 64 < r_end) {
+            load_q(r0 + 64);
+            lse = row_of(r0 + 64, tk, h);
+        }
         __syncthreads();                            // (the other buffer is read until the next one)
-        const int p = past + tk, first = a.window > 0 ? p - a.window + 1 : INT32_MIN;
-        const float slope = mod ? paged_slope(a, h) : 0.f;
+        const int p = past + tk_now, first = a.window > 0 ? p - a.window + 1 : INT32_MIN;
+        const float slope = MOD ? paged_slope(a, h_now) : 0.f;
         half8 qb[KS];
         const char* row = smem + buf * STEP + (32 * rh + nl) * ROW;
 #pragma unroll
@@ -122,13 +141,13 @@ __global__ __launch_bounds__(256, 2) void paged_weights_kernel(WeightsArgs wa) {
             for (int ks = 0; ks < KS; ++ks) x = __builtin_amdgcn_mfma_f32_32x32x16_f16(kr[b][ks], qb[ks], x, 0, 0, 0);
             // element j: row pos + 8 (j / 4) + 4 hh + j % 4
             const int j0 = pos[b] + 4 * hh;
-            if (mod) {
+            if constexpr (MOD) {
 #pragma unroll
                 for (int j = 0; j < 16; ++j)
-                    x[j] = fmaf(slope, (float)(j0 + 8 * (j >> 2) + (j & 3) - p), paged_score(x[j], a.c, a.cap)) - lse;
+                    x[j] = fmaf(slope, (float)(j0 + 8 * (j >> 2) + (j & 3) - p), paged_score(x[j], a.c, a.cap)) - lse_now;
             } else {
 #pragma unroll
-                for (int j = 0; j < 16; ++j) x[j] = fmaf(a.c, x[j], -lse);
+                for (int j = 0; j < 16; ++j) x[j] = fmaf(a.c, x[j], -lse_now);
             }
             // (a block that all the wavefront's query rows see whole needs no mask)
             if (__any(pos[b] + 31 > p || pos[b] < first)) {
@@ -140,6 +159,7 @@ __global__ __launch_bounds__(256, 2) void paged_weights_kernel(WeightsArgs wa) {
             }
 #pragma unroll
             for (int j = 0; j < 16; ++j) sum[b][j] += exp2_fast(x[j]);
+            __builtin_amdgcn_sched_barrier(0);      // (one block's scores at a time: registers)
         }
     }
     // ---- over the lanes of a half, then the wavefronts ----------------------------
@@ -161,22 +181,25 @@ __global__ __launch_bounds__(256, 2) void paged_weights_kernel(WeightsArgs wa) {
             if (((nl >> 2) & 1) == hh) part[ph][32 * b + nl] = mine[b];
     }
     __syncthreads();
-    if (rh == 0) {
+    if (writes) {
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            const int j = pos[b] + nl;
-            if (((nl >> 2) & 1) == hh && j < st.n) {
-                const int page = paged_page(a.b, s, j >> lg);
-                if (page >= 0) paged_weight_add(a, page, hk, j & pmask, mine[b] + part[ph][32 * b + nl]);
-            }
-        }
+        for (int b = 0; b < 2; ++b)
+            if (pages[b] >= 0)
+                *(float*)((char*)a.w_out + pages[b] * a.wo_nb3 + hk * a.wo_nb2 + 4 * (int64_t)((pos[b] + nl) & pmask)) =
+                    old[b] + (mine[b] + part[ph][32 * b + nl]);
     }
 }
 
 template <int D>
 static void launch_pw(const WeightsArgs& wa, const dim3& grid, hipStream_t st) {
-    if (wa.a.q_f16) hipLaunchKernelGGL((paged_weights_kernel<D, true>), grid, dim3(256), 0, st, wa);
-    else hipLaunchKernelGGL((paged_weights_kernel<D, false>), grid, dim3(256), 0, st, wa);
+    const bool mod = wa.a.cap != 0.f || wa.a.bias1 != 0.f;
+    if (wa.a.q_f16) {
+        if (mod) hipLaunchKernelGGL((paged_weights_kernel<D, true, true>), grid, dim3(256), 0, st, wa);
+        else hipLaunchKernelGGL((paged_weights_kernel<D, true, false>), grid, dim3(256), 0, st, wa);
+    } else {
+        if (mod) hipLaunchKernelGGL((paged_weights_kernel<D, false, true>), grid, dim3(256), 0, st, wa);
+        else hipLaunchKernelGGL((paged_weights_kernel<D, false, false>), grid, dim3(256), 0, st, wa);
+    }
 }
 
 hipError_t launch_paged_weights(const PagedAttn& a, int head_dim, hipStream_t st) {
