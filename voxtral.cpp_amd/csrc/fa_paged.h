@@ -78,18 +78,18 @@ __device__ __forceinline__ int paged_page(const PagedBatch& b, int s, int i) {
     return (uint32_t)p < (uint32_t)b.n_pages ? p : -1;
 }
 
-// One matrix of the pool: row r of head h in page p at
-// base + p * nb3 + h * nb2 + r * nb1.
+// The pool: row r of head h in page p lies at (of K) or (of V) + at(p, h, r).
 struct PagedPool {
-    char* base;
+    char *k, *v;
     int64_t nb1, nb2, nb3;
+    __device__ __forceinline__ int64_t at(int page, int h, int r) const { return page * nb3 + h * nb2 + r * nb1; }
 };
 
 struct PagedAttn {
     PagedBatch b;
     const void* q;            // [token][head][D], F16 or F32
     int64_t q_nb1, q_nb2;     // bytes between tokens, heads
-    PagedPool k, v;
+    PagedPool kv;
     void* dst;                // [token][head][D], F16 or F32
     uint8_t q_f16, dst_f16;
     int32_t hq, hkv, window;
@@ -141,7 +141,7 @@ struct PagedAppend {
     const float* k_new;       // [token][Hkv D]
     const float* v_new;
     int64_t kn_nb1, vn_nb1;
-    PagedPool k, v;
+    PagedPool kv;
     int32_t d, hq, hkv;
     const int32_t* rope_pos;  // [token]; null: no rotation
     float rope_ts;
@@ -154,7 +154,7 @@ struct PagedAppend {
 
 struct PagedEvict {
     PagedBatch b;
-    PagedPool k, v;
+    PagedPool kv;
     char* w;                  // weights [row of the page] at w + page nb3 + head nb2
     int64_t w_nb2, w_nb3;
     int32_t d, hkv;

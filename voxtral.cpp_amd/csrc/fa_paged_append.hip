@@ -30,7 +30,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppend a) {
     }
     const int row = s.n - s.t + i;
     const int page = row >= 0 ? paged_page(a.b, lo, row >> a.b.ps_log2) : -1;
-    const int64_t r = row & ((1 << a.b.ps_log2) - 1);
+    const int r = row & ((1 << a.b.ps_log2) - 1);
     const int per = a.hkv * a.d / 8, perq = a.q ? a.hq * a.d / 8 : 0;
     for (int c = (int)threadIdx.x; c < 2 * per + perq; c += 256) {
         const int m = c < per ? 0 : (c < 2 * per ? 1 : 2);   // K, V, Q
@@ -46,9 +46,8 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppend a) {
         half8 y;
 #pragma unroll
         for (int j = 0; j < 8; ++j) y[j] = (_Float16)x[j];
-        const PagedPool& pool = m == 0 ? a.k : a.v;
         char* dst = m == 2 ? (char*)a.q_out + (int64_t)t * a.qo_nb1 + (int64_t)h * a.qo_nb2
-                           : pool.base + page * pool.nb3 + (int64_t)h * pool.nb2 + r * pool.nb1;
+                           : (m == 0 ? a.kv.k : a.kv.v) + a.kv.at(page, h, r);
         *(half8*)(dst + 2 * d) = y;
     }
 }

@@ -142,50 +142,79 @@ __global__ __launch_bounds__(PC<HD>::NT, 2) void paged_chunk_kernel(ChunkArgs ca
     static_assert(2 * NW * RPI == 2 * BK && 16 % RPI == 0, "two instructions per matrix and step, rows of a granule");
     const int nstep = (nb + 1) >> 1;
     const int lg = a.b.ps_log2;
-    // lane l: the page of granule l of the 16 steps from ids_from on; bit l: it is there
-    int ids = 0, ids_from = 0;
-    uint64_t there = 0, there_before = 0;
     // (step u and block t count in the order of the walk)
     auto step_row = [&](int u) -> int { return (bs + 2 * (REV ? nstep - 1 - u : u)) * BK; };
     auto block_row = [&](int t) -> int { return step_row(t >> 1) + (REV ? 1 - (t & 1) : t & 1) * BK; };
     auto block_lds = [&](int t) -> int { return (REV ? (t ^ 1) : t) & (2 * NS - 1); };
+    // lane l: where granule l of the 16 steps from ids_from on lies from K's and V's
+    // bases (the page's part worked out here, 64 lanes at once: the products on the
+    // scalar unit cost every wavefront 6 % of its issue slots); bit l of `there`: it is
+    // there (and of the 16 steps before, which may not all be computed yet)
+    int64_t offs = -1;
+    int ids_from = 0;
+    uint64_t there = 0, there_before = 0;
     auto load_ids = [&](int u0) {
         const int u = u0 + (lane >> 2), row = step_row(u) + 16 * (lane & 3);
         const int p = u < nstep && row < st.n ? paged_page(a.b, it.s, row >> lg) : -1;
-        ids = p;
+        offs = p >= 0 ? a.kv.at(p, hk, row & ((1 << lg) - 1)) : -1;
         there_before = there;
         there = __ballot(p >= 0);
         ids_from = u0;
     };
     const uint32_t lds0 = lds_offset(smem);
     const int lrow = lane / CH;
+    uint32_t ldk[2], ldv[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int r = RPI * (wave + NW * i) + lrow;
+        ldk[i] = (uint32_t)(r & 15) * (uint32_t)a.kv.nb1 + ((lane % CH) ^ swz_k<D>(r)) * 16;
+        ldv[i] = (uint32_t)(r & 15) * (uint32_t)a.kv.nb1 + ((lane % CH) ^ swz_v<D>(r)) * 16;
+    }
     auto issue = [&](int u) {
         if ((u & 15) == 0) load_ids(u);
         const int kv0 = step_row(u);
         const uint32_t kd = lds0 + (u & (NS - 1)) * STEP, vd = kd + NS * STEP;
         const char *kp[2], *vp[2];
-        uint32_t ok[2], ov[2];
+        bool plain = kv0 + 2 * BK <= st.n;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const int rs = RPI * (wave + NW * i);                 // the instruction's first row of the step
-            const int page = __builtin_amdgcn_readlane(ids, 4 * (u & 15) + rs / 16);
-            const int r = rs + lrow;
-            ok[i] = ((lane % CH) ^ swz_k<D>(r)) * 16;
-            ov[i] = ((lane % CH) ^ swz_v<D>(r)) * 16;
-            kp[i] = vp[i] = pc_zeros;
-            if (page >= 0 && kv0 + rs < st.n) {
-                const int64_t r_page = (kv0 + rs) & ((1 << lg) - 1);
-                kp[i] = a.k.base + page * a.k.nb3 + (int64_t)hk * a.k.nb2 + r_page * a.k.nb1;
-                vp[i] = a.v.base + page * a.v.nb3 + (int64_t)hk * a.v.nb2 + r_page * a.v.nb1;
-                const uint32_t rr = (uint32_t)min(lrow, st.n - 1 - kv0 - rs);   // rows past the end read the last one
-                ok[i] += rr * (uint32_t)a.k.nb1;
-                ov[i] += rr * (uint32_t)a.v.nb1;
-            }
+            const int g = 4 * (u & 15) + RPI * (wave + NW * i) / 16;
+            const int lo = __builtin_amdgcn_readlane((int)(uint32_t)offs, g), hi = __builtin_amdgcn_readlane((int)(offs >> 32), g);
+            const int64_t at = ((int64_t)hi << 32) | (uint32_t)lo;
+            plain = plain && hi >= 0;
+            kp[i] = a.kv.k + at;
+            vp[i] = a.kv.v + at;
         }
+        if (plain) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) dma16(kp[i], ok[i], kd + RPI * (wave + NW * i) * ROW);
+            for (int i = 0; i < 2; ++i) dma16(kp[i], ldk[i], kd + RPI * (wave + NW * i) * ROW);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) dma16(vp[i], ov[i], vd + RPI * (wave + NW * i) * ROW);
+            for (int i = 0; i < 2; ++i) dma16(vp[i], ldv[i], vd + RPI * (wave + NW * i) * ROW);
+        } else {
+            // rows of zeros in place of an absent granule and behind the last row, whose
+            // own instruction reads it for those behind it (worked out here rather than
+            // held across the loop; the empty asm keeps it here)
+            int ln = lane;
+            asm volatile("" : "+v"(ln));
+            uint32_t ok[2], ov[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int rs = RPI * (wave + NW * i), r = rs + ln / CH;
+                ok[i] = ((ln % CH) ^ swz_k<D>(r)) * 16;
+                ov[i] = ((ln % CH) ^ swz_v<D>(r)) * 16;
+                if (__builtin_amdgcn_readlane((int)(offs >> 32), 4 * (u & 15) + rs / 16) < 0 || kv0 + rs >= st.n) {
+                    kp[i] = vp[i] = pc_zeros;
+                } else {
+                    const uint32_t rr = (uint32_t)min(r & 15, (st.n - 1 - kv0) - (rs & ~15)) * (uint32_t)a.kv.nb1;
+                    ok[i] += rr;
+                    ov[i] += rr;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) dma16(kp[i], ok[i], kd + RPI * (wave + NW * i) * ROW);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) dma16(vp[i], ov[i], vd + RPI * (wave + NW * i) * ROW);
+        }
     };
     for (int u = 0; u < min(nstep, 2); ++u) issue(u);
 

@@ -149,8 +149,7 @@ __global__ __launch_bounds__(256) void paged_move_kernel(PagedEvict a) {
     const int h = (int)blockIdx.x % a.hkv, r0 = ((int)blockIdx.x / a.hkv * 4 + wave) * 8, s = (int)blockIdx.y;
     const int lg = a.b.ps_log2, mask = (1 << lg) - 1;
     const int32_t* kept = a.kept + ((int64_t)s * a.hkv + h) * a.kept_row;
-    const PagedPool& pool = (lane / CH) & 1 ? a.v : a.k;
-    const int64_t col = 16 * (lane % CH) + h * pool.nb2;
+    char* const pool = ((lane / CH) & 1 ? a.kv.v : a.kv.k) + 16 * (lane % CH);
     int j[U], to[U], from[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -168,7 +167,7 @@ __global__ __launch_bounds__(256) void paged_move_kernel(PagedEvict a) {
         x[u] = u32x4{0, 0, 0, 0};
         w[u] = __builtin_nanf("");
         if (from[u] >= 0) {
-            x[u] = __builtin_nontemporal_load((const u32x4*)(pool.base + from[u] * pool.nb3 + (j[u] & mask) * pool.nb1 + col));
+            x[u] = __builtin_nontemporal_load((const u32x4*)(pool + a.kv.at(from[u], h, j[u] & mask)));
             if (lane % (2 * CH) == 0) w[u] = *(const float*)(a.w + from[u] * a.w_nb3 + h * a.w_nb2 + 4 * (j[u] & mask));
         }
     }
@@ -176,7 +175,7 @@ __global__ __launch_bounds__(256) void paged_move_kernel(PagedEvict a) {
     for (int u = 0; u < U; ++u) {
         const int r = r0 + RPW * u + lane / (2 * CH);
         if (j[u] < 0 || to[u] < 0) continue;
-        *(u32x4*)(pool.base + to[u] * pool.nb3 + (r & mask) * pool.nb1 + col) = x[u];
+        *(u32x4*)(pool + a.kv.at(to[u], h, r & mask)) = x[u];
         if (lane % (2 * CH) == 0) *(float*)(a.w + to[u] * a.w_nb3 + h * a.w_nb2 + 4 * (r & mask)) = w[u];
     }
 }

@@ -143,19 +143,18 @@ __global__ __launch_bounds__(64 * PR_WAVES, 2) void paged_rows_kernel(RowsArgs r
         const int page = max(__builtin_amdgcn_readlane(ids, k & 63), 0);   // (absent: page 0, not used)
         const int j0 = part.lo + PR_TILE * (tb + wave + PR_WAVES * k);
         const int last = min(st.n - 1 - j0, PR_TILE - 1);                  // rows past the stream read its last one
-        const int64_t r0 = j0 & ((1 << lg) - 1);
-        const char* kp = a.k.base + page * a.k.nb3 + (int64_t)hk * a.k.nb2 + r0 * a.k.nb1;
-        const char* vp = a.v.base + page * a.v.nb3 + (int64_t)hk * a.v.nb2 + r0 * a.v.nb1;
+        const int64_t at = a.kv.at(page, hk, j0 & ((1 << lg) - 1));
+        const char *kp = a.kv.k + at, *vp = a.kv.v + at;
         const uint32_t slot = lds0 + (k & (NS - 1)) * TILE;
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
             const int r = RPI * i + lane / CH, c = lane % CH;
-            dma16(kp, (uint32_t)min(r, last) * (uint32_t)a.k.nb1 + ((c ^ swk(r)) * 16), slot + RPI * i * ROW);
+            dma16(kp, (uint32_t)min(r, last) * (uint32_t)a.kv.nb1 + ((c ^ swk(r)) * 16), slot + RPI * i * ROW);
         }
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
             const int r = RPI * i + lane / CH, c = lane % CH;
-            dma16(vp, (uint32_t)min(r, last) * (uint32_t)a.v.nb1 + ((c ^ swv(r)) * 16), slot + MAT + RPI * i * ROW);
+            dma16(vp, (uint32_t)min(r, last) * (uint32_t)a.kv.nb1 + ((c ^ swv(r)) * 16), slot + MAT + RPI * i * ROW);
         }
     };
     for (int k = 0; k < min(nk, NS - 1); ++k) issue(k);

@@ -64,7 +64,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void paged_weights_kernel(Wei
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) kr[b][ks] = half8{};
         if (page >= 0 && r_begin < r_end) {
-            const char* p = a.k.base + page * a.k.nb3 + (int64_t)hk * a.k.nb2 + (int64_t)(j & pmask) * a.k.nb1 + 16 * hh;
+            const char* p = a.kv.k + a.kv.at(page, hk, j & pmask) + 16 * hh;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) kr[b][ks] = *(const half8*)(p + 32 * ks);
         }

@@ -75,6 +75,8 @@ int check_pool(const vxfa_tensor* k, const vxfa_tensor* v, const vxfa_paged* b, 
         *why = "k/v row stride must be below 8 MiB";
         return VXFA_UNSUPPORTED;
     }
+    for (int d = 1; d < 4; ++d)
+        if (k->nb[d] != v->nb[d]) { *why = "k and v pools must have the same strides"; return VXFA_UNSUPPORTED; }
     if (!vector_rows(k, 2, 4) || !vector_rows(v, 2, 4)) {
         *why = "pool rows must be contiguous, data and strides 16-byte aligned";
         return VXFA_UNSUPPORTED;
@@ -100,8 +102,9 @@ PagedBatch batch_of(const vxfa_paged* b, const vxfa_tensor* k, int64_t tokens) {
     return r;
 }
 
-PagedPool pool_of(const vxfa_tensor* t) {
-    return PagedPool{static_cast<char*>(t->data), (int64_t)t->nb[1], (int64_t)t->nb[2], (int64_t)t->nb[3]};
+PagedPool pool_of(const vxfa_tensor* k, const vxfa_tensor* v) {
+    return PagedPool{static_cast<char*>(k->data), static_cast<char*>(v->data), (int64_t)k->nb[1], (int64_t)k->nb[2],
+                     (int64_t)k->nb[3]};
 }
 
 // F32 [Hkv * D, T, 1, 1]
@@ -192,8 +195,7 @@ int vxfa_paged_append(vxfa_ctx* c, const vxfa_tensor* k_new, const vxfa_tensor* 
     a.v_new = static_cast<const float*>(v_new->data);
     a.kn_nb1 = (int64_t)k_new->nb[1];
     a.vn_nb1 = (int64_t)v_new->nb[1];
-    a.k = pool_of(k);
-    a.v = pool_of(v);
+    a.kv = pool_of(k, v);
     a.d = (int32_t)D;
     a.hkv = (int32_t)k->ne[2];
     if (rope) {
@@ -246,8 +248,7 @@ int vxfa_flash_attn_ext_paged(vxfa_ctx* c, const vxfa_tensor* q, const vxfa_tens
     a.b = batch_of(batch, k, T);
     a.q = q->data;
     a.q_nb1 = (int64_t)q->nb[1]; a.q_nb2 = (int64_t)q->nb[2];
-    a.k = pool_of(k);
-    a.v = pool_of(v);
+    a.kv = pool_of(k, v);
     a.dst = dst->data;
     a.q_f16 = q->type == VXFA_TYPE_F16;
     a.dst_f16 = dst->type == VXFA_TYPE_F16;
@@ -313,8 +314,7 @@ int vxfa_paged_evict(vxfa_ctx* c, vxfa_tensor* k, vxfa_tensor* v, vxfa_tensor* w
     vxfa::PagedEvict a;
     memset(&a, 0, sizeof(a));
     a.b = batch_of(batch, k, 0);
-    a.k = pool_of(k);
-    a.v = pool_of(v);
+    a.kv = pool_of(k, v);
     a.w = static_cast<char*>(weights->data);
     a.w_nb2 = (int64_t)weights->nb[1]; a.w_nb3 = (int64_t)weights->nb[2];
     a.d = (int32_t)k->ne[0];
