@@ -39,20 +39,14 @@ __device__ __forceinline__ int2 sel_before(int total, int* w, int wave, int lane
 __global__ __launch_bounds__(SEL_NT) void paged_select_kernel(PagedEvict a) {
     const int s = (int)blockIdx.x, h = (int)blockIdx.y, tid = (int)threadIdx.x;
     const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int n = min(max(a.b.n_kv[s], 0), a.b.max_nkv);
     int32_t* kept = a.kept + ((int64_t)s * a.hkv + h) * a.kept_row;
-    if (h == 0 && tid == 0 && a.n_out) a.n_out[s] = min(n, a.budget);
-    if (n <= a.budget) {
-        for (int r = tid; r < a.kept_row; r += SEL_NT) kept[r] = r < n ? r : -1;
-        return;
-    }
-    const int end = n - a.n_recent;   // rows [n_sink, end) compete
     const int lg = a.b.ps_log2;
     uint32_t key[SEL_PER];
-    // (8 rows are half a page at most)
+    // the keys of 8 rows, which are half a page at most (of rows that the table has;
+    // those from n on are not looked at, so the first loads need not wait for n)
     auto load = [&](int j0) {
         const int j = j0 + SEL_PER * tid;
-        const int page = j < n ? paged_page(a.b, s, j >> lg) : -1;
+        const int page = j < a.b.max_nkv ? paged_page(a.b, s, j >> lg) : -1;
         const float* w = (const float*)(a.w + max(page, 0) * a.w_nb3 + h * a.w_nb2 + 4 * (int64_t)(j & ((1 << lg) - 1)));
         float x[SEL_PER];
 #pragma unroll
@@ -60,14 +54,21 @@ __global__ __launch_bounds__(SEL_NT) void paged_select_kernel(PagedEvict a) {
 #pragma unroll
         for (int i = 0; i < SEL_PER; ++i) key[i] = page >= 0 ? sel_key(x[i]) : 0;
     };
+    load(0);
+    const int n = min(max(a.b.n_kv[s], 0), a.b.max_nkv);
+    if (h == 0 && tid == 0 && a.n_out) a.n_out[s] = min(n, a.budget);
+    if (n <= a.budget) {
+        for (int r = tid; r < a.kept_row; r += SEL_NT) kept[r] = r < n ? r : -1;
+        return;
+    }
+    const int end = n - a.n_recent;   // rows [n_sink, end) compete
     __shared__ uint32_t hists[3][SEL_BINS];
     __shared__ int list[SEL_SEG];
     __shared__ int wsum[2][SEL_NT / 64];
     __shared__ uint32_t pick[2];
-    // (a histogram for each pass, cleared while the first keys are on their way)
+    // (a histogram for each pass)
     for (int i = tid; i < 3 * SEL_BINS; i += SEL_NT) (&hists[0][0])[i] = 0;
     const bool one = n <= SEL_SEG;
-    if (one) load(0);
     __syncthreads();
     int want = a.budget - a.n_sink - a.n_recent;   // of the competing rows
     const bool any = want > 0;

@@ -356,14 +356,23 @@ __global__ __launch_bounds__(256) void paged_rows_weights(RowsArgs ra) {
     if (j + 3 >= rows_first(st, a.window)) {       // (a multiple of 16, as the tiles are)
         for (int sub = 0; sub < ra.groups; ++sub) {
             const float* x = ra.x + ((int64_t)(hk * ra.groups + sub) * a.b.n_streams + s) * ra.rows * ra.xrow + j;
-            const int heads = min(hpw, G - sub * hpw);
-            for (int i = 0; i < min(st.t, a.b.max_nq); ++i) {
-                const float* lse = a.lse + (int64_t)(st.q0 + i) * a.hq + hk * G + sub * hpw;
-                for (int h = 0; h < heads; ++h) {
-                    const floatx4 y = *(const floatx4*)(x + (int64_t)(i * hpw + h) * ra.xrow);
+            const int heads = min(hpw, G - sub * hpw), nrow = min(st.t, a.b.max_nq) * hpw;
+            // (four query rows' loads at once)
+            for (int r0 = 0; r0 < nrow; r0 += 4) {
+                floatx4 y[4];
+                float lse[4];
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) sum[c] += exp2_fast(y[c] - lse[h]);
+                for (int u = 0; u < 4; ++u) {
+                    const int i = (int)ra.hpw.div((uint32_t)(r0 + u)), h = r0 + u - i * hpw;
+                    const bool in = r0 + u < nrow && h < heads;
+                    y[u] = *(const floatx4*)(x + (int64_t)(in ? r0 + u : 0) * ra.xrow);
+                    lse[u] = a.lse[(int64_t)(st.q0 + (in ? i : 0)) * a.hq + hk * G + sub * hpw + (in ? h : 0)];
+                    if (!in) lse[u] = INFINITY;    // (weight 0)
                 }
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) sum[c] += exp2_fast(y[u][c] - lse[u]);
             }
         }
     }
