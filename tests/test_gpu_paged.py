@@ -21,6 +21,16 @@ def ctx():
     c.close()
 
 
+@pytest.fixture(params=[1, 2, 7])
+def pieces(request, monkeypatch):
+    """A context whose chunk calls cut the longest walk into this many pieces."""
+    from gpu_util import vxfa
+    monkeypatch.setenv("VXFA_PAGED_PIECES", str(request.param))
+    c = vxfa.Context(0)
+    yield c
+    c.close()
+
+
 def attend(ctx, c, scale=None, window=0, cap=0.0, bias=0.0, dst="f16", weights=None):
     """One call, checked; weights: "new", "on top" or "in place". Returns the output."""
     import torch
@@ -230,7 +240,7 @@ def test_pool_beyond_32_bits(ctx, t):
     """Pages more than 4 GiB apart."""
     import torch
     from gpu_util import vxfa
-    c = Batch([(100, t), (70, t)], hq=4, hkv=1, page=32, seed=16, spare=20)
+    c = Batch([(100, t), (70, t)], hq=4, hkv=1, page=32, seed=16, spare=20)   # (27 pages)
     row = 7 << 20                        # 7 MiB between rows, 224 MiB a page
     pools = [torch.zeros((c.n_pages * c.page * row,), dtype=torch.uint8, device="cuda") for _ in range(2)]
     assert pools[0].numel() > (1 << 32)
@@ -244,6 +254,80 @@ def test_pool_beyond_32_bits(ctx, t):
     torch.cuda.synchronize()
     want, _, err, _ = reference(c, 0.09)
     check_out(d.out(), want, err, True)
+
+
+@pytest.mark.parametrize("opt", [dict(), dict(bias=8.0), dict(cap=30.0, bias=2.0), dict(window=900)], ids=str)
+@pytest.mark.parametrize("hq,hkv,hd", [(8, 2, 128), (5, 5, 64)])
+def test_walks_of_many_steps_with_absent_pages(pieces, opt, hq, hkv, hd):
+    """Pages are looked up 16 steps (1024 rows) at a time; absent ones on both sides of that."""
+    absent = [(0, i) for i in (0, 1, 7, 31, 32, 33, 63, 64, 65, 100, 126, 127, 128, 129, 130, 191, 192, 200, 218)] + [(1, i) for i in range(60, 70)]
+    attend(pieces, Batch([(3500, 70), (2100, 150), (40, 3)], hq, hkv, hd, absent=absent, seed=21), weights="new", **opt)
+
+
+@pytest.mark.parametrize("t", [1, 20])
+@pytest.mark.parametrize("weights", [None, "on top"])
+def test_many_streams(ctx, t, weights):
+    """More streams than a wavefront has lanes."""
+    rng = np.random.default_rng(22)
+    attend(ctx, Batch([(int(n) + t, int(x)) for n, x in zip(rng.integers(0, 300, 150), rng.integers(0, t + 1, 150))], 4, 2, 64, seed=22), weights=weights)
+
+
+def test_streams_whose_parts_have_no_room(ctx):
+    """Records of 16 heads for 300 streams do not fit the workspace: whole streams, more than 64 tiles a wavefront, absent pages among them."""
+    sizes = [(9000, 1)] + [(1 + i % 20, 1) for i in range(299)]
+    attend(ctx, Batch(sizes, 256, 16, 64, seed=23, absent=[(0, i) for i in (0, 3, 250, 255, 256, 257, 300, 511, 512, 562)]))
+
+
+@pytest.mark.parametrize("t", [1, 2])
+def test_weights_without_room_for_scores(ctx, t):
+    """Bounds so wide that single tokens' scores do not fit the workspace: the weights form them again."""
+    c = Batch([(500, t), (33, t), (260, t), (1, 1)] * 10, 16, 4, 128, seed=24)
+    wide = np.full((c.B, 1 << 12), -1, np.int32)          # 65536 rows a stream
+    wide[:, :c.max_pages] = c.table
+    c.table, c.max_pages = wide, 1 << 12
+    attend(ctx, c, weights="on top")
+
+
+@pytest.mark.parametrize("t", [1, 40])
+@pytest.mark.parametrize("q_type", ["f16", "f32"])
+def test_strided_queries(ctx, t, q_type):
+    """Queries [head][token] with room between the rows."""
+    import torch
+    c = Batch([(100, t), (300, t)], 8, 2, 64, q_type=q_type, seed=25)
+    d = Device(c)
+    e = c.q.itemsize
+    x = np.full((c.hq, c.T, c.hd + 16), np.nan, c.q.dtype)
+    x[..., :c.hd] = c.q.transpose(1, 0, 2)
+    g = torch.from_numpy(x).cuda()
+    row = (c.hd + 16) * e
+    q = d.vxfa.desc(g.data_ptr(), d.q.type, (c.hd, c.T, c.hq, 1), (e, row, c.T * row, c.hq * c.T * row))
+    ctx.flash_attn_ext_paged(q, d.k, d.v, d.batch, d.dst, 0.12, weights=d.w)
+    torch.cuda.synchronize()
+    want, add, err, adderr = reference(c, 0.12)
+    check_out(d.out(), want, err, True)
+    check_weights(c, d.weights(), None, add, adderr, c.w)
+
+
+@pytest.mark.parametrize("t", [1, 40])
+def test_no_pages_at_all(ctx, t):
+    """An empty pool: every row is absent, outputs are zeros."""
+    import torch
+    c = Batch([(0, t), (0, t)], seed=26, spare=1)
+    c.n_kv[:] = 50
+    c.sizes = [(0, t), (0, t)]
+    d = Device(c)
+    d.n_kv.copy_(torch.from_numpy(c.n_kv.view(np.uint8)))
+    for x in (d.k, d.v):
+        x.ne[3] = 0
+    d.w.ne[2] = 0
+    ctx.flash_attn_ext_paged(d.q, d.k, d.v, d.batch, d.dst, 0.12, weights=d.w)
+    torch.cuda.synchronize()
+    assert (d.out() == 0).all()
+    d.batch.max_nq = 0
+    d.dt.fill_(0xA5)
+    ctx.flash_attn_ext_paged(d.q, d.k, d.v, d.batch, d.dst, 0.12, weights=d.w)
+    torch.cuda.synchronize()
+    assert (d.dt == 0xA5).all()
 
 
 # ---- append ----------------------------------------------------------------------
@@ -384,6 +468,15 @@ def test_evict(ctx, hkv, hd, page, layout, budget, sink, recent):
     c = Batch([(n, 0) for n in (0, 1, 39, 40, 41, 101, 333, 1000, 2100)], hkv * 2, hkv, hd, page, layout, seed=budget, spare=9 * (-(-budget // page)) + 2)
     evict(ctx, c, budget, sink, recent)
     evict(ctx, c, budget, sink, recent, with_kept=False)
+
+
+def test_evict_long_streams(ctx):
+    """Streams of several segments of 8192 rows, ties across them."""
+    c = Batch([(20000, 0), (8193, 0), (8192, 0)], 2, 2, 64, 64, seed=6, spare=3 * 150)
+    c.w = np.round(c.w * 50) / 50
+    evict(ctx, c, 9000, 100, 1000)
+    evict(ctx, c, 8192, 0, 0)
+    evict(ctx, c, 5, 1, 2)
 
 
 @pytest.mark.parametrize("kind", ["equal", "few", "signs", "nan", "inf", "tiny"])

@@ -60,8 +60,10 @@ __device__ __forceinline__ int rows_first(const PagedStream& s, int window) {
     return window > 0 ? max(s.n - s.t - window + 1, 0) & ~15 : 0;
 }
 
+#endif
+
 // rows of a part, given all streams' rows: whole rounds of four tiles
-__device__ __forceinline__ int rows_chunk(const RowsPlan& p, int64_t total) {
+__host__ __device__ __forceinline__ int rows_chunk(const RowsPlan& p, int64_t total) {
     int64_t c = (total + p.small - 1) / p.small;
     if (c > p.limit) {
         c = (total + p.large - 1) / p.large;
@@ -70,14 +72,21 @@ __device__ __forceinline__ int rows_chunk(const RowsPlan& p, int64_t total) {
     c = (c + 63) & ~(int64_t)63;
     return c < 64 ? 64 : (c > 0x40000000 ? 0x40000000 : (int)c);
 }
+// all streams' rows as rows_chunk takes them: `tiles` whole tiles, and what is left of
+// each stream counted as a tile less one row
+__host__ __device__ __forceinline__ int64_t rows_total(int64_t tiles, int n_streams) { return 16 * tiles + 15 * (int64_t)n_streams; }
+// parts of a stream of len rows
+__host__ __device__ __forceinline__ int rows_parts(const RowsPlan& p, int len, int chunk) {
+    return p.cuts && len > chunk ? (int)(((int64_t)len + chunk - 1) / chunk) : 1;
+}
 
+#ifdef __HIPCC__
 __device__ __forceinline__ Part rows_locate(const PagedBatch& b, const RowsPlan& p, int window, int item) {
     Part r;
     const int lane = (int)threadIdx.x & 63;
     auto parts = [&](const PagedStream& s, int chunk) -> int {
         if (s.t <= 0) return 0;
-        const int len = s.n - rows_first(s, window);
-        return p.cuts && len > chunk ? (len + chunk - 1) / chunk : 1;
+        return rows_parts(p, s.n - rows_first(s, window), chunk);
     };
     if (b.n_streams == 1) {
         r.st = paged_stream(b, 0);
@@ -97,7 +106,7 @@ __device__ __forceinline__ Part rows_locate(const PagedBatch& b, const RowsPlan&
         if (s0 == 0) mine = s;
         if (p.cuts) total += wave_sum(s.t > 0 ? max(s.n - rows_first(s, window), 0) >> 4 : 0);
     }
-    const int chunk = rows_chunk(p, 16 * total + 15 * (int64_t)b.n_streams);
+    const int chunk = rows_chunk(p, rows_total(total, b.n_streams));
     int before = 0;
     r.s = -1;
     for (int s0 = 0; s0 < b.n_streams; s0 += 64) {

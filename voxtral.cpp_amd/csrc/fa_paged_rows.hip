@@ -405,7 +405,7 @@ hipError_t launch_paged_rows(const PagedAttn& a, int head_dim, hipStream_t st, b
     ra.xrow = ((int64_t)a.b.max_nkv + 15) & ~(int64_t)15;
     const double xb = (double)nhg * a.b.n_streams * ra.rows * (double)ra.xrow * sizeof(float);
     const size_t usual = (size_t)(512 + (size_t)a.b.n_streams * nhg) * ra.rec * sizeof(float);
-    if (a.w_out && xb + (double)used + (double)usual <= (double)a.ws_bytes) {
+    if (a.w_out && a.b.max_nkv > 0 && xb + (double)used + (double)usual <= (double)a.ws_bytes) {
         ra.x = reinterpret_cast<float*>(a.ws + used);
         used += ((size_t)xb + 255) & ~(size_t)255;
         weighed = true;

@@ -43,7 +43,7 @@ static thread_local char t_noalloc_err[256] = {0};   // message of this thread's
 
 namespace {
 
-constexpr int kVersion = 1 * 10000 + 1 * 100 + 0;
+constexpr int kVersion = 1 * 10000 + 2 * 100 + 0;
 constexpr int kMaskedSplitCap = 32;
 
 void set_err(Workspace& w, const char* fmt, ...) {

@@ -28,8 +28,8 @@ bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) &
 
 bool sane(const vxfa_tensor* t) {
     if (t->type != VXFA_TYPE_F32 && t->type != VXFA_TYPE_F16) return false;
-    for (int d = 0; d < 4; ++d)
-        if (t->ne[d] < 0 || t->nb[d] > ((size_t)1 << 62)) return false;
+    for (int d = 0; d < 4; ++d)   // (offsets have to fit 64 bits)
+        if (t->ne[d] < 0 || t->nb[d] > ((size_t)1 << 60) / (size_t)(t->ne[d] > 0 ? t->ne[d] : 1)) return false;
     return true;
 }
 
@@ -290,7 +290,7 @@ int vxfa_flash_attn_ext_paged(vxfa_ctx* c, const vxfa_tensor* q, const vxfa_tens
     // (up to 16); else tiles of 32 query rows
     hipError_t e = hipSuccess;
     bool weighed = false;
-    if (T * Hq > 0 && a.b.n_streams > 0)
+    if (T * Hq > 0 && a.b.n_streams > 0 && a.b.max_nq > 0)
         e = vxfa::paged_rows_takes(a) ? vxfa::launch_paged_rows(a, (int)D, st, weighed) : vxfa::launch_paged_chunk(a, (int)D, st);
     if (e == hipSuccess && weights && !weighed) e = vxfa::launch_paged_weights(a, (int)D, st);
     if (e != hipSuccess) return fail(c, VXFA_HIP_ERROR, "paged attention: %s", hipGetErrorString(e));
