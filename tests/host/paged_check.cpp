@@ -112,7 +112,7 @@ static void grids() {
         const int nhg = pick(1, 64);
         int32_t items = 0;
         const int64_t room = it % 4 ? 100000 : pick(0, 500);
-        const vxfa::RowsPlan p = vxfa::rows_plan(b, nhg, room, items);
+        const vxfa::RowsPlan p = vxfa::rows_plan(b, nhg, it % 7 ? 128 : 64, room, items);
         int64_t tiles = 0, parts = 0;
         std::vector<int> len((size_t)b.n_streams);
         for (int& l : len) {

@@ -19,14 +19,29 @@ struct RowsPlan {
     int32_t small, large;     // parts (per head group) that all streams' rows are cut into
     int32_t limit;            // rows of a part from which `large` holds
     int32_t cuts;             // 0: a part per stream
+    int32_t empty;            // 1: one, too, for a stream without tokens
 };
 
+// Whether streams are left whole: what a cut costs (its join, a launch of its own)
+// against what it gains, by the bounds. In us: a workgroup alone takes 9.0 ns a row
+// (hd 64: 7.3), all together move 5 TB/s; the streams are taken for three quarters
+// of the bound on average, and for too uneven beyond 2048 rows. Measured, cut ->
+// whole: 1 stream of up to 256 rows 8.1 -> 5.6, 512 8.3 -> 9.2, 16 streams x 8 kv
+// heads of up to 512 12.5 -> 10.1, 4096 39.7 -> 53.0, 32 x 8 of up to 256 12.9 -> 8.3,
+// 1024 23.7 -> 17.3, 2048 40.2 -> 35.9, 8192 117 -> 128.
+inline bool rows_whole(const PagedBatch& b, int nhg, int head_dim) {
+    const double n = 1e-3 * b.max_nkv, alone = head_dim == 128 ? 9.0 : 7.3;
+    const double together = 0.75 * (double)b.n_streams * nhg * 4 * head_dim / 5000;
+    return b.max_nkv <= 2048 && 4.5 + n * (alone > together ? alone : together) < 8.0 + 1.05 * n * together;
+}
+
 // The grid of a call: `items` parts per head group.
-inline RowsPlan rows_plan(const PagedBatch& b, int nhg, int64_t room, int32_t& items) {
+inline RowsPlan rows_plan(const PagedBatch& b, int nhg, int head_dim, int64_t room, int32_t& items) {
     RowsPlan p;
+    p.empty = 0;
     p.small = 512 / nhg > 0 ? 512 / nhg : 1;
     p.large = 2048 / nhg > 0 ? 2048 / nhg : 1;
-    p.limit = 512;
+    p.limit = 1024;
     // n parts' worth of rows are at most n parts of one stream, n + streams of more
     const int64_t more = b.n_streams > 1 ? b.n_streams : 0;
     const int64_t all = (int64_t)b.n_streams * b.max_nkv;
@@ -37,7 +52,7 @@ inline RowsPlan rows_plan(const PagedBatch& b, int nhg, int64_t room, int32_t& i
         else p.cuts = 0;
     }
     if (p.small > p.large) p.small = p.large;
-    if (b.max_nkv <= 64) p.cuts = 0;
+    if (rows_whole(b, nhg, head_dim)) p.cuts = 0;
     items = b.n_streams;
     if (p.cuts) {
         const int64_t by_rows = (int64_t)b.n_streams * ((b.max_nkv + 63) / 64);
@@ -85,7 +100,7 @@ __device__ __forceinline__ Part rows_locate(const PagedBatch& b, const RowsPlan&
     Part r;
     const int lane = (int)threadIdx.x & 63;
     auto parts = [&](const PagedStream& s, int chunk) -> int {
-        if (s.t <= 0) return 0;
+        if (s.t <= 0) return s.t == 0 ? p.empty : 0;   // (-1: no such stream)
         return rows_parts(p, s.n - rows_first(s, window), chunk);
     };
     if (b.n_streams == 1) {
@@ -101,7 +116,7 @@ __device__ __forceinline__ Part rows_locate(const PagedBatch& b, const RowsPlan&
     PagedStream mine{0, 0, 0};
     int64_t total = 0;
     for (int s0 = 0; s0 < b.n_streams; s0 += 64) {
-        PagedStream s{0, 0, 0};
+        PagedStream s{0, -1, 0};
         if (s0 + lane < b.n_streams) s = paged_stream(b, s0 + lane);
         if (s0 == 0) mine = s;
         if (p.cuts) total += wave_sum(s.t > 0 ? max(s.n - rows_first(s, window), 0) >> 4 : 0);
@@ -112,7 +127,7 @@ __device__ __forceinline__ Part rows_locate(const PagedBatch& b, const RowsPlan&
     for (int s0 = 0; s0 < b.n_streams; s0 += 64) {
         PagedStream s = mine;
         if (s0 > 0) {
-            s = PagedStream{0, 0, 0};
+            s = PagedStream{0, -1, 0};
             if (s0 + lane < b.n_streams) s = paged_stream(b, s0 + lane);
         }
         const int n = parts(s, chunk);

@@ -45,6 +45,7 @@ struct RowsArgs {
     // [head group][stream][query row][xrow], -inf where a row is not seen
     float* x;
     int64_t xrow;
+    int32_t whole;            // no stream is cut and no group shared: the weights need no launch of their own
 };
 
 template <int N>
@@ -77,7 +78,7 @@ __global__ __launch_bounds__(64 * PR_WAVES, 2) void paged_rows_kernel(RowsArgs r
     constexpr int NS = D == 128 ? 2 : 4;       // slots (64 KiB a workgroup: two of them on a CU)
     static_assert(PR_WAVES * 16 * D * 4 <= PR_WAVES * NS * TILE, "the join uses the slots");
     __shared__ __attribute__((aligned(16))) char smem[PR_WAVES * NS * TILE];
-    __shared__ float sm[PR_WAVES][16], sl[PR_WAVES][16];
+    __shared__ float sm[PR_WAVES][16], sl[PR_WAVES][16], slse[16];
 
     const PagedAttn& a = ra.a;
     const int lane = (int)threadIdx.x & 63;
@@ -91,7 +92,7 @@ __global__ __launch_bounds__(64 * PR_WAVES, 2) void paged_rows_kernel(RowsArgs r
     if (part.piece == 0 && hg == 0 && threadIdx.x == 0) ra.cut[part.s] = int2{part.first, part.n};
 
     // ---- this part's tiles, their pages -------------------------------------------
-    const int nall = (st.n - part.lo + PR_TILE - 1) / PR_TILE;      // of the stream (none: n <= lo)
+    const int nall = st.t > 0 ? (st.n - part.lo + PR_TILE - 1) / PR_TILE : 0;   // of the stream (none: n <= lo)
     const int tb = (int)((int64_t)nall * part.piece / part.n), te = (int)((int64_t)nall * (part.piece + 1) / part.n);
     const int nk = max((te - tb - wave + PR_WAVES - 1) / PR_WAVES, 0);   // the wavefront's: tb + wave + 4 k
     const int lg = a.b.ps_log2;
@@ -253,7 +254,11 @@ __global__ __launch_bounds__(64 * PR_WAVES, 2) void paged_rows_kernel(RowsArgs r
                 const int64_t at = (int64_t)(st.q0 + tk) * a.hq + hk * G + sub * (int)ra.hpw.d + hh;
                 const float inv = L == 0.f ? 0.f : 1.f / L;
                 paged_store4(a, at * D + 4 * c, x * inv);
-                if (a.lse && c == 0) a.lse[at] = L == 0.f ? INFINITY : M + log2f(L);
+                if (a.lse && c == 0) {
+                    const float lse = L == 0.f ? INFINITY : M + log2f(L);
+                    a.lse[at] = lse;
+                    slse[r] = lse;
+                }
             }
         } else {
             *(floatx4*)(rec + r * D + 4 * c) = x;
@@ -261,6 +266,21 @@ __global__ __launch_bounds__(64 * PR_WAVES, 2) void paged_rows_kernel(RowsArgs r
                 rec[ra.rows * D + r] = M;
                 rec[ra.rows * (D + 1) + r] = L;
             }
+        }
+    }
+    // a whole stream's rows have their weights at once (as paged_rows_weights does)
+    if (ra.whole) {
+        __syncthreads();
+        const float* x = ra.x + ((int64_t)hg * a.b.n_streams + part.s) * ra.rows * ra.xrow;
+        for (int j = (int)threadIdx.x; j < st.n; j += 64 * PR_WAVES) {
+            const int page = paged_page(a.b, part.s, j >> lg);
+            if (page < 0) continue;
+            float sum = 0.f;
+            if (j >= part.lo)
+                for (int r = 0; r < nrow; ++r) sum += exp2_fast(x[r * ra.xrow + j] - slse[r]);
+            const int64_t at = 4 * (int64_t)(j & ((1 << lg) - 1));
+            const float old = a.w_in ? *(const float*)((const char*)a.w_in + page * a.wi_nb3 + hk * a.wi_nb2 + at) : 0.f;
+            *(float*)((char*)a.w_out + page * a.wo_nb3 + hk * a.wo_nb2 + at) = old + sum;
         }
     }
 }
@@ -412,7 +432,10 @@ hipError_t launch_paged_rows(const PagedAttn& a, int head_dim, hipStream_t st, b
     }
     ra.recs = reinterpret_cast<float*>(a.ws + used);
     const int64_t room = used < a.ws_bytes ? (int64_t)((a.ws_bytes - used) / ((size_t)ra.rec * sizeof(float))) / nhg : 0;
-    ra.p = rows_plan(a.b, nhg, room, ra.items);
+    ra.p = rows_plan(a.b, nhg, head_dim, room, ra.items);
+    // (streams without tokens have a part then, too: their rows' weights are taken over)
+    ra.whole = ra.x && !ra.p.cuts && ra.groups == 1;
+    ra.p.empty = ra.whole;
     const int64_t nwg = (int64_t)ra.items * nhg;
     if (nwg > 0x7fffffff / 256) return hipErrorInvalidValue;
     const dim3 grid((unsigned)nwg), block(64 * PR_WAVES);
@@ -427,7 +450,7 @@ hipError_t launch_paged_rows(const PagedAttn& a, int head_dim, hipStream_t st, b
         e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
-    if (!ra.x) return e;
+    if (!ra.x || ra.whole) return e;
     const int64_t gx = ((int64_t)a.b.max_nkv + 1023) / 1024 * a.hkv;
     if (gx > kMaxGridX) return hipErrorInvalidValue;
     hipLaunchKernelGGL(paged_rows_weights, dim3((unsigned)gx, (unsigned)a.b.n_streams), dim3(256), 0, st, ra);
