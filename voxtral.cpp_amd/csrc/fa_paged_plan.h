@@ -41,7 +41,7 @@ inline RowsPlan rows_plan(const PagedBatch& b, int nhg, int head_dim, int64_t ro
     p.empty = 0;
     p.small = 512 / nhg > 0 ? 512 / nhg : 1;
     p.large = 2048 / nhg > 0 ? 2048 / nhg : 1;
-    p.limit = 1024;
+    p.limit = 512;
     // n parts' worth of rows are at most n parts of one stream, n + streams of more
     const int64_t more = b.n_streams > 1 ? b.n_streams : 0;
     const int64_t all = (int64_t)b.n_streams * b.max_nkv;
