@@ -146,7 +146,7 @@ static void grids() {
         vxfa::ChunkPlan p;
         std::memset(&p, 0, sizeof(p));
         const size_t ws = (size_t)pick(1, 40) << 20, record = 133120;
-        const vxfa::ChunkBounds r = vxfa::chunk_plan(b, nhg, bm, it % 3 ? 0 : pick(1, 5000), record, ws, p);
+        const vxfa::ChunkBounds r = vxfa::chunk_plan(b, it % 2 ? 128 : 64, nhg, bm, it % 3 ? 0 : pick(1, 5000), record, ws, p);
         const bool ok = tiles <= r.tiles && tiles <= p.items && (b.n_streams > 1 || p.pieces <= 1 || !p.cuts || p.items <= p.room) &&
                         (!p.cuts || r.table + (size_t)p.room * record * nhg <= ws) && p.items >= 1;
         if (!ok) {

@@ -24,6 +24,11 @@
 //   2^8 in every block of a steep head, and every block's softmax be done twice.
 //   The sum of P is taken in F32 before P is rounded: its logarithm is what the
 //   accumulated weights are divided by.
+//   hd 64, up to 256 workgroups: two groups of 4 wavefronts, each with half of the
+//   piece's blocks and a ring of its own, joined through LDS: alone on its CU a
+//   workgroup has one wavefront a SIMD, and the chain of a block's dependent steps
+//   takes 0.6 us (600 tokens on 3000 rows, 20 heads: 41.3 -> 35.5 us; with 320
+//   workgroups, two on some CUs either way, 41 -> 50).
 // What bounds it: see fa_prefill_group.hip; with a cap the two further
 // transcendentals a score (exp2, reciprocal).
 #pragma once
@@ -35,7 +40,7 @@
 
 namespace vxfa {
 
-template <int HD>
+template <int HD, int KVGROUPS = 1>
 struct PC {
     static constexpr int D = HD;
     static constexpr int KS = D / 16;             // S-MFMA k-steps
@@ -45,8 +50,9 @@ struct PC {
     static constexpr int BLK = BK * ROW;          // bytes of one matrix block
     static constexpr int STEP = 2 * BLK;          // one matrix of a 64-row step
     static constexpr int NS = 4;                  // ring slots
-    static constexpr int NW = D / 16;             // wavefronts (8 or 4)
-    static constexpr int NT = 64 * NW;
+    static constexpr int NW = D / 16;             // wavefronts of 32 query rows (8 or 4)
+    static constexpr int KVG = KVGROUPS;          // groups of them, each with its share of the blocks
+    static constexpr int NT = 64 * NW * KVG;
     static constexpr int RECO = 64 * 16 * DB;     // floats of O in a wavefront's record
     static constexpr int REC = RECO + 64;         // and (m, l) of 32 rows
 };
@@ -69,21 +75,24 @@ __device__ __forceinline__ void pc_wait_vm() {
 }
 
 // MOD: 1 the scores have a distance term, 2 a cap (and a slope, or 0). QF16: q is F16.
-template <int HD, bool QF16, int MOD>
-__global__ __launch_bounds__(PC<HD>::NT, 2) void paged_chunk_kernel(ChunkArgs ca) {
-    using P = PC<HD>;
+template <int HD, int KVGROUPS, bool QF16, int MOD>
+__global__ __launch_bounds__((PC<HD, KVGROUPS>::NT), 2) void paged_chunk_kernel(ChunkArgs ca) {
+    using P = PC<HD, KVGROUPS>;
     constexpr int D = P::D, KS = P::KS, DB = P::DB, BK = P::BK, ROW = P::ROW, BLK = P::BLK, STEP = P::STEP, NS = P::NS,
                   NW = P::NW, REC = P::REC;
     // K steps, V steps, and with 8 wavefronts half of the Q staging. The first block
     // past the ring is zeros from step 0 on: V of a block dead for a wavefront's rows.
-    constexpr int ZERO = 2 * NS * STEP;
+    constexpr int ZERO = 2 * NS * STEP, KVG = P::KVG;
+    constexpr int REGION = ZERO + (NW == 8 ? 4 : 1) * BLK;     // a group's
     constexpr bool REV = MOD != 0;                        // blocks from the last
-    __shared__ __attribute__((aligned(16))) char smem[ZERO + (NW == 8 ? 4 : 1) * BLK];
+    __shared__ __attribute__((aligned(16))) char smem_all[KVG * REGION];
 
     const PagedAttn& a = ca.a;
     const int tid = (int)threadIdx.x;
     const int lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int grp = KVG == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid >> 6) / NW;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6) - grp * NW;
+    char* const smem = smem_all + grp * REGION;
     const int hg = (int)blockIdx.x % ca.nhg;
     const int item = (int)blockIdx.x / ca.nhg;
     const int hpw = 1 << ca.p.hpw_log2;
@@ -119,6 +128,14 @@ __global__ __launch_bounds__(PC<HD>::NT, 2) void paged_chunk_kernel(ChunkArgs ca
         const int len = ((nblk + it.n - 1) / it.n + 1) & ~1;   // whole steps
         bs = blo + min(it.piece * len, nblk);
         nb = min(len, blo + nblk - bs);
+    }
+    // the group's share: whole steps, the first group's the longer
+    int steps = (nb + 1) >> 1;                            // of the first group
+    if constexpr (KVG == 2) {
+        const int n0 = min(((nb + 1) / 2 + 1) & ~1, nb);
+        steps = (n0 + 1) >> 1;
+        bs += grp ? n0 : 0;
+        nb = grp ? nb - n0 : n0;
     }
 
     // ---- Q loads: whole rows of the wavefront's 32, through LDS below -------------
@@ -252,8 +269,8 @@ __global__ __launch_bounds__(PC<HD>::NT, 2) void paged_chunk_kernel(ChunkArgs ca
             for (int i = 0; i < BLK / 1024; ++i) *(half8*)(smem + ZERO + 1024 * i + 16 * lane) = half8{};
         }
     } else {
-        static_assert(NW == 8 || BLK == 16 * P::NT, "one 16-byte store per thread");
-        *(half8*)(smem + ZERO + 16 * tid) = half8{};
+        static_assert(NW == 8 || BLK == 16 * 64 * NW, "one 16-byte store per thread of the group");
+        *(half8*)(smem + ZERO + 16 * (64 * wave + lane)) = half8{};
     }
 
     // ---- operand reads (layouts of fa_prefill.hip) ----------------------------------
@@ -420,7 +437,7 @@ __global__ __launch_bounds__(PC<HD>::NT, 2) void paged_chunk_kernel(ChunkArgs ca
     }
     __syncthreads();
 
-    if (nb > 0) {
+    {
         half8 kr[KS], vr[2][DB], pa[2], pb[2];
         floatx16 sa, sb;
         // PV of the block before the first adds zero
@@ -430,11 +447,13 @@ __global__ __launch_bounds__(PC<HD>::NT, 2) void paged_chunk_kernel(ChunkArgs ca
 #pragma unroll
             for (int db = 0; db < DB; ++db) vr[cc][db] = half8{};
         }
-        read_k(0, kr);
-        s_mfma(sa, kr);
-        mask_test(0);
-        mask_fix(sa, 0);
-        m = block_max(sa, 0);
+        if (nb > 0) {
+            read_k(0, kr);
+            s_mfma(sa, kr);
+            mask_test(0);
+            mask_fix(sa, 0);
+            m = block_max(sa, 0);
+        }
         // half t: PV(t - 1), S(t + 1) and the softmax of S(t)
         auto half = [&](int t, floatx16& scur, floatx16& snext, half8 (&pcur)[2], half8 (&pprev)[2]) {
             const int va = mask_test(t);
@@ -448,9 +467,9 @@ __global__ __launch_bounds__(PC<HD>::NT, 2) void paged_chunk_kernel(ChunkArgs ca
         };
         // (whole steps: a second block past nb has no live score, and the last
         // half's S is not used)
-        for (int u = 0; u < nstep; ++u) {
+        for (int u = 0; u < (KVG == 1 ? nstep : steps); ++u) {
             if (u + NS - 1 < nstep) issue(u + NS - 1);
-            if (active) {
+            if (active && (KVG == 1 || u < nstep)) {
                 half(2 * u, sa, sb, pa, pb);
                 half(2 * u + 1, sb, sa, pb, pa);
             }
@@ -461,11 +480,41 @@ __global__ __launch_bounds__(PC<HD>::NT, 2) void paged_chunk_kernel(ChunkArgs ca
             else pc_wait_vm<0>();
             __syncthreads();
         }
-        pv_mfma(pb, vr);
+        if (nb > 0) pv_mfma(pb, vr);
     }
 
     // ---- output, or this piece's record --------------------------------------------
-    const float lt = pair32_sum(l);
+    float lt = pair32_sum(l);
+    if constexpr (KVG == 2) {
+        // the second group's O, m and l through LDS (its ring has been read)
+        static_assert(KVG == 1 || NW * 64 * (16 * DB + 2) * 4 <= REGION, "the join's room");
+        float* const x = reinterpret_cast<float*>(smem_all) + wave * 64 * (16 * DB + 2);
+        __syncthreads();
+        if (grp == 1) {
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
+#pragma unroll
+                for (int a4 = 0; a4 < 4; ++a4)
+                    *(floatx4*)(x + (4 * db + a4) * 256 + 4 * lane) =
+                        floatx4{o[db][4 * a4], o[db][4 * a4 + 1], o[db][4 * a4 + 2], o[db][4 * a4 + 3]};
+            *(float2*)(x + 64 * 16 * DB + 2 * lane) = float2{m, lt};
+        }
+        __syncthreads();
+        if (grp == 1) return;
+        const float2 ml = *(const float2*)(x + 64 * 16 * DB + 2 * lane);
+        const float mn = fmaxf(m, ml.x), ms = mn == -INFINITY ? 0.f : mn;
+        const float w0 = exp2_fast(m - ms), w1 = exp2_fast(ml.x - ms);
+        m = mn;
+        lt = lt * w0 + ml.y * w1;
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int a4 = 0; a4 < 4; ++a4) {
+                const floatx4 y = *(const floatx4*)(x + (4 * db + a4) * 256 + 4 * lane);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[db][4 * a4 + e] = fmaf(y[e], w1, o[db][4 * a4 + e] * w0);
+            }
+    }
     if (it.n == 1) {
         const float inv = (lt == 0.f) ? 0.f : 1.0f / lt;
         if (qvalid) {
@@ -560,12 +609,12 @@ __global__ __launch_bounds__(64 * PC<HD>::DB) void paged_chunk_combine(ChunkArgs
     if (a.lse && db == 0 && hh == 0) a.lse[row] = L == 0.f ? INFINITY : M + log2f(L);
 }
 
-template <int HD, bool QF16>
+template <int HD, int KVG, bool QF16>
 static void launch_pc(const ChunkArgs& ca, unsigned nwg, hipStream_t st) {
-    const dim3 grid(nwg), block(PC<HD>::NT);
-    if (ca.a.cap != 0.f) hipLaunchKernelGGL((paged_chunk_kernel<HD, QF16, 2>), grid, block, 0, st, ca);
-    else if (ca.a.bias1 != 0.f) hipLaunchKernelGGL((paged_chunk_kernel<HD, QF16, 1>), grid, block, 0, st, ca);
-    else hipLaunchKernelGGL((paged_chunk_kernel<HD, QF16, 0>), grid, block, 0, st, ca);
+    const dim3 grid(nwg), block(PC<HD, KVG>::NT);
+    if (ca.a.cap != 0.f) hipLaunchKernelGGL((paged_chunk_kernel<HD, KVG, QF16, 2>), grid, block, 0, st, ca);
+    else if (ca.a.bias1 != 0.f) hipLaunchKernelGGL((paged_chunk_kernel<HD, KVG, QF16, 1>), grid, block, 0, st, ca);
+    else hipLaunchKernelGGL((paged_chunk_kernel<HD, KVG, QF16, 0>), grid, block, 0, st, ca);
 }
 
 template <int HD>
@@ -578,15 +627,23 @@ static hipError_t launch_chunk(const PagedAttn& a, hipStream_t st) {
     const int hpw = 1 << l2;
     ca.nhg = a.hq / hpw;
     ca.p.pieces = a.pieces;
-    const ChunkBounds cb = chunk_plan(a.b, ca.nhg, 32 * (P::NW >> l2), a.window, (size_t)P::NW * P::REC * sizeof(float), a.ws_bytes, ca.p);
+    const ChunkBounds cb = chunk_plan(a.b, HD, ca.nhg, 32 * (P::NW >> l2), a.window, (size_t)P::NW * P::REC * sizeof(float), a.ws_bytes, ca.p);
     ca.p.hpw_log2 = l2;
     if (cb.table > a.ws_bytes) return hipErrorInvalidValue;   // (16 bytes a tile: 2.5 million of them fit)
     ca.tiles = reinterpret_cast<ChunkTile*>(a.ws);
     ca.rec = reinterpret_cast<float*>(a.ws + cb.table);
     const int64_t nwg = (int64_t)ca.p.items * ca.nhg;
-    if (nwg > 0xffffffffll / P::NT) return hipErrorInvalidValue;
-    if (a.q_f16) launch_pc<HD, true>(ca, (unsigned)nwg, st);
-    else launch_pc<HD, false>(ca, (unsigned)nwg, st);
+    if (nwg > 0xffffffffll / 512) return hipErrorInvalidValue;
+    if constexpr (HD == 64) {
+        if (ca.p.kvg == 2) {
+            if (a.q_f16) launch_pc<HD, 2, true>(ca, (unsigned)nwg, st);
+            else launch_pc<HD, 2, false>(ca, (unsigned)nwg, st);
+        }
+    }
+    if (ca.p.kvg == 1) {
+        if (a.q_f16) launch_pc<HD, 1, true>(ca, (unsigned)nwg, st);
+        else launch_pc<HD, 1, false>(ca, (unsigned)nwg, st);
+    }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || !ca.p.cuts) return e;
     hipLaunchKernelGGL((paged_chunk_combine<HD>), dim3((unsigned)(cb.tiles * ca.nhg * P::NW)), dim3(64 * P::DB), 0, st, ca);

@@ -158,6 +158,7 @@ __device__ __forceinline__ Part rows_locate(const PagedBatch& b, const RowsPlan&
 
 struct ChunkPlan {
     uint32_t hpw_log2;        // log2 of the query heads per workgroup
+    int32_t kvg;              // groups of wavefronts that share a piece's blocks
     int32_t cuts;             // 0: a piece per tile
     int32_t pieces;           // > 0: pieces of the longest walk (else chunk_choose's)
     int32_t items;            // pieces in the grid per head group
@@ -176,12 +177,13 @@ constexpr int kChunkStreams = 64;   // more streams are not cut
 
 // A cut's time in blocks of 32 rows: `total` blocks of a head group, in `items`
 // workgroups (of each head group) of `lp` at most. A workgroup costs its blocks
-// and kWg, 256 run at once; a record costs its traffic, and the joining of a
-// walk's pieces goes one after another.
-__host__ __device__ inline float chunk_cost(float total, int items, int recs, int lp, int nhg, int pieces) {
+// (shared among kvg groups of wavefronts) and kWg, 256 run at once; a record costs
+// its traffic, and the joining of a walk's pieces goes one after another.
+__host__ __device__ inline float chunk_cost(float total, int items, int recs, int lp, int nhg, int pieces, int kvg) {
     constexpr float kWg = 4.f, kRecord = 0.05f, kPiece = 0.3f;
     const float count = (float)(items * nhg), rounds = ceilf(count * (1.f / 256.f));
-    return fmaxf(rounds * (total * (float)nhg / fmaxf(count, 1.f) + kWg), (float)lp + kWg) + kRecord * (float)(recs * nhg) +
+    const float share = 1.f / (float)kvg;
+    return fmaxf(rounds * (share * total * (float)nhg / fmaxf(count, 1.f) + kWg), share * (float)lp + kWg) + kRecord * (float)(recs * nhg) +
            (recs ? kPiece * (float)pieces : 0.f);
 }
 // length of the pieces of a walk of nb blocks in n pieces: whole steps
@@ -198,7 +200,7 @@ __host__ __device__ inline float chunk_blocks(int tiles, int nb, int bm, int win
     return less > (float)tiles ? less : (float)tiles;
 }
 
-inline ChunkBounds chunk_plan(const PagedBatch& b, int nhg, int bm, int window, size_t record, size_t ws_bytes, ChunkPlan& p) {
+inline ChunkBounds chunk_plan(const PagedBatch& b, int head_dim, int nhg, int bm, int window, size_t record, size_t ws_bytes, ChunkPlan& p) {
     ChunkBounds r;
     // sum of ceil(t / bm) over streams of `tokens` tokens in all, max_nq at most each
     const int64_t per = ((int64_t)b.max_nq + bm - 1) / bm;
@@ -208,6 +210,7 @@ inline ChunkBounds chunk_plan(const PagedBatch& b, int nhg, int bm, int window, 
     if (r.tiles > b.tokens) r.tiles = b.tokens;
     r.table = ((size_t)(1 + r.tiles) * sizeof(ChunkTile) + 255) & ~(size_t)255;
     p.nhg = nhg;
+    p.kvg = head_dim == 64 && r.tiles * nhg <= 256 ? 2 : 1;
     p.tiles = (int32_t)r.tiles;
     const int64_t room = r.table < ws_bytes ? (int64_t)((ws_bytes - r.table) / (record * (size_t)nhg)) : 0;
     p.room = (int32_t)(room < 4096 ? room : 4096);
@@ -228,7 +231,7 @@ inline ChunkBounds chunk_plan(const PagedBatch& b, int nhg, int bm, int window, 
         for (int n = 1; n <= 64; ++n) {
             const int lp = chunk_length((int)nb, n), k = n == 1 ? 1 : (int)((nb + lp - 1) / lp), all = k * tiles;
             if (k > 1 && all > p.room) break;
-            const float cost = chunk_cost(chunk_blocks(tiles, (int)nb, bm, window), all, k > 1 ? all : 0, lp, nhg, k);
+            const float cost = chunk_cost(chunk_blocks(tiles, (int)nb, bm, window), all, k > 1 ? all : 0, lp, nhg, k, p.kvg);
             if (cost < best) {
                 best = cost;
                 p.pieces = k;
@@ -290,7 +293,7 @@ __device__ __forceinline__ int chunk_choose(const PagedBatch& b, const ChunkPlan
         items += n * ts;
         recs += n > 1 ? n * ts : 0;
     }
-    float cost = chunk_cost(total, items, recs, lp, p.nhg, chunk_pieces(longest, lp, inv));
+    float cost = chunk_cost(total, items, recs, lp, p.nhg, chunk_pieces(longest, lp, inv), p.kvg);
     if (items > p.items || recs > p.room) cost = 3.0e38f;
     if (lane == 0) cost = fminf(cost, 1.0e38f);   // (one piece a tile always fits)
     // (costs are positive: they order as integers)
