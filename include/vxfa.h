@@ -82,7 +82,8 @@ typedef struct vxfa_tensor {
  * records (8 MiB at most: partial O, running max and sum per split), or a
  * prefill call's f16 copies of F32 K/V (32 MiB at most: K and V of up to 8192
  * rows of 8 x 128), mask row intervals, rotated queries and records of KV
- * pieces. No other call allocates, frees or synchronises, so every call
+ * pieces, or what a paged call needs (records, scores and row sums, numbers of
+ * kept rows). No other call allocates, frees or synchronises, so every call
  * can be captured into a HIP graph; a call whose records would need more
  * runs with fewer splits or pieces, a
  * prefill call with F32 K/V beyond the 32 MiB returns VXFA_NO_WORKSPACE. The

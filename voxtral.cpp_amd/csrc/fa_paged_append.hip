@@ -6,7 +6,9 @@
 // is rounded once, F32 -> f16 to nearest even. One workgroup per packed token:
 // it looks its stream up in q_start (by bisection), its page in the table,
 // forms the cos / sin of its position once for all heads, and converts 8
-// elements per thread and step (two 16-byte loads, one 16-byte store).
+// elements per thread and step (two 16-byte loads, one 16-byte store). Bound by
+// HBM: 8192 tokens of 32 + 8 + 8 heads of 128 57 us, 5.3 TB/s read and written;
+// 32 tokens 4.4 us in a graph (launch cadence and three dependent loads).
 #include "fa_paged.h"
 
 namespace vxfa {

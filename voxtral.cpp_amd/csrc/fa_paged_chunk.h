@@ -14,9 +14,9 @@
 //   all lanes weigh a piece length each). Long streams come first, and long
 //   tiles within a stream.
 //   Rows. A load instruction fills 4 (8) rows, which lie in one 16-row granule
-//   and so in one page: its base is that page's, a scalar. The granules'
-//   pages are read 64 at a time, a lane each. Rows past the stream's end and
-//   absent pages read a row of zeros.
+//   and so in one page: its base is a scalar. The granules' pages are read, and
+//   their addresses worked out, 64 at a time, a lane each. Absent pages and rows
+//   past the stream's last granule read a row of zeros.
 //   Scores. MOD 1: with the distance term, two FMAs a score where the plain
 //   softmax has one (slope j + (slope (kv0 - p) - m), then c s + that); MOD 2: with
 //   a cap, too. These walk a tile's blocks from the last: far rows lie lower by
@@ -29,8 +29,12 @@
 //   workgroup has one wavefront a SIMD, and the chain of a block's dependent steps
 //   takes 0.6 us (600 tokens on 3000 rows, 20 heads: 41.3 -> 35.5 us; with 320
 //   workgroups, two on some CUs either way, 41 -> 50).
-// What bounds it: see fa_prefill_group.hip; with a cap the two further
-// transcendentals a score (exp2, reciprocal).
+// What bounds it, 32/8 heads of 128: 8192 tokens 554-579 us, 0.95-0.99 PFLOP/s (power,
+// as fa_prefill_group.hip; matrix pipe busy 49 % of the cycles); with slopes 565,
+// with a cap 748 (the VALU: exp2 and reciprocal a score more). 600 tokens on 3000
+// rows 53 us, 3 pieces: 38 blocks of ~0.9 us, ~8 before and after, 7 for the join.
+// 16 streams of up to 512 tokens and 4096 rows, half of them single tokens, cap and
+// slopes 208-220 us: 416 workgroups of 8 to 128 blocks, one a CU; VALU 56 % busy.
 #pragma once
 
 #include "fa_paged.h"

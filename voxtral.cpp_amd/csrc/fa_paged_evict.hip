@@ -13,6 +13,10 @@
 //   a time).
 //   paged_move_kernel: 8 kept rows a wavefront, K and V at once, 16 bytes a lane,
 //   the four loads of a lane in flight together.
+// Measured, 8 kv heads of 128: 32 streams of up to 8192 rows to 1000 74 us (the move
+// 52: 5.1 TB/s read and written, what a large copy reaches), one stream of 8192 to
+// 4096 22 us: 14 the selection, whose 8 workgroups are a chain of loads, three
+// passes of about 2 us and the list, 8 the move.
 #include "fa_paged.h"
 
 namespace vxfa {

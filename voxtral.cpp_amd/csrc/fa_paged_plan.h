@@ -15,9 +15,14 @@ inline int rows_heads(int group) {
     return n > 0 ? (group + n - 1) / n : 1;
 }
 
+// All streams' rows are cut into `small` parts per head group (512 workgroups), two
+// a CU at once; where these would hold more than `limit` rows, into parts of that
+// many, up to `large` (2048 workgroups), so that streams of uneven lengths leave no
+// long last round. (Parts of 1024 rows: 16 equal streams of 8192 107.9 -> 103.7 us,
+// 32 uneven ones with weights 151.6 -> 155.3; of 2048: uneven ones +3 to 7 %.)
 struct RowsPlan {
-    int32_t small, large;     // parts (per head group) that all streams' rows are cut into
-    int32_t limit;            // rows of a part from which `large` holds
+    int32_t small, large;
+    int32_t limit;
     int32_t cuts;             // 0: a part per stream
     int32_t empty;            // 1: one, too, for a stream without tokens
 };

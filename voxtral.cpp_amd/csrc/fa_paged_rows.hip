@@ -3,7 +3,10 @@
 //
 // The paged form of fa_decode.hip's decode step (src/voxtral.cpp:1802 with
 // n_tokens = 1), for a ragged batch: up to 16 query rows (tokens x query heads
-// of a kv head) share each K/V row that is read. Bound by HBM.
+// of a kv head) share each K/V row that is read. Bound by HBM. Measured, 32/8
+// heads of 128: 32 streams of up to 8192 rows 117 us (4.97 TB/s of K and V, what a
+// large copy reaches), one full stream 10.1 us in a graph (6.5 of them this kernel,
+// 3 the join), the first token of a prompt 4.1 (launch cadence).
 //
 // Work: the rows of all streams together are cut into parts of `chunk` rows,
 // a workgroup of four wavefronts for each part and head group; every
@@ -22,7 +25,14 @@
 // product, its sum taken before that rounding.
 // The four wavefronts join through LDS; a stream of one part is finished
 // there, else each part leaves (O, m, l) and paged_rows_combine joins them
-// in order.
+// in order. Short streams are left whole (rows_whole in fa_paged_plan.h).
+// Accumulated weights: the kernel leaves its scores (4 bytes a row and query row,
+// against 512 of K and V), paged_rows_weights sums 2^(x - lse) when the row sums
+// are known, or the workgroup itself where streams are whole: 32 streams of up to
+// 8192 rows 117 -> 152 us, of up to 512 11.4 -> 13.8; forming the scores again from
+// K (where they do not fit the scratch) took 240. Of the 35 us 16 are the stores,
+// 14 the sums. Kept in LDS and stored 8 tiles at a time they gained 3 %,
+// nontemporal stores lost 2.
 #include "fa_paged.h"
 #include "fa_paged_plan.h"
 
@@ -51,10 +61,10 @@ struct RowsArgs {
 template <int N>
 __device__ __forceinline__ void pr_wait_vm() {
     static_assert(N >= 0 && N < 64, "vmcnt range");
-    __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (15 << 8) | ((N >> 4) << 14));
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 // LDS reads done: their slot may be written again
-__device__ __forceinline__ void pr_wait_lds() { __builtin_amdgcn_s_waitcnt(15 | (7 << 4) | (3 << 14)); }
+__device__ __forceinline__ void pr_wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
 __device__ __forceinline__ float quad_max(float x) {   // over lanes l ^ 16, l ^ 32
     const int xi = __builtin_bit_cast(int, x);
@@ -177,7 +187,6 @@ __global__ __launch_bounds__(64 * PR_WAVES, 2) void paged_rows_kernel(RowsArgs r
         } else {
             pr_wait_vm<0>();
         }
-        asm volatile("" ::: "memory");
         if (!(((k >= ids_from ? there : there_before) >> (k & 63)) & 1)) continue;   // an absent page
         const char* slot = mine + (k & (NS - 1)) * TILE;
         floatx4 s = {0.f, 0.f, 0.f, 0.f};
