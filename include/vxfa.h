@@ -309,9 +309,9 @@ int vxfa_flash_attn_ext_noalloc(const vxfa_tensor* q, const vxfa_tensor* k,
  * t lies in row p = n_kv[s] - t + i. The tables and sizes are device memory,
  * read when the kernels run, so a captured call follows them from replay to
  * replay; the host gives bounds. Values out of range do no harm: n_kv is
- * taken as at most max_nkv, q_start as within the call's tokens and not
- * decreasing, a row p below 0 takes no part, and tokens past max_nq of a
- * stream are left out. Rows of q and dst behind the last stream's are neither
+ * taken as at most max_nkv (2^30 at most), q_start as within the call's tokens
+ * and not decreasing, a row p below 0 takes no part, and tokens past max_nq of
+ * a stream are left out; where chunks overlap, outputs may stay unwritten. Rows of q and dst behind the last stream's are neither
  * read nor written. */
 typedef struct vxfa_paged {
     const int32_t* pages;    /* device [n_streams][max_pages]                        */
@@ -331,7 +331,8 @@ typedef struct vxfa_paged {
  * be the rows' numbers) K is rotated first as by vxfa_flash_attn_ext_rope,
  * and, with q (F32 [D, T, Hq, 1]) and q_out (F16, same ne), so are the
  * queries, rounded to f16 into q_out; q and q_out come together and need rope.
- * Two tokens of one row (streams that share a page) leave one of them.
+ * Two tokens of one row (streams that share a page) leave either's values, 8
+ * elements at a time.
  * One launch; asynchronous on `stream`. */
 int vxfa_paged_append(vxfa_ctx* ctx, const vxfa_tensor* k_new,
                       const vxfa_tensor* v_new, const vxfa_paged* batch,
@@ -385,9 +386,9 @@ typedef struct vxfa_evict {
 
 /* Keep the best rows of every stream, for each kv head its own: the kept rows
  * of k, v and weights move, in their order, to rows 0, 1, .. of the pages that
- * evict->pages names, pages of the same pool that no stream of the call lies
- * in (streams may share pages, which an eviction in place would spoil for the
- * others). The old pages are left as they were. batch->q_start, max_nq and
+ * evict->pages names, each at most once, pages of the same pool that no stream
+ * of the call lies in (streams may share pages, which an eviction in place
+ * would spoil for the others). The old pages are left as they were. batch->q_start, max_nq and
  * window are not looked at. Rows that lie in absent pages count as rows of
  * weight NaN and of zeros. Afterwards row numbers are no longer token
  * positions: the distances and windows of further calls go by rows. Needs

@@ -173,6 +173,12 @@ int main() {
         c.cap = 20.f;
         c.bias = 8.f;
         CHECK(attend(c, true, false) == VXFA_OK && g_attn.window == 32 && !g_attn.w_in && g_attn.cap > 28.f && g_attn.n2 == 8 && g_attn.bias1 == -1.f);
+        const size_t nb2 = c.dst.nb[2];
+        c.q.ne[2] = c.dst.ne[1] = 0;   // no heads: nothing of q is read, the weights are taken over
+        c.dst.nb[2] = 0;
+        CHECK(attend(c) == VXFA_OK && g_attn.b.max_nq == 0);
+        c.q.ne[2] = c.dst.ne[1] = 8;
+        c.dst.nb[2] = nb2;
         const int before = g_launches;
         c.b.max_nq = 0;
         CHECK(attend(c, false, false) == VXFA_OK && g_launches == before);
@@ -188,6 +194,7 @@ int main() {
     { Call c; CHECK(append(c, false, false) == VXFA_OK && !g_append.rope_pos && !g_append.q); }
     { Call c; CHECK(evict(c) == VXFA_OK && g_last == "evict" && g_evict.kept_row == 50 && g_evict.kept == c.e.kept); }
     { Call c; c.e.kept = nullptr; c.e.budget = 1000; CHECK(evict(c) == VXFA_OK && g_evict.kept_row == 160 && (char*)g_evict.kept == g_ctx.ws); }
+    { Call c; c.b.max_pages = 0x7fffffff; c.e.budget = 1 << 20; CHECK(evict(c) == VXFA_OK && g_evict.b.max_nkv == 1 << 30); }
     { Call c; c.b.q_start = nullptr; c.b.n_streams = 0; CHECK(evict(c) == VXFA_OK); }
     CHECK(vxfa_flash_attn_ext_paged(nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, 0, 0, 0, nullptr, nullptr, nullptr) == VXFA_INVALID_ARG);
     CHECK(vxfa_paged_append(nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr) == VXFA_INVALID_ARG);
@@ -235,6 +242,9 @@ int main() {
     REFUSES(attend, VXFA_INVALID_ARG, c.w.ne[2] = 99);
     REFUSES(attend, VXFA_UNSUPPORTED, c.w.type = VXFA_TYPE_F16);
     REFUSES(attend, VXFA_UNSUPPORTED, c.w_in.nb[1] += 2);
+    REFUSES(attend, VXFA_UNSUPPORTED, c.scale = 1.f; c.cap = 1e-39f);
+    REFUSES(attend, VXFA_UNSUPPORTED, c.scale = 3e38f);
+    REFUSES(attend, VXFA_UNSUPPORTED, c.b.max_pages = 0x7fffffff; c.k.ne[2] = c.v.ne[2] = c.w.ne[1] = c.w_in.ne[1] = 8);
     REFUSES(attend, VXFA_NO_WORKSPACE, c.q.ne[1] = c.dst.ne[2] = 2000000);
     { Call c; CHECK(attend(c, false, true) == VXFA_INVALID_ARG); }
     // append
@@ -253,6 +263,7 @@ int main() {
     { Call c; CHECK(append(c, false, true) == VXFA_INVALID_ARG); }
     // eviction
     REFUSES(evict, VXFA_INVALID_ARG, c.e.budget = 0);
+    REFUSES(evict, VXFA_UNSUPPORTED, c.e.budget = (1 << 30) + 1);
     REFUSES(evict, VXFA_INVALID_ARG, c.e.n_sink = 45);
     REFUSES(evict, VXFA_INVALID_ARG, c.e.n_recent = -1);
     REFUSES(evict, VXFA_INVALID_ARG, c.e.pages = nullptr);

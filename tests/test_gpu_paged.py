@@ -152,7 +152,7 @@ def test_sizes_out_of_range_do_no_harm(ctx, t):
     import torch
     c = Batch([(100, t), (60, t), (90, t)], seed=2)
     for n_kv, q_start in (([2 ** 31 - 1, -5, 90], [0, t, 2 * t, 3 * t]), ([100, 60, 90], [-7, t, 5 * t, 2 ** 31 - 1]),
-                          ([100, 60, 90], [2 * t, t, 0, 3 * t])):
+                          ([100, 60, 90], [2 * t, t, 0, 3 * t]), ([100, 60, 90], [0, 3 * t, 0, 3 * t])):
         for limit in (t, 1):
             d = Device(c)
             d.n_kv.copy_(torch.from_numpy(np.array(n_kv, np.int32).view(np.uint8)))
@@ -330,6 +330,20 @@ def test_no_pages_at_all(ctx, t):
     assert (d.dt == 0xA5).all()
 
 
+def test_rising_scores_with_slopes(ctx):
+    """Keys that grow along the rows, the nearest the largest or the smallest, under distance slopes: the walk from the last block, too, has
+    to follow a rising maximum."""
+    for t in (1, 3, 70):
+        for lo, hi in ((0.1, 12.0), (12.0, 0.1)):
+            c = Batch([(700, t), (1500, t)], seed=27)
+            g = np.linspace(lo, hi, 1500).astype(np.float16)
+            for s, (n, _) in enumerate(c.sizes):
+                r = np.arange(n)
+                c.k[c.table[s, r // c.page], r % c.page] *= g[:n, None, None]
+            attend(ctx, c, scale=0.4, bias=8.0, weights="new")
+            attend(ctx, c, scale=0.4, bias=1.0, cap=60.0)
+
+
 # ---- append ----------------------------------------------------------------------
 
 
@@ -494,6 +508,53 @@ def test_evict_absent_pages(ctx):
     c = Batch([(400, 0), (100, 0)], absent=[(0, 0), (0, 3), (1, 6)], seed=5, spare=2 * 20)
     evict(ctx, c, 130, 20, 30)
     evict(ctx, c, 130, 20, 30, drop=[(0, 1), (1, 0)])
+
+
+def test_captured_step_of_all_three(ctx):
+    """Append, attention with weights and eviction in one graph, replayed on other sizes with eager work in between, against the same calls
+    made directly."""
+    import torch
+    from gpu_util import vxfa
+    T, hkv, hd, page = 3, 2, 128, 16
+    c = Batch([(300, 1), (300, 1), (300, 1)], 8, hkv, hd, page, seed=28, spare=3 * 6)
+    new = torch.randn((2, T, hkv * hd), device="cuda")
+    pos = torch.tensor([299, 5, 1000], device="cuda", dtype=torch.int32)
+    to = torch.from_numpy(c.free[:18].reshape(3, 6).copy()).cuda()
+    w = hkv * hd
+
+    def bind(d):
+        nd = [vxfa.desc(x.data_ptr(), vxfa.F32, (w, T, 1, 1), (4, 4 * w, 4 * w * T, 4 * w * T)) for x in new]
+        kept = torch.full((3, hkv, 90), -7, device="cuda", dtype=torch.int32)
+        ev = vxfa.evict(to.data_ptr(), 6, 90, 4, 20, kept=kept.data_ptr())
+        rope = vxfa.rope(pos.data_ptr(), hd, 1e6)
+
+        def step(s):
+            ctx.paged_append(*nd, d.batch, d.k, d.v, rope=rope, stream=s)
+            ctx.flash_attn_ext_paged(d.q, d.k, d.v, d.batch, d.dst, 0.09, 2.0, 20.0, weights_in=d.w, weights=d.w, stream=s)
+            ctx.paged_evict(d.k, d.v, d.w, d.batch, ev, stream=s)
+        return step, kept
+
+    a, b = Device(c), Device(c)
+    (sa, ka), (sb, kb) = bind(a), bind(b)
+    st = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=st):
+        sa(st.cuda_stream)
+    for sizes in ([300, 250, 120], [299, 33, 300], [100, 300, 17]):
+        n = torch.from_numpy(np.array(sizes, np.int32).view(np.uint8)).cuda()
+        for d in (a, b):
+            d.n_kv.copy_(n)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        attend(ctx, Batch([(900, 40), (70, 1)], seed=29), weights="new")
+        sb(torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+        assert torch.equal(ka, kb) and torch.equal(a.dt, b.dt)
+        assert torch.equal(a.wt.view(torch.int32), b.wt.view(torch.int32))
+        for name in "kv":
+            assert torch.equal(a.pools[name][0], b.pools[name][0])
 
 
 def test_serving_run(ctx):

@@ -171,9 +171,22 @@ hipError_t launch_paged_append(const PagedAppend& a, hipStream_t st);
 bool paged_rows_takes(const PagedAttn& a);
 // weighed: the accumulated weights are done, too (else launch_paged_weights)
 hipError_t launch_paged_rows(const PagedAttn& a, int head_dim, hipStream_t st, bool& weighed);
-// any chunks
+// any chunks (hipErrorOutOfMemory, as from launch_paged_rows: the workspace does not
+// hold the work's tables)
 hipError_t launch_paged_chunk(const PagedAttn& a, int head_dim, hipStream_t st);
 hipError_t launch_paged_chunk64(const PagedAttn& a, hipStream_t st);
+// what the launches below take: workgroups along x
+constexpr int kPagedWeightRows = 128;        // rows of a workgroup of the weights
+constexpr int kPagedMoveRows = 32;           // of the eviction's move
+inline bool paged_weights_fit(const PagedAttn& a) {
+    return ((int64_t)a.b.max_nkv + kPagedWeightRows - 1) / kPagedWeightRows * a.hkv <= kMaxGridX;
+}
+inline int64_t paged_move_grid(const PagedEvict& a) {
+    const int64_t rows = a.kept_row < a.b.max_nkv ? a.kept_row : a.b.max_nkv;   // kept of a stream at most
+    return (rows + kPagedMoveRows - 1) / kPagedMoveRows * a.hkv;
+}
+inline bool paged_evict_fits(const PagedEvict& a) { return paged_move_grid(a) <= kMaxGridX; }
+
 hipError_t launch_paged_weights(const PagedAttn& a, int head_dim, hipStream_t st);
 hipError_t launch_paged_evict(const PagedEvict& a, hipStream_t st);
 

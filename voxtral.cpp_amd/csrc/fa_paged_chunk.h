@@ -633,7 +633,7 @@ static hipError_t launch_chunk(const PagedAttn& a, hipStream_t st) {
     ca.p.pieces = a.pieces;
     const ChunkBounds cb = chunk_plan(a.b, HD, ca.nhg, 32 * (P::NW >> l2), a.window, (size_t)P::NW * P::REC * sizeof(float), a.ws_bytes, ca.p);
     ca.p.hpw_log2 = l2;
-    if (cb.table > a.ws_bytes) return hipErrorInvalidValue;   // (16 bytes a tile: 2.5 million of them fit)
+    if (cb.table > a.ws_bytes) return hipErrorOutOfMemory;    // (16 bytes a tile: 2.5 million of them fit)
     ca.tiles = reinterpret_cast<ChunkTile*>(a.ws);
     ca.rec = reinterpret_cast<float*>(a.ws + cb.table);
     const int64_t nwg = (int64_t)ca.p.items * ca.nhg;

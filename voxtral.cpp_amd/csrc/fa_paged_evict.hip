@@ -146,12 +146,13 @@ __global__ __launch_bounds__(SEL_NT) void paged_select_kernel(PagedEvict a) {
     for (int r = done + tid; r < a.kept_row; r += SEL_NT) kept[r] = -1;
 }
 
+static_assert(kPagedMoveRows == 4 * 8, "four wavefronts");
 template <int D>
 __global__ __launch_bounds__(256) void paged_move_kernel(PagedEvict a) {
     constexpr int CH = D / 8, RPW = 64 / (2 * CH);   // rows of one step: CH lanes of K, CH of V each
     constexpr int U = 8 / RPW;
     const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
-    const int h = (int)blockIdx.x % a.hkv, r0 = ((int)blockIdx.x / a.hkv * 4 + wave) * 8, s = (int)blockIdx.y;
+    const int h = (int)blockIdx.x % a.hkv, r0 = (int)blockIdx.x / a.hkv * kPagedMoveRows + 8 * wave, s = (int)blockIdx.y;
     const int lg = a.b.ps_log2, mask = (1 << lg) - 1;
     const int32_t* kept = a.kept + ((int64_t)s * a.hkv + h) * a.kept_row;
     char* const pool = ((lane / CH) & 1 ? a.kv.v : a.kv.k) + 16 * (lane % CH);
@@ -187,15 +188,14 @@ __global__ __launch_bounds__(256) void paged_move_kernel(PagedEvict a) {
 
 hipError_t launch_paged_evict(const PagedEvict& a, hipStream_t st) {
     if (a.b.n_streams <= 0 || a.kept_row <= 0) return hipSuccess;
+    if (!paged_evict_fits(a) || (a.d != 64 && a.d != 128)) return hipErrorInvalidValue;
     hipLaunchKernelGGL(paged_select_kernel, dim3((unsigned)a.b.n_streams, (unsigned)a.hkv), dim3(SEL_NT), 0, st, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    const int64_t gx = ((int64_t)a.kept_row + 31) / 32 * a.hkv;
-    if (gx > kMaxGridX) return hipErrorInvalidValue;
-    const dim3 grid((unsigned)gx, (unsigned)a.b.n_streams);
+    const dim3 grid((unsigned)paged_move_grid(a), (unsigned)a.b.n_streams);
+    if (grid.x == 0) return e;
     if (a.d == 128) hipLaunchKernelGGL((paged_move_kernel<128>), grid, dim3(256), 0, st, a);
-    else if (a.d == 64) hipLaunchKernelGGL((paged_move_kernel<64>), grid, dim3(256), 0, st, a);
-    else return hipErrorInvalidValue;
+    else hipLaunchKernelGGL((paged_move_kernel<64>), grid, dim3(256), 0, st, a);
     return hipGetLastError();
 }
 

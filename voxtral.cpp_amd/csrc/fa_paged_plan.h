@@ -354,7 +354,8 @@ __device__ __forceinline__ ChunkItem chunk_locate(const PagedBatch& b, const Chu
         r.tiles += tall;
         if (hit && item > 0) return r;              // (the first one goes on to count the tiles)
     }
-    r.tiles = min(r.tiles, p.tiles);
+    // (sizes that break the bounds: tiles of which no workgroup knows are not joined)
+    r.tiles = before > p.items ? 0 : min(r.tiles, p.tiles);
     return r;
 }
 #endif

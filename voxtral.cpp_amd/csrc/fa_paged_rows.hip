@@ -426,7 +426,7 @@ hipError_t launch_paged_rows(const PagedAttn& a, int head_dim, hipStream_t st, b
     ra.rec = (ra.rows * (head_dim + 2) + 3) & ~3;
     const int nhg = a.hkv * ra.groups;
     const size_t cut = ((size_t)a.b.n_streams * sizeof(int2) + 255) & ~(size_t)255;
-    if (cut > a.ws_bytes) return hipErrorInvalidValue;   // (65535 streams at most: half a MiB)
+    if (cut > a.ws_bytes) return hipErrorOutOfMemory;    // (65535 streams at most: half a MiB)
     ra.cut = reinterpret_cast<int2*>(a.ws);
     size_t used = cut;
     // scores, if they leave the records' usual room; else the weights form them again
@@ -460,8 +460,7 @@ hipError_t launch_paged_rows(const PagedAttn& a, int head_dim, hipStream_t st, b
         if (e != hipSuccess) return e;
     }
     if (!ra.x || ra.whole) return e;
-    const int64_t gx = ((int64_t)a.b.max_nkv + 1023) / 1024 * a.hkv;
-    if (gx > kMaxGridX) return hipErrorInvalidValue;
+    const int64_t gx = ((int64_t)a.b.max_nkv + 1023) / 1024 * a.hkv;   // (paged_weights_fit's are more)
     hipLaunchKernelGGL(paged_rows_weights, dim3((unsigned)gx, (unsigned)a.b.n_streams), dim3(256), 0, st, ra);
     return hipGetLastError();
 }

@@ -22,7 +22,7 @@
 
 namespace vxfa {
 
-constexpr int PW_ROWS = 128;
+constexpr int PW_ROWS = kPagedWeightRows;
 
 struct WeightsArgs {
     PagedAttn a;
@@ -212,7 +212,7 @@ hipError_t launch_paged_weights(const PagedAttn& a, int head_dim, hipStream_t st
     wa.a = a;
     wa.grp = DivMod::make((uint32_t)(a.hq / a.hkv > 0 ? a.hq / a.hkv : 1));
     wa.ntiles = (int32_t)(((int64_t)a.b.max_nkv + PW_ROWS - 1) / PW_ROWS);
-    if ((int64_t)wa.ntiles * a.hkv > kMaxGridX) return hipErrorInvalidValue;
+    if (!paged_weights_fit(a)) return hipErrorInvalidValue;
     const dim3 grid((unsigned)(wa.ntiles * a.hkv), (unsigned)a.b.n_streams);
     if (head_dim == 128) launch_pw<128>(wa, grid, st);
     else if (head_dim == 64) launch_pw<64>(wa, grid, st);

@@ -84,6 +84,8 @@ int check_pool(const vxfa_tensor* k, const vxfa_tensor* v, const vxfa_paged* b, 
     return VXFA_OK;
 }
 
+constexpr int64_t kMaxRows = (int64_t)1 << 30;
+
 PagedBatch batch_of(const vxfa_paged* b, const vxfa_tensor* k, int64_t tokens) {
     PagedBatch r;
     r.pages = b->pages; r.n_kv = b->n_kv; r.q_start = b->q_start;
@@ -94,9 +96,9 @@ PagedBatch batch_of(const vxfa_paged* b, const vxfa_tensor* k, int64_t tokens) {
     while (((int64_t)1 << r.ps_log2) < k->ne[1]) ++r.ps_log2;
     r.tokens = (int32_t)tokens;
     r.max_nq = b->max_nq;
-    // (rows are 32-bit numbers; room for a block past the last)
+    // (rows, and sums and differences of two of their numbers, fit 32 bits)
     int64_t rows = (int64_t)b->max_pages << r.ps_log2;
-    if (rows > 0x7fff0000) rows = 0x7fff0000;
+    if (rows > kMaxRows) rows = kMaxRows;
     r.max_nkv = (int32_t)(b->max_nkv > 0 && b->max_nkv < rows ? b->max_nkv : rows);
     if (r.n_pages == 0) r.max_nkv = 0;   // (an absent page's rows may be loaded from page 0)
     return r;
@@ -238,6 +240,9 @@ int vxfa_flash_attn_ext_paged(vxfa_ctx* c, const vxfa_tensor* q, const vxfa_tens
         return fail(c, VXFA_UNSUPPORTED, "q rows must be contiguous and 16-byte aligned");
     if (!isfinite(scale) || !isfinite(max_bias) || !isfinite(logit_softcap) || max_bias < 0 || logit_softcap < 0)
         return fail(c, VXFA_UNSUPPORTED, "scale, max_bias and logit_softcap must be finite, the latter two not negative");
+    const float c_score = logit_softcap > 0 ? 2.0f * vxfa::kLog2e * (scale / logit_softcap) : scale * vxfa::kLog2e;
+    if (!isfinite(c_score) || !isfinite(logit_softcap * vxfa::kLog2e))
+        return fail(c, VXFA_UNSUPPORTED, "scale and logit_softcap: their ratio is out of range");
     if (T > kMaxTokens || Hq > 65535) return fail(c, VXFA_UNSUPPORTED, "sizes beyond the launch limits");
     if (weights_in && !weights) return fail(c, VXFA_INVALID_ARG, "weights_in without weights");
     if (weights && (rc = check_weights(weights, k, &why)) != VXFA_OK) return fail(c, rc, "%s", why);
@@ -246,6 +251,7 @@ int vxfa_flash_attn_ext_paged(vxfa_ctx* c, const vxfa_tensor* q, const vxfa_tens
     vxfa::PagedAttn a;
     memset(&a, 0, sizeof(a));
     a.b = batch_of(batch, k, T);
+    if (Hq == 0) a.b.max_nq = 0;   // (nothing of q is read)
     a.q = q->data;
     a.q_nb1 = (int64_t)q->nb[1]; a.q_nb2 = (int64_t)q->nb[2];
     a.kv = pool_of(k, v);
@@ -255,11 +261,8 @@ int vxfa_flash_attn_ext_paged(vxfa_ctx* c, const vxfa_tensor* q, const vxfa_tens
     a.hq = (int32_t)Hq;
     a.hkv = (int32_t)Hkv;
     a.window = batch->window < a.b.max_nkv ? batch->window : 0;   // (a window of all rows is none)
-    a.c = scale * vxfa::kLog2e;
-    if (logit_softcap > 0) {
-        a.c = 2.0f * vxfa::kLog2e * (scale / logit_softcap);
-        a.cap = logit_softcap * vxfa::kLog2e;
-    }
+    a.c = c_score;
+    if (logit_softcap > 0) a.cap = logit_softcap * vxfa::kLog2e;
     if (max_bias > 0 && Hq > 0) {
         int64_t n2 = 1;
         while (2 * n2 <= Hq) n2 *= 2;
@@ -270,6 +273,7 @@ int vxfa_flash_attn_ext_paged(vxfa_ctx* c, const vxfa_tensor* q, const vxfa_tens
     a.ws = c->ws;
     a.ws_bytes = kWorkspaceBytes;
     if (weights) {
+        if (!vxfa::paged_weights_fit(a)) return fail(c, VXFA_UNSUPPORTED, "sizes beyond the launch limits");
         const size_t lse = ((size_t)T * (size_t)Hq * sizeof(float) + 255) & ~(size_t)255;
         if (lse > a.ws_bytes)
             return fail(c, VXFA_NO_WORKSPACE, "weights need %zu bytes; the workspace holds %zu", lse, a.ws_bytes);
@@ -293,6 +297,7 @@ int vxfa_flash_attn_ext_paged(vxfa_ctx* c, const vxfa_tensor* q, const vxfa_tens
     if (T * Hq > 0 && a.b.n_streams > 0 && a.b.max_nq > 0)
         e = vxfa::paged_rows_takes(a) ? vxfa::launch_paged_rows(a, (int)D, st, weighed) : vxfa::launch_paged_chunk(a, (int)D, st);
     if (e == hipSuccess && weights && !weighed) e = vxfa::launch_paged_weights(a, (int)D, st);
+    if (e == hipErrorOutOfMemory) return fail(c, VXFA_NO_WORKSPACE, "the tables of the call's work do not fit the workspace");
     if (e != hipSuccess) return fail(c, VXFA_HIP_ERROR, "paged attention: %s", hipGetErrorString(e));
     return VXFA_OK;
 }
@@ -311,6 +316,7 @@ int vxfa_paged_evict(vxfa_ctx* c, vxfa_tensor* k, vxfa_tensor* v, vxfa_tensor* w
     if (ev->max_pages < 0 || (ev->max_pages > 0 && !ev->pages) || !aligned(ev->pages, 4) || !aligned(ev->kept, 4) || !aligned(ev->n_kv, 4))
         return fail(c, VXFA_INVALID_ARG, "evict: pages are required, arrays 4-byte aligned");
     if (ev->n_kv && ev->n_kv == batch->n_kv) return fail(c, VXFA_INVALID_ARG, "evict: n_kv must not be the batch's");
+    if (ev->budget > kMaxRows) return fail(c, VXFA_UNSUPPORTED, "sizes beyond the launch limits");
     vxfa::PagedEvict a;
     memset(&a, 0, sizeof(a));
     a.b = batch_of(batch, k, 0);
@@ -334,6 +340,7 @@ int vxfa_paged_evict(vxfa_ctx* c, vxfa_tensor* k, vxfa_tensor* v, vxfa_tensor* w
             return fail(c, VXFA_NO_WORKSPACE, "the kept rows' numbers need %zu bytes; the workspace holds %zu", need, kWorkspaceBytes);
         a.kept = reinterpret_cast<int32_t*>(c->ws);
     }
+    if (!vxfa::paged_evict_fits(a)) return fail(c, VXFA_UNSUPPORTED, "sizes beyond the launch limits");
     OnDevice on(c->device);
     if (on.e != hipSuccess) return fail(c, VXFA_HIP_ERROR, "hipSetDevice: %s", hipGetErrorString(on.e));
     const hipError_t e = vxfa::launch_paged_evict(a, reinterpret_cast<hipStream_t>(stream));
