@@ -58,6 +58,11 @@ struct RowsArgs {
     int32_t whole;            // no stream is cut and no group shared: the weights need no launch of their own
 };
 
+// dma16 with a nontemporal hint: rows are read once
+__device__ __forceinline__ void dma16_nt(const char* base, uint32_t off, uint32_t lds) {
+    asm volatile("global_load_lds_dwordx4 %0, %1 nt" ::"v"(off), "s"(base), "{m0}"(lds) : "memory");
+}
+
 template <int N>
 __device__ __forceinline__ void pr_wait_vm() {
     static_assert(N >= 0 && N < 64, "vmcnt range");
@@ -160,12 +165,12 @@ __global__ __launch_bounds__(64 * PR_WAVES, 2) void paged_rows_kernel(RowsArgs r
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
             const int r = RPI * i + lane / CH, c = lane % CH;
-            dma16(kp, (uint32_t)min(r, last) * (uint32_t)a.kv.nb1 + ((c ^ swk(r)) * 16), slot + RPI * i * ROW);
+            dma16_nt(kp, (uint32_t)min(r, last) * (uint32_t)a.kv.nb1 + ((c ^ swk(r)) * 16), slot + RPI * i * ROW);
         }
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
             const int r = RPI * i + lane / CH, c = lane % CH;
-            dma16(vp, (uint32_t)min(r, last) * (uint32_t)a.kv.nb1 + ((c ^ swv(r)) * 16), slot + MAT + RPI * i * ROW);
+            dma16_nt(vp, (uint32_t)min(r, last) * (uint32_t)a.kv.nb1 + ((c ^ swv(r)) * 16), slot + MAT + RPI * i * ROW);
         }
     };
     for (int k = 0; k < min(nk, NS - 1); ++k) issue(k);
