@@ -42,7 +42,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppend a) {
         const char* src = m == 0 ? (const char*)a.k_new + (int64_t)t * a.kn_nb1 + 4 * (int64_t)e
                         : m == 1 ? (const char*)a.v_new + (int64_t)t * a.vn_nb1 + 4 * (int64_t)e
                                  : (const char*)a.q + (int64_t)t * a.q_nb1 + (int64_t)h * a.q_nb2 + 4 * d;
-        const floatx4 x0 = ((const floatx4*)src)[0], x1 = ((const floatx4*)src)[1];
+        const floatx4 x0 = __builtin_nontemporal_load((const floatx4*)src), x1 = __builtin_nontemporal_load((const floatx4*)src + 1);
         float x[8] = {x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]};
         if (m != 1 && a.rope_pos) rope8_tab(x, d, cs, a.rope_dims);
         half8 y;
