@@ -7,7 +7,8 @@
 // it looks its stream up in q_start (by bisection), its page in the table,
 // forms the cos / sin of its position once for all heads, and converts 8
 // elements per thread and step (two 16-byte loads, one 16-byte store). Bound by
-// HBM: 8192 tokens of 32 + 8 + 8 heads of 128 57 us, 5.3 TB/s read and written;
+// HBM: 8192 tokens of 32 + 8 + 8 heads of 128 53.5 us, 5.6 TB/s read and
+// written (the sources' nontemporal hint: 58.3 -> 53.5; one at the stores: 54.3);
 // 32 tokens 4.4 us in a graph (launch cadence and three dependent loads).
 #include "fa_paged.h"
 

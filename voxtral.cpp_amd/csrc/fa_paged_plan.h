@@ -28,16 +28,19 @@ struct RowsPlan {
 };
 
 // Whether streams are left whole: what a cut costs (its join, a launch of its own)
-// against what it gains, by the bounds. In us: a workgroup alone takes 9.0 ns a row
-// (hd 64: 7.3), all together move 5 TB/s; the streams are taken for three quarters
-// of the bound on average, and for too uneven beyond 2048 rows. Measured, cut ->
-// whole: 1 stream of up to 256 rows 8.1 -> 5.6, 512 8.3 -> 9.2, 16 streams x 8 kv
-// heads of up to 512 12.5 -> 10.1, 4096 39.7 -> 53.0, 32 x 8 of up to 256 12.9 -> 8.3,
-// 1024 23.7 -> 17.3, 2048 40.2 -> 35.9, 8192 117 -> 128.
+// against what it gains, by the bounds. In us: a workgroup alone takes about 10.5 ns
+// a row (hd 64: 6.5), all together move 5.6 TB/s; the streams are taken for seven
+// tenths of the bound on average, and for too uneven beyond 2048 rows. Measured, cut
+// -> whole, 8 kv heads of 128: 1 stream of 256 rows 8.5 -> 7.1, of 512 8.6 -> 9.8; 4
+// uneven ones of up to 256 8.8 -> 6.9, 1024 9.5 -> 12.7; 16 of up to 512 12.1 -> 10.3,
+// 2048 22.1 -> 27.5; 32 of up to 1024 24.2 -> 18.3, 2048 35.7 -> 32.4, 8192 102.8 ->
+// 117.4. Over 196 mixes of heads, streams and rows (half of them even, half uneven)
+// the rule is 0.5 % off the better choice on average, 15 % at worst: 1 stream
+// that is shorter than its bound of 512.
 inline bool rows_whole(const PagedBatch& b, int nhg, int head_dim) {
-    const double n = 1e-3 * b.max_nkv, alone = head_dim == 128 ? 9.0 : 7.3;
-    const double together = 0.75 * (double)b.n_streams * nhg * 4 * head_dim / 5000;
-    return b.max_nkv <= 2048 && 4.5 + n * (alone > together ? alone : together) < 8.0 + 1.05 * n * together;
+    const double n = 1e-3 * b.max_nkv, alone = head_dim == 128 ? 10.5 : 6.5;
+    const double together = 0.7 * (double)b.n_streams * nhg * 4 * head_dim / 5600;
+    return b.max_nkv <= 2048 && 4.5 + n * (alone > together ? alone : together) < 7.5 + 1.05 * n * together;
 }
 
 // The grid of a call: `items` parts per head group.

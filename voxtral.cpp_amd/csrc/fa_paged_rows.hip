@@ -4,9 +4,10 @@
 // The paged form of fa_decode.hip's decode step (src/voxtral.cpp:1802 with
 // n_tokens = 1), for a ragged batch: up to 16 query rows (tokens x query heads
 // of a kv head) share each K/V row that is read. Bound by HBM. Measured, 32/8
-// heads of 128: 32 streams of up to 8192 rows 117 us (4.97 TB/s of K and V, what a
-// large copy reaches), one full stream 10.1 us in a graph (6.5 of them this kernel,
-// 3 the join), the first token of a prompt 4.1 (launch cadence).
+// heads of 128: 32 streams of up to 8192 rows 105 us (5.6 TB/s of K and V, 0.89 of a
+// large read's rate; without the nontemporal hint at the tiles, which are read once,
+// 117), one full stream 10.1 us in a graph (6.5 of them this kernel, 3 the join), the
+// first token of a prompt 4.1 (launch cadence).
 //
 // Work: the rows of all streams together are cut into parts of `chunk` rows,
 // a workgroup of four wavefronts for each part and head group; every
@@ -29,10 +30,10 @@
 // Accumulated weights: the kernel leaves its scores (4 bytes a row and query row,
 // against 512 of K and V), paged_rows_weights sums 2^(x - lse) when the row sums
 // are known, or the workgroup itself where streams are whole: 32 streams of up to
-// 8192 rows 117 -> 152 us, of up to 512 11.4 -> 13.8; forming the scores again from
-// K (where they do not fit the scratch) took 240. Of the 35 us 16 are the stores,
-// 14 the sums. Kept in LDS and stored 8 tiles at a time they gained 3 %,
-// nontemporal stores lost 2.
+// 8192 rows 105 -> 133 us, of up to 512 11.4 -> 13.8; forming the scores again from
+// K (where they do not fit the scratch) took 240. Of the 28 us 16 are the stores,
+// 12 the sums (which read the scores with the same hint: 134.7 -> 132.7). Kept in LDS
+// and stored 8 tiles at a time they gained 3 %, nontemporal stores lost 2.
 #include "fa_paged.h"
 #include "fa_paged_plan.h"
 
@@ -399,7 +400,7 @@ __global__ __launch_bounds__(256) void paged_rows_weights(RowsArgs ra) {
                 for (int u = 0; u < 4; ++u) {
                     const int i = (int)ra.hpw.div((uint32_t)(r0 + u)), h = r0 + u - i * hpw;
                     const bool in = r0 + u < nrow && h < heads;
-                    y[u] = *(const floatx4*)(x + (int64_t)(in ? r0 + u : 0) * ra.xrow);
+                    y[u] = __builtin_nontemporal_load((const floatx4*)(x + (int64_t)(in ? r0 + u : 0) * ra.xrow));
                     lse[u] = a.lse[(int64_t)(st.q0 + (in ? i : 0)) * a.hq + hk * G + sub * hpw + (in ? h : 0)];
                     if (!in) lse[u] = INFINITY;    // (weight 0)
                 }
