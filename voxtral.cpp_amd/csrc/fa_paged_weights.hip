@@ -5,9 +5,9 @@
 // P_ij = 2^(x_ij - lse_i), where lse_i (the logarithm of the row sum) is only
 // known when the attention is done: the scores are formed again, from K alone,
 // half the attention's products. (Single tokens: paged_rows_kernel has left its
-// scores, and paged_weights_rows sums them; see there.)
-//   Workgroup = 128 rows of a stream and kv head, 4 wavefronts: two halves of 64
-//   rows by two halves of the query rows. S^T = K Q^T by
+// scores, and paged_rows_weights sums them; see there.)
+//   Workgroup = 128 rows of a stream and kv head, 4 wavefronts: 32 rows each, or two
+//   halves of 64 rows by two halves of the query rows (NB below). S^T = K Q^T by
 //   v_mfma_f32_32x32x16_f16: a lane has the scores of 16 rows for one query row,
 //   so lse, position and slope are one register each, and the sums over query rows
 //   stay in 16 registers a block until the end. K stays in registers; 64 query
@@ -16,7 +16,7 @@
 // One workgroup owns a row's sum: no atomics, the same bits every time.
 // Bound by its VALU work (three instructions a score, and the masks of the blocks
 // on the diagonal and at a window's edge) and each workgroup's chain of loads: 8
-// streams of 250 tokens, window 750, 20 heads of 64, 28 us (a thread per row and
+// streams of 250 tokens, window 750, 20 heads of 64, 22 us (a thread per row and
 // head, which this replaced, 331).
 #include "fa_paged.h"
 
@@ -30,17 +30,23 @@ struct WeightsArgs {
     int32_t ntiles;           // row tiles of a stream at most
 };
 
-// MOD: the scores have a cap or a distance term
+// MOD: the scores have a cap or a distance term.
+// NB blocks of 32 rows a wavefront, NB wavefronts share a step's 64 query rows: 2 at
+// hd 128, whose products wait for the query rows from LDS (2000 tokens on as many rows
+// 195 us of a call, with one block 208; 600 on 3000 with slopes 123, 129), 1 at hd 64
+// for the registers, four workgroups a CU in place of three (the window case's call 58
+// against 67, 16 streams of 100 tokens and up to 8000 rows 297 against 395).
 template <int D, bool QF16, bool MOD>
-__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void paged_weights_kernel(WeightsArgs wa) {
+__global__ __launch_bounds__(256, (D == 128 ? 2 : QF16 ? 4 : 3)) void paged_weights_kernel(WeightsArgs wa) {
     constexpr int KS = D / 16, ROW = 2 * D, CH = D / 8;
     constexpr int STEP = 64 * ROW;                  // bytes of 64 query rows
+    constexpr int NB = D == 128 ? 2 : 1, QB = 2 / NB;   // blocks of rows, of query rows a wavefront
     __shared__ __attribute__((aligned(16))) char smem[2 * STEP];
-    __shared__ float part[2][64];
+    __shared__ float part[NB == 2 ? PW_ROWS : 1];
     const PagedAttn& a = wa.a;
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int nl = lane & 31, hh = lane >> 5;
-    const int ph = wave & 1, rh = wave >> 1;        // half of the rows, of the query rows
+    const int ph = wave / NB, rh = wave % NB;       // part of the rows, of the query rows
     const int s = (int)blockIdx.y, hk = (int)blockIdx.x % a.hkv, kv0 = (int)blockIdx.x / a.hkv * PW_ROWS;
     const PagedStream st = paged_stream(a.b, s);
     if (kv0 >= st.n) return;
@@ -53,27 +59,14 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void paged_weights_kernel(Wei
     if (a.window > 0) t1 = min((int)min((int64_t)kv0 + PW_ROWS - 1 + a.window - past, (int64_t)nq), nq);
     const int r_begin = t0 * G, r_end = max(t1, t0) * G;
 
-    // ---- K: A operand, row nl of a block, dims 16 ks + 8 hh .. (rows that are not
-    // there: zeros) ------------------------------------------------------------------
-    half8 kr[2][KS];
-    int pos[2], pages[2];
-    float old[2] = {0.f, 0.f};                     // what the lane's rows have gathered so far
-    const bool writes = rh == 0 && ((nl >> 2) & 1) == hh;
+    // (the table's entries first, then the query rows, then K: the entries' latency is
+    // hidden behind the second)
+    int pos[NB], pages[NB];
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-        pos[b] = kv0 + 64 * ph + 32 * b;
+    for (int b = 0; b < NB; ++b) {
+        pos[b] = kv0 + 32 * (NB * ph + b);
         const int j = pos[b] + nl;
-        const int page = j < st.n ? paged_page(a.b, s, j >> lg) : -1;
-        pages[b] = page;
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) kr[b][ks] = half8{};
-        if (page >= 0 && r_begin < r_end) {
-            const char* p = a.kv.k + a.kv.at(page, hk, j & pmask) + 16 * hh;
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) kr[b][ks] = *(const half8*)(p + 32 * ks);
-        }
-        if (page >= 0 && writes && a.w_in)
-            old[b] = *(const float*)((const char*)a.w_in + page * a.wi_nb3 + hk * a.wi_nb2 + 4 * (int64_t)(j & pmask));
+        pages[b] = j < st.n ? paged_page(a.b, s, j >> lg) : -1;
     }
 
     constexpr int QN = QF16 ? 64 * CH / 256 : 2 * 64 * CH / 256;   // 16-byte loads of a thread
@@ -103,73 +96,106 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void paged_weights_kernel(Wei
             }
         }
     };
-    float sum[2][16];
+    // the lane's query row of each block of a step: its token, head and lse
+    int tk[QB], h[QB];
+    float lse[QB];
+    auto rows_of = [&](int r0) {
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+        for (int c = 0; c < QB; ++c) {
+            const int r = r0 + 32 * (QB * rh + c) + nl, rc = min(r, r_end - 1);
+            tk[c] = (int)wa.grp.div((uint32_t)rc);
+            h[c] = hk * G + rc - tk[c] * G;
+            const float y = a.lse[(int64_t)(st.q0 + tk[c]) * a.hq + h[c]];
+            lse[c] = r < r_end ? y : INFINITY;      // (weight 0)
+        }
+    };
+    if (r_begin < r_end) {
+        load_q(r_begin);
+        rows_of(r_begin);
+    }
+
+    // ---- K: A operand, row nl of a block, dims 16 ks + 8 hh .. (rows that are not
+    // there: zeros) ------------------------------------------------------------------
+    half8 kr[NB][KS];
+    float old[NB];                                  // what the lane's rows have gathered so far
+    const bool writes = rh == 0 && ((nl >> 2) & 1) == hh;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        const int j = pos[b] + nl, page = pages[b];
+        old[b] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) kr[b][ks] = half8{};
+        if (page >= 0 && r_begin < r_end) {
+            const char* p = a.kv.k + a.kv.at(page, hk, j & pmask) + 16 * hh;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) kr[b][ks] = *(const half8*)(p + 32 * ks);
+        }
+        if (page >= 0 && writes && a.w_in)
+            old[b] = *(const float*)((const char*)a.w_in + page * a.wi_nb3 + hk * a.wi_nb2 + 4 * (int64_t)(j & pmask));
+    }
+
+    float sum[NB][16];
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int j = 0; j < 16; ++j) sum[b][j] = 0.f;
 
-    // a step's query row of the lane: its token, head and lse
-    auto row_of = [&](int r0, int& tk, int& h) -> float {
-        const int r = r0 + 32 * rh + nl, rc = min(r, r_end - 1);
-        tk = (int)wa.grp.div((uint32_t)rc);
-        h = hk * G + rc - tk * G;
-        const float lse = a.lse[(int64_t)(st.q0 + tk) * a.hq + h];
-        return r < r_end ? lse : INFINITY;          // (weight 0)
-    };
-    int tk = 0, h = 0;
-    float lse = 0.f;
-    if (r_begin < r_end) {
-        load_q(r_begin);
-        lse = row_of(r_begin, tk, h);
-    }
     for (int r0 = r_begin, buf = 0; r0 < r_end; r0 += 64, buf ^= 1) {
         put_q(buf);
-        const int tk_now = tk, h_now = h;
-        const float lse_now = lse;
+        int p[QB];
+        float slope[QB], lse_now[QB];
+#pragma unroll
+        for (int c = 0; c < QB; ++c) {
+            p[c] = past + tk[c];
+            slope[c] = MOD ? paged_slope(a, h[c]) : 0.f;
+            lse_now[c] = lse[c];
+        }
         if (r0 + 64 < r_end) {
             load_q(r0 + 64);
-            lse = row_of(r0 + 64, tk, h);
+            rows_of(r0 + 64);
         }
         __syncthreads();                            // (the other buffer is read until the next one)
-        const int p = past + tk_now, first = a.window > 0 ? p - a.window + 1 : INT32_MIN;
-        const float slope = MOD ? paged_slope(a, h_now) : 0.f;
-        half8 qb[KS];
-        const char* row = smem + buf * STEP + (32 * rh + nl) * ROW;
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) qb[ks] = *(const half8*)(row + (((2 * ks + hh) ^ (nl % CH)) * 16));
+        for (int c = 0; c < QB; ++c) {
+            const int first = a.window > 0 ? p[c] - a.window + 1 : INT32_MIN;
+            half8 qb[KS];
+            const char* row = smem + buf * STEP + (32 * (QB * rh + c) + nl) * ROW;
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            floatx16 x = {};
+            for (int ks = 0; ks < KS; ++ks) qb[ks] = *(const half8*)(row + (((2 * ks + hh) ^ (nl % CH)) * 16));
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) x = __builtin_amdgcn_mfma_f32_32x32x16_f16(kr[b][ks], qb[ks], x, 0, 0, 0);
-            // element j: row pos + 8 (j / 4) + 4 hh + j % 4
-            const int j0 = pos[b] + 4 * hh;
-            if constexpr (MOD) {
+            for (int b = 0; b < NB; ++b) {
+                floatx16 x = {};
 #pragma unroll
-                for (int j = 0; j < 16; ++j)
-                    x[j] = fmaf(slope, (float)(j0 + 8 * (j >> 2) + (j & 3) - p), paged_score(x[j], a.c, a.cap)) - lse_now;
-            } else {
+                for (int ks = 0; ks < KS; ++ks) x = __builtin_amdgcn_mfma_f32_32x32x16_f16(kr[b][ks], qb[ks], x, 0, 0, 0);
+                // element j: row pos + 8 (j / 4) + 4 hh + j % 4
+                const int j0 = pos[b] + 4 * hh;
+                if constexpr (MOD) {
 #pragma unroll
-                for (int j = 0; j < 16; ++j) x[j] = fmaf(a.c, x[j], -lse_now);
-            }
-            // (a block that all the wavefront's query rows see whole needs no mask)
-            if (__any(pos[b] + 31 > p || pos[b] < first)) {
+                    for (int j = 0; j < 16; ++j)
+                        x[j] = fmaf(slope[c], (float)(j0 + 8 * (j >> 2) + (j & 3) - p[c]), paged_score(x[j], a.c, a.cap)) - lse_now[c];
+                } else {
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const int k = j0 + 8 * (j >> 2) + (j & 3);
-                    x[j] = k > p || k < first ? -INFINITY : x[j];
+                    for (int j = 0; j < 16; ++j) x[j] = fmaf(a.c, x[j], -lse_now[c]);
                 }
-            }
+                // (a block that all the wavefront's query rows see whole needs no mask)
+                if (__any(pos[b] + 31 > p[c] || pos[b] < first)) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) sum[b][j] += exp2_fast(x[j]);
-            __builtin_amdgcn_sched_barrier(0);      // (one block's scores at a time: registers)
+                    for (int j = 0; j < 16; ++j) {
+                        const int k = j0 + 8 * (j >> 2) + (j & 3);
+                        x[j] = k > p[c] || k < first ? -INFINITY : x[j];
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 16; ++j) sum[b][j] += exp2_fast(x[j]);
+                if constexpr (NB == 2) __builtin_amdgcn_sched_barrier(0);   // (one block's scores at a time: registers)
+            }
         }
     }
     // ---- over the lanes of a half, then the wavefronts ----------------------------
-    float mine[2] = {0.f, 0.f};                     // lane nl: block b's row nl (both halves of lanes alike)
+    float mine[NB];                                 // lane nl: block b's row nl (both halves of lanes alike)
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+    for (int b = 0; b < NB; ++b) {
+        mine[b] = 0.f;
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
             float y = row16_sum(sum[b][j]);
@@ -179,18 +205,23 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void paged_weights_kernel(Wei
             // (lanes of half hh now hold row 8 (j / 4) + 4 hh + j % 4)
             if (nl == 8 * (j >> 2) + 4 * hh + (j & 3)) mine[b] = y;
         }
-    if (rh == 1) {
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-            if (((nl >> 2) & 1) == hh) part[ph][32 * b + nl] = mine[b];
     }
-    __syncthreads();
+    if constexpr (NB == 2) {
+        if (rh == 1) {
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+                if (((nl >> 2) & 1) == hh) part[pos[b] - kv0 + nl] = mine[b];
+        }
+        __syncthreads();
+    }
     if (writes) {
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+        for (int b = 0; b < NB; ++b) {
+            if constexpr (NB == 2) mine[b] += part[pos[b] - kv0 + nl];
             if (pages[b] >= 0)
                 *(float*)((char*)a.w_out + pages[b] * a.wo_nb3 + hk * a.wo_nb2 + 4 * (int64_t)((pos[b] + nl) & pmask)) =
-                    old[b] + (mine[b] + part[ph][32 * b + nl]);
+                    old[b] + mine[b];
+        }
     }
 }
 
