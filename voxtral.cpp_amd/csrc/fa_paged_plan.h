@@ -222,9 +222,17 @@ inline ChunkBounds chunk_plan(const PagedBatch& b, int head_dim, int nhg, int bm
     p.tiles = (int32_t)r.tiles;
     const int64_t room = r.table < ws_bytes ? (int64_t)((ws_bytes - r.table) / (record * (size_t)nhg)) : 0;
     p.room = (int32_t)(room < 4096 ? room : 4096);
-    // tiles for two rounds of the chip's 256 CUs (16 streams of up to 512 tokens on up
-    // to 4096 rows, 600 workgroups: uncut 169 us, in halves 172), or too few rows: not cut
-    p.cuts = r.tiles * nhg < 512 && b.max_nkv >= 128 && b.n_streams <= kChunkStreams && p.room >= 2;
+    int64_t nb = ((int64_t)b.max_nkv + 31) / 32;          // blocks of the longest walk
+    if (window > 0 && nb > ((int64_t)window + bm) / 32 + 1) nb = ((int64_t)window + bm) / 32 + 1;
+    // Not cut: tiles for two rounds of the chip's 256 CUs (16 streams of up to 512
+    // tokens on up to 4096 rows, 600 workgroups: uncut 169 us, in halves 172), or for
+    // one round and more where the longest walk is short, so that a cut gains less than
+    // its join's launch takes (cut -> uncut, 320 workgroups: 8 streams of 250 tokens,
+    // 20 heads of 64, window 750 37.9 -> 35.2 us, 1500 rows 43.8 -> 41.1; 4 of 634, 32/8
+    // heads of 128, 1500 rows 92.6 -> 89.0; but uneven ones, 4 streams of up to 890 tokens
+    // of 20 heads, 2000 rows 37.3 -> 35.4, 4000 56.5 -> 61.7, 8192 79.9 -> 113.4; 16 of
+    // up to 512, a cap, 2048 rows 136.8 -> 142.1), or too few rows.
+    p.cuts = r.tiles * nhg < (nb > 48 ? 512 : 257) && b.max_nkv >= 128 && b.n_streams <= kChunkStreams && p.room >= 2;
     int64_t items = r.tiles;
     if (p.cuts) items = r.tiles > 512 / nhg ? r.tiles : (512 / nhg > 1 ? 512 / nhg : 1);
     if (p.cuts && items < 2) items = 2;
@@ -232,8 +240,6 @@ inline ChunkBounds chunk_plan(const PagedBatch& b, int head_dim, int nhg, int bm
         // one stream, whose sizes are near the bounds: the pieces are chosen here,
         // and the grid holds no more
         const int tiles = (int)r.tiles;
-        int64_t nb = ((int64_t)b.max_nkv + 31) / 32;
-        if (window > 0 && nb > ((int64_t)window + bm) / 32 + 1) nb = ((int64_t)window + bm) / 32 + 1;
         float best = 3.0e38f;
         p.pieces = 1;
         for (int n = 1; n <= 64; ++n) {
