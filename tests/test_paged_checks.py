@@ -30,7 +30,7 @@ def test_views():
     assert ne == (128, 16, 8, 7) and nb == (2, 2048, 256, 32768)
     ne, nb = views.weight_pages(7, 16, 8)
     assert ne == (16, 8, 7, 1) and nb == (4, 64, 512, 3584)
-    assert views.dst(64, 4, 3) == ((64, 4, 3, 1), (4, 256, 1024, 3072))
+    assert views.dst(64, 4, 5) == ((64, 4, 5, 1), (4, 256, 1024, 5120))
     assert views.dst(64, 4, 3, elt=2) == ((64, 4, 3, 1), (2, 128, 512, 1536))
 
 
