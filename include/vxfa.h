@@ -347,8 +347,9 @@ int vxfa_paged_append(vxfa_ctx* ctx, const vxfa_tensor* k_new,
  *   x += slope_h (j - p), with ggml's slopes for max_bias > 0: n the largest
  *   power of two in Hq, slope_h = 2^(-max_bias (h + 1) / n) for h < n, else
  *   2^(-max_bias (2 (h - n) + 1) / (2 n)); 0 for max_bias = 0.
- * Sums and statistics are F32, the products f16 MFMA; a token that sees no row
- * gets zeros. Rows that a window removes may still be read where a block of
+ * Sums and statistics are F32, the products f16 MFMA; a capped x is off by at
+ * most 2^-22 of a cap of up to 64, by 2^-18 of itself with larger ones (which
+ * take longer, chunks up to 1.5 times). A token that sees no row gets zeros. Rows that a window removes may still be read where a block of
  * 32 rows holds one that a token sees, and have to be finite there.
  *
  * weights (nullable) collects what each row is worth to the tokens:

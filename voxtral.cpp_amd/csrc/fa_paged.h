@@ -93,10 +93,12 @@ struct PagedAttn {
     void* dst;                // [token][head][D], F16 or F32
     uint8_t q_f16, dst_f16;
     int32_t hq, hkv, window;
-    // scores in log2 units: c s; with a cap, cap tanh of it, as
-    // cap - 2 cap / (1 + 2^(c s)) with c = 2 log2(e) scale / softcap
+    // scores in log2 units: c s; with a cap, cap tanh of it: up to kNarrowCap as
+    // cap - 2 cap / (1 + 2^(c s)) with c = 2 log2(e) scale / softcap, beyond by
+    // paged_wide_cap
     float c;                  // scale * log2(e), or the factor above
     float cap;                // softcap * log2(e); 0: none
+    float capk;               // a wide cap's 2 / softcap; 0: a narrow one, or none
     // distance slopes (bias1 != 0): head h of hq, n2 the largest power of two
     // in hq: 2^(bias1 (h + 1)) for h < n2, else 2^(bias1 (h - n2 + 1/2))
     float bias1;              // -max_bias / n2
@@ -116,12 +118,29 @@ __device__ __forceinline__ float paged_slope(const PagedAttn& a, int h) {
     if (a.bias1 == 0.f) return 0.f;
     return kLog2e * exp2f(a.bias1 * (h < a.n2 ? (float)(h + 1) : (float)(h - a.n2) + 0.5f));
 }
-// log2-domain score of a product s, without the distance term. (The cap's
-// subtraction near s = 0 leaves 2^-24 of the cap, an absolute error in an
-// exponent.)
-__device__ __forceinline__ float paged_score(float s, float c, float cap) {
-    if (cap == 0.f) return c * s;
-    return fmaf(-2.f * cap, __builtin_amdgcn_rcpf(1.f + exp2_fast(c * s)), cap);
+// A cap on scores w = c s in log2 units, to the digits of w whatever the cap:
+// cap tanh(w / cap) with u = 2 w / softcap (so that 2^u = e^(2 w / cap)). Below a
+// fifth of the cap (y = w / cap = u ln(2) / 2 < 0.2) by tanh's series,
+// w (1 - y^2/3 + 2 y^4/15 - 17 y^6/315), off by 62/2835 y^8 < 2^-24 of w; from there on
+// by cap (1 - 2 / (1 + 2^u)), whose subtraction leaves 2^-22 of the cap (E, 1 + E,
+// reciprocal and difference rounded), 2^-18.6 of w at most. That second form alone, at
+// all scores, is what narrow caps take (kNarrowCap): 2^-22 of 64 is 1.5e-5 in an
+// exponent, a thirtieth of the step that P is rounded by. (With the wide form for all
+// caps: 16 streams of up to 512 tokens and 4096 rows, cap and slopes, 193 -> 278 us, with
+// weights 354 -> 486; 8192 tokens with a cap 760 -> 1060; single tokens, which wait for
+// HBM, 113.3 -> 113.9.)
+constexpr float kNarrowCap = 64.f;
+__device__ __forceinline__ float paged_wide_cap(float w, float cap, float k) {
+    constexpr float h = 0.34657359028f * 0.34657359028f;   // (ln(2) / 2)^2
+    const float u = k * w, z = u * u;
+    const float p = fmaf(fmaf(-17.f / 315.f * h * h * h, z, 2.f / 15.f * h * h), z, -h / 3.f) * z;
+    const float far = cap * fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + exp2_fast(u)), 1.f);   // (2 cap may be infinite)
+    return fabsf(u) < 0.57707802f ? fmaf(w, p, w) : far;   // (0.4 / ln(2))
+}
+// log2-domain score of a product s, without the distance term (no cap or a narrow one)
+__device__ __forceinline__ float paged_score(const PagedAttn& a, float s) {
+    if (a.cap == 0.f) return a.c * s;
+    return fmaf(-2.f * a.cap, __builtin_amdgcn_rcpf(1.f + exp2_fast(a.c * s)), a.cap);
 }
 
 // four output values at element `at`, 16-byte (F16: 8-byte) aligned

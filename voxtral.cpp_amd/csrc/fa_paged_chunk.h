@@ -19,7 +19,7 @@
 //   past the stream's last granule read a row of zeros.
 //   Scores. MOD 1: with the distance term, two FMAs a score where the plain
 //   softmax has one (slope j + (slope (kv0 - p) - m), then c s + that); MOD 2: with
-//   a cap, too. These walk a tile's blocks from the last: far rows lie lower by
+//   a cap, too, MOD 3 with one above kNarrowCap. These walk a tile's blocks from the last: far rows lie lower by
 //   the distance, so from the first on the running maximum would rise by more than
 //   2^8 in every block of a steep head, and every block's softmax be done twice.
 //   The sum of P is taken in F32 before P is rounded: its logarithm is what the
@@ -31,7 +31,8 @@
 //   workgroups, two on some CUs either way, 41 -> 50).
 // What bounds it, 32/8 heads of 128: 8192 tokens 554-579 us, 0.95-0.99 PFLOP/s (power,
 // as fa_prefill_group.hip; matrix pipe busy 49 % of the cycles); with slopes 565,
-// with a cap 748 (the VALU: exp2 and reciprocal a score more). 600 tokens on 3000
+// with a cap 750-775 (the VALU: exp2 and reciprocal a score more), with a wide one 1060
+// (the series beside them). 600 tokens on 3000
 // rows 53 us, 3 pieces: 38 blocks of ~0.9 us, ~8 before and after, 7 for the join.
 // 16 streams of up to 512 tokens and 4096 rows, half of them single tokens, cap and
 // slopes 208-220 us: 416 workgroups of 8 to 128 blocks, one a CU; VALU 56 % busy.
@@ -78,7 +79,7 @@ __device__ __forceinline__ void pc_wait_vm() {
     __builtin_amdgcn_s_waitcnt(N | (7 << 4) | (15 << 8));
 }
 
-// MOD: 1 the scores have a distance term, 2 a cap (and a slope, or 0). QF16: q is F16.
+// MOD: 1 the scores have a distance term, 2 a cap (and a slope, or 0), 3 a wide one. QF16: q is F16.
 template <int HD, int KVGROUPS, bool QF16, int MOD>
 __global__ __launch_bounds__((PC<HD, KVGROUPS>::NT), 2) void paged_chunk_kernel(ChunkArgs ca) {
     using P = PC<HD, KVGROUPS>;
@@ -348,7 +349,7 @@ __global__ __launch_bounds__((PC<HD, KVGROUPS>::NT), 2) void paged_chunk_kernel(
 
     // ---- softmax ------------------------------------------------------------------
     // P = 2^(x - m), x the score in log2 units: c s; MOD 1: c s + slope (j - p);
-    // MOD 2: cap - 2 cap / (1 + 2^(c s)) + slope (j - p)
+    // MOD 2: cap - 2 cap / (1 + 2^(c s)) + slope (j - p); MOD 3: paged_wide_cap of c s + slope (j - p)
     const float slope = MOD ? __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, paged_slope(a, h)))) : 0.f;
     float m = -INFINITY, l = 0.f;
     // element j of block t, plus `base`
@@ -366,11 +367,12 @@ __global__ __launch_bounds__((PC<HD, KVGROUPS>::NT), 2) void paged_chunk_kernel(
         if constexpr (MOD == 0) return fmaf(s, c, e[0]);
         const float tj = fmaf(slope, (float)j, e[j >> 3]);
         if constexpr (MOD == 1) return fmaf(s, c, tj);
+        if constexpr (MOD == 3) return paged_wide_cap(s * c, a.cap, a.capk) + tj;
         return fmaf(-2.f * a.cap, __builtin_amdgcn_rcpf(1.f + exp2_fast(s * c)), tj);
     };
     // a few scores at a time: with all 16 in flight the registers do not do
     auto few = [](int j) {
-        if (MOD == 2 ? (j & 3) == 3 : MOD == 1 && (j & 7) == 7) __builtin_amdgcn_sched_barrier(0x3FC);   // VALU may not cross
+        if (MOD >= 2 ? (j & 3) == 3 : MOD == 1 && (j & 7) == 7) __builtin_amdgcn_sched_barrier(0x3FC);   // VALU may not cross
     };
     auto exps = [&](const floatx16& sc, half8 (&p)[2], int t) -> float {
         float nm = (m == -INFINITY) ? 0.f : -m;
@@ -388,7 +390,7 @@ __global__ __launch_bounds__((PC<HD, KVGROUPS>::NT), 2) void paged_chunk_kernel(
             }
         };
         // (MOD 0 and 1: a removed score is -inf already)
-        if (MOD == 2 && masked) all(std::true_type{});
+        if (MOD >= 2 && masked) all(std::true_type{});
         else all(std::false_type{});
         return (ls[0] + ls[1]) + (ls[2] + ls[3]);
     };
@@ -398,13 +400,13 @@ __global__ __launch_bounds__((PC<HD, KVGROUPS>::NT), 2) void paged_chunk_kernel(
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
             const float x = score(sc[j], e, j);
-            r = fmaxf(r, MOD == 2 && dead(t, j) ? -INFINITY : x);
+            r = fmaxf(r, MOD >= 2 && dead(t, j) ? -INFINITY : x);
             few(j);
         }
         return pair32_max(r);
     };
     auto mask_fix = [&](floatx16& sc, int t) {
-        if (MOD != 2 && masked) {
+        if (MOD < 2 && masked) {
 #pragma unroll
             for (int j = 0; j < 16; ++j) sc[j] = dead(t, j) ? -INFINITY : sc[j];
         }
@@ -616,7 +618,8 @@ __global__ __launch_bounds__(64 * PC<HD>::DB) void paged_chunk_combine(ChunkArgs
 template <int HD, int KVG, bool QF16>
 static void launch_pc(const ChunkArgs& ca, unsigned nwg, hipStream_t st) {
     const dim3 grid(nwg), block(PC<HD, KVG>::NT);
-    if (ca.a.cap != 0.f) hipLaunchKernelGGL((paged_chunk_kernel<HD, KVG, QF16, 2>), grid, block, 0, st, ca);
+    if (ca.a.capk != 0.f) hipLaunchKernelGGL((paged_chunk_kernel<HD, KVG, QF16, 3>), grid, block, 0, st, ca);
+    else if (ca.a.cap != 0.f) hipLaunchKernelGGL((paged_chunk_kernel<HD, KVG, QF16, 2>), grid, block, 0, st, ca);
     else if (ca.a.bias1 != 0.f) hipLaunchKernelGGL((paged_chunk_kernel<HD, KVG, QF16, 1>), grid, block, 0, st, ca);
     else hipLaunchKernelGGL((paged_chunk_kernel<HD, KVG, QF16, 0>), grid, block, 0, st, ca);
 }

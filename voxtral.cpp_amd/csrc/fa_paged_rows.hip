@@ -206,7 +206,7 @@ __global__ __launch_bounds__(64 * PR_WAVES, 2) void paged_rows_kernel(RowsArgs r
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int j = j0 + i;
-            x[i] = fmaf(slope, (float)(j - p), paged_score(s[i], a.c, a.cap));
+            x[i] = fmaf(slope, (float)(j - p), a.capk != 0.f ? paged_wide_cap(a.c * s[i], a.cap, a.capk) : paged_score(a, s[i]));
             x[i] = j >= first && j <= p ? x[i] : -INFINITY;
             mx = fmaxf(mx, x[i]);
         }

@@ -30,13 +30,14 @@ struct WeightsArgs {
     int32_t ntiles;           // row tiles of a stream at most
 };
 
-// MOD: the scores have a cap or a distance term.
+// MOD: 1 the scores have a cap or a distance term, 2 a wide cap (as a test at run time it
+// cost the narrow one 6 to 15 % of this kernel).
 // NB blocks of 32 rows a wavefront, NB wavefronts share a step's 64 query rows: 2 at
 // hd 128, whose products wait for the query rows from LDS (2000 tokens on as many rows
 // 195 us of a call, with one block 208; 600 on 3000 with slopes 123, 129), 1 at hd 64
 // for the registers, four workgroups a CU in place of three (the window case's call 58
 // against 67, 16 streams of 100 tokens and up to 8000 rows 297 against 395).
-template <int D, bool QF16, bool MOD>
+template <int D, bool QF16, int MOD>
 __global__ __launch_bounds__(256, (D == 128 ? 2 : QF16 ? 4 : 3)) void paged_weights_kernel(WeightsArgs wa) {
     constexpr int KS = D / 16, ROW = 2 * D, CH = D / 8;
     constexpr int STEP = 64 * ROW;                  // bytes of 64 query rows
@@ -169,10 +170,12 @@ __global__ __launch_bounds__(256, (D == 128 ? 2 : QF16 ? 4 : 3)) void paged_weig
                 for (int ks = 0; ks < KS; ++ks) x = __builtin_amdgcn_mfma_f32_32x32x16_f16(kr[b][ks], qb[ks], x, 0, 0, 0);
                 // element j: row pos + 8 (j / 4) + 4 hh + j % 4
                 const int j0 = pos[b] + 4 * hh;
-                if constexpr (MOD) {
+                if constexpr (MOD != 0) {
 #pragma unroll
-                    for (int j = 0; j < 16; ++j)
-                        x[j] = fmaf(slope[c], (float)(j0 + 8 * (j >> 2) + (j & 3) - p[c]), paged_score(x[j], a.c, a.cap)) - lse_now[c];
+                    for (int j = 0; j < 16; ++j) {
+                        const float y = MOD == 2 ? paged_wide_cap(a.c * x[j], a.cap, a.capk) : paged_score(a, x[j]);
+                        x[j] = fmaf(slope[c], (float)(j0 + 8 * (j >> 2) + (j & 3) - p[c]), y) - lse_now[c];
+                    }
                 } else {
 #pragma unroll
                     for (int j = 0; j < 16; ++j) x[j] = fmaf(a.c, x[j], -lse_now[c]);
@@ -225,16 +228,16 @@ __global__ __launch_bounds__(256, (D == 128 ? 2 : QF16 ? 4 : 3)) void paged_weig
     }
 }
 
+template <int D, bool QF16>
+static void launch_pw_q(const WeightsArgs& wa, const dim3& grid, hipStream_t st) {
+    if (wa.a.capk != 0.f) hipLaunchKernelGGL((paged_weights_kernel<D, QF16, 2>), grid, dim3(256), 0, st, wa);
+    else if (wa.a.cap != 0.f || wa.a.bias1 != 0.f) hipLaunchKernelGGL((paged_weights_kernel<D, QF16, 1>), grid, dim3(256), 0, st, wa);
+    else hipLaunchKernelGGL((paged_weights_kernel<D, QF16, 0>), grid, dim3(256), 0, st, wa);
+}
 template <int D>
 static void launch_pw(const WeightsArgs& wa, const dim3& grid, hipStream_t st) {
-    const bool mod = wa.a.cap != 0.f || wa.a.bias1 != 0.f;
-    if (wa.a.q_f16) {
-        if (mod) hipLaunchKernelGGL((paged_weights_kernel<D, true, true>), grid, dim3(256), 0, st, wa);
-        else hipLaunchKernelGGL((paged_weights_kernel<D, true, false>), grid, dim3(256), 0, st, wa);
-    } else {
-        if (mod) hipLaunchKernelGGL((paged_weights_kernel<D, false, true>), grid, dim3(256), 0, st, wa);
-        else hipLaunchKernelGGL((paged_weights_kernel<D, false, false>), grid, dim3(256), 0, st, wa);
-    }
+    if (wa.a.q_f16) launch_pw_q<D, true>(wa, grid, st);
+    else launch_pw_q<D, false>(wa, grid, st);
 }
 
 hipError_t launch_paged_weights(const PagedAttn& a, int head_dim, hipStream_t st) {

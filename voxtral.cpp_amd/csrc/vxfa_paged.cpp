@@ -240,7 +240,8 @@ int vxfa_flash_attn_ext_paged(vxfa_ctx* c, const vxfa_tensor* q, const vxfa_tens
         return fail(c, VXFA_UNSUPPORTED, "q rows must be contiguous and 16-byte aligned");
     if (!isfinite(scale) || !isfinite(max_bias) || !isfinite(logit_softcap) || max_bias < 0 || logit_softcap < 0)
         return fail(c, VXFA_UNSUPPORTED, "scale, max_bias and logit_softcap must be finite, the latter two not negative");
-    const float c_score = logit_softcap > 0 ? 2.0f * vxfa::kLog2e * (scale / logit_softcap) : scale * vxfa::kLog2e;
+    const bool wide_cap = logit_softcap > vxfa::kNarrowCap;
+    const float c_score = logit_softcap > 0 && !wide_cap ? 2.0f * vxfa::kLog2e * (scale / logit_softcap) : scale * vxfa::kLog2e;
     if (!isfinite(c_score) || !isfinite(logit_softcap * vxfa::kLog2e))
         return fail(c, VXFA_UNSUPPORTED, "scale and logit_softcap: their ratio is out of range");
     if (T > kMaxTokens || Hq > 65535) return fail(c, VXFA_UNSUPPORTED, "sizes beyond the launch limits");
@@ -263,6 +264,7 @@ int vxfa_flash_attn_ext_paged(vxfa_ctx* c, const vxfa_tensor* q, const vxfa_tens
     a.window = batch->window < a.b.max_nkv ? batch->window : 0;   // (a window of all rows is none)
     a.c = c_score;
     if (logit_softcap > 0) a.cap = logit_softcap * vxfa::kLog2e;
+    if (wide_cap) a.capk = 2.0f / logit_softcap;
     if (max_bias > 0 && Hq > 0) {
         int64_t n2 = 1;
         while (2 * n2 <= Hq) n2 *= 2;
