@@ -135,3 +135,11 @@ def test_the_bounds_hold_a_planted_error():
     x2 = 0.125 * c.q[:4, 1].astype(np.float64) @ k.T
     e2 = np.where(live, np.exp(x2), 0)
     assert (np.abs(one + (e2 / e2.sum(1, keepdims=True)).sum(0) - add[0, 0]) > adderr[0, 0]).any()
+
+
+@pytest.mark.parametrize("bias", [1e-45, 1e-38, 1e-3])
+@pytest.mark.parametrize("hq,hkv,hd", [(8, 2, 128), (6, 2, 64)])
+@pytest.mark.parametrize("t", [1, 50])
+def test_smallest_exponents_of_the_slopes(ctx, bias, hq, hkv, hd, t):
+    """Slopes near 1 for all heads (max_bias over the number of heads may be 0 in F32: no less a slope)."""
+    check(ctx, without_weights(Batch([(t, t), (97, t), (300, t)], hq, hkv, hd, seed=t + 1)), bias=bias)

@@ -99,9 +99,9 @@ struct PagedAttn {
     float c;                  // scale * log2(e), or the factor above
     float cap;                // softcap * log2(e); 0: none
     float capk;               // a wide cap's 2 / softcap; 0: a narrow one, or none
-    // distance slopes (bias1 != 0): head h of hq, n2 the largest power of two
+    // distance slopes (n2 != 0): head h of hq, n2 the largest power of two
     // in hq: 2^(bias1 (h + 1)) for h < n2, else 2^(bias1 (h - n2 + 1/2))
-    float bias1;              // -max_bias / n2
+    float bias1;              // -max_bias / n2 (which may be 0: slopes of 1)
     int32_t n2;
     // accumulated weights
     const float* w_in;        // null: zeros
@@ -115,7 +115,7 @@ struct PagedAttn {
 
 // slope_h * log2(e)
 __device__ __forceinline__ float paged_slope(const PagedAttn& a, int h) {
-    if (a.bias1 == 0.f) return 0.f;
+    if (a.n2 == 0) return 0.f;
     return kLog2e * exp2f(a.bias1 * (h < a.n2 ? (float)(h + 1) : (float)(h - a.n2) + 0.5f));
 }
 // A cap on scores w = c s in log2 units, to the digits of w whatever the cap:

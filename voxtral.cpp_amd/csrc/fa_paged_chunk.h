@@ -620,7 +620,7 @@ static void launch_pc(const ChunkArgs& ca, unsigned nwg, hipStream_t st) {
     const dim3 grid(nwg), block(PC<HD, KVG>::NT);
     if (ca.a.capk != 0.f) hipLaunchKernelGGL((paged_chunk_kernel<HD, KVG, QF16, 3>), grid, block, 0, st, ca);
     else if (ca.a.cap != 0.f) hipLaunchKernelGGL((paged_chunk_kernel<HD, KVG, QF16, 2>), grid, block, 0, st, ca);
-    else if (ca.a.bias1 != 0.f) hipLaunchKernelGGL((paged_chunk_kernel<HD, KVG, QF16, 1>), grid, block, 0, st, ca);
+    else if (ca.a.n2 != 0) hipLaunchKernelGGL((paged_chunk_kernel<HD, KVG, QF16, 1>), grid, block, 0, st, ca);
     else hipLaunchKernelGGL((paged_chunk_kernel<HD, KVG, QF16, 0>), grid, block, 0, st, ca);
 }
 

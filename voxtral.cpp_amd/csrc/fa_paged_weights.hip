@@ -231,7 +231,7 @@ __global__ __launch_bounds__(256, (D == 128 ? 2 : QF16 ? 4 : 3)) void paged_weig
 template <int D, bool QF16>
 static void launch_pw_q(const WeightsArgs& wa, const dim3& grid, hipStream_t st) {
     if (wa.a.capk != 0.f) hipLaunchKernelGGL((paged_weights_kernel<D, QF16, 2>), grid, dim3(256), 0, st, wa);
-    else if (wa.a.cap != 0.f || wa.a.bias1 != 0.f) hipLaunchKernelGGL((paged_weights_kernel<D, QF16, 1>), grid, dim3(256), 0, st, wa);
+    else if (wa.a.cap != 0.f || wa.a.n2 != 0) hipLaunchKernelGGL((paged_weights_kernel<D, QF16, 1>), grid, dim3(256), 0, st, wa);
     else hipLaunchKernelGGL((paged_weights_kernel<D, QF16, 0>), grid, dim3(256), 0, st, wa);
 }
 template <int D>
