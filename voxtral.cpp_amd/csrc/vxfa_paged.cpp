@@ -33,6 +33,14 @@ bool sane(const vxfa_tensor* t) {
     return true;
 }
 
+// elements that a call over streams would touch, but no data
+bool missing(const vxfa_paged* b, const vxfa_tensor* t) {
+    if (t->data || b->n_streams == 0) return false;
+    for (int d = 0; d < 4; ++d)
+        if (t->ne[d] == 0) return false;
+    return true;
+}
+
 // 16-byte loads of rows of `elt`-sized elements
 bool vector_rows(const vxfa_tensor* t, size_t elt, int dims) {
     if (t->nb[0] != elt || !aligned(t->data, 16)) return false;
@@ -59,6 +67,7 @@ int check_pool(const vxfa_tensor* k, const vxfa_tensor* v, const vxfa_paged* b, 
         *why = "batch: misaligned arrays";
         return VXFA_INVALID_ARG;
     }
+    if (missing(b, k) || missing(b, v)) { *why = "k and v: data is required"; return VXFA_INVALID_ARG; }
     const int64_t ps = k->ne[1];
     if (ps < (1 << vxfa::kPagedMinLog2) || ps > (1 << vxfa::kPagedMaxLog2) || (ps & (ps - 1))) {
         *why = "page size must be a power of two from 16 to 65536";
@@ -168,6 +177,7 @@ int vxfa_paged_append(vxfa_ctx* c, const vxfa_tensor* k_new, const vxfa_tensor* 
     if (!sane(k_new) || !sane(v_new)) return fail(c, VXFA_INVALID_ARG, "new rows: unknown type, negative ne or absurd nb");
     if ((rc = check_new(k_new, k, &why)) != VXFA_OK || (rc = check_new(v_new, v, &why)) != VXFA_OK)
         return fail(c, rc, "%s", why);
+    if (missing(batch, k_new) || missing(batch, v_new)) return fail(c, VXFA_INVALID_ARG, "new rows: data is required");
     const int64_t T = k_new->ne[1], D = k->ne[0];
     if (v_new->ne[1] != T) return fail(c, VXFA_INVALID_ARG, "k_new and v_new row counts differ");
     if ((q == nullptr) != (q_out == nullptr) || (q && !rope))
@@ -182,6 +192,7 @@ int vxfa_paged_append(vxfa_ctx* c, const vxfa_tensor* k_new, const vxfa_tensor* 
         if (!sane(q) || !sane(q_out)) return fail(c, VXFA_INVALID_ARG, "q and q_out: unknown type, negative ne or absurd nb");
         for (int d = 0; d < 4; ++d)
             if (q->ne[d] != q_out->ne[d]) return fail(c, VXFA_INVALID_ARG, "q and q_out shapes differ");
+        if (missing(batch, q) || missing(batch, q_out)) return fail(c, VXFA_INVALID_ARG, "q and q_out: data is required");
         if (q->ne[0] != D || q->ne[1] != T || q->ne[3] != 1 || q->ne[2] > 65535)
             return fail(c, VXFA_INVALID_ARG, "q must be [D, T, Hq, 1]");
         if (q->type != VXFA_TYPE_F32 || q_out->type != VXFA_TYPE_F16)
@@ -229,6 +240,7 @@ int vxfa_flash_attn_ext_paged(vxfa_ctx* c, const vxfa_tensor* q, const vxfa_tens
     if (rc != VXFA_OK) return fail(c, rc, "%s", why);
     if (!q || !dst) return fail(c, VXFA_INVALID_ARG, "q and dst are required");
     if (!sane(q) || !sane(dst)) return fail(c, VXFA_INVALID_ARG, "q and dst: unknown type, negative ne or absurd nb");
+    if (missing(batch, q) || missing(batch, dst)) return fail(c, VXFA_INVALID_ARG, "q and dst: data is required");
     const int64_t D = k->ne[0], T = q->ne[1], Hq = q->ne[2], Hkv = k->ne[2];
     if (q->ne[0] != D || q->ne[3] != 1 || Hq % Hkv) return fail(c, VXFA_INVALID_ARG, "q must be [D, T, Hq, 1], Hq a multiple of Hkv");
     if (dst->ne[0] != D || dst->ne[1] != Hq || dst->ne[2] != T || dst->ne[3] != 1)
@@ -248,6 +260,8 @@ int vxfa_flash_attn_ext_paged(vxfa_ctx* c, const vxfa_tensor* q, const vxfa_tens
     if (weights_in && !weights) return fail(c, VXFA_INVALID_ARG, "weights_in without weights");
     if (weights && (rc = check_weights(weights, k, &why)) != VXFA_OK) return fail(c, rc, "%s", why);
     if (weights_in && (rc = check_weights(weights_in, k, &why)) != VXFA_OK) return fail(c, rc, "%s", why);
+    if ((weights && missing(batch, weights)) || (weights_in && missing(batch, weights_in)))
+        return fail(c, VXFA_INVALID_ARG, "weights: data is required");
 
     vxfa::PagedAttn a;
     memset(&a, 0, sizeof(a));
@@ -313,6 +327,7 @@ int vxfa_paged_evict(vxfa_ctx* c, vxfa_tensor* k, vxfa_tensor* v, vxfa_tensor* w
     if (rc != VXFA_OK) return fail(c, rc, "%s", why);
     if (!weights || !ev) return fail(c, VXFA_INVALID_ARG, "weights and evict are required");
     if ((rc = check_weights(weights, k, &why)) != VXFA_OK) return fail(c, rc, "%s", why);
+    if (missing(batch, weights)) return fail(c, VXFA_INVALID_ARG, "weights: data is required");
     if (ev->budget <= 0 || ev->n_sink < 0 || ev->n_recent < 0 || (int64_t)ev->n_sink + ev->n_recent > ev->budget)
         return fail(c, VXFA_INVALID_ARG, "evict: budget > 0, n_sink >= 0, n_recent >= 0 and their sum within the budget");
     if (ev->max_pages < 0 || (ev->max_pages > 0 && !ev->pages) || !aligned(ev->pages, 4) || !aligned(ev->kept, 4) || !aligned(ev->n_kv, 4))
