@@ -1,7 +1,7 @@
 // Host check of the paged entry points as libvxfa.so has them, launchers and all,
 // without a GPU: the HIP calls are stand-ins of this program, which the library's
-// references bind to, and count the launches. Descriptors without data are refused
-// before any launch. Built and run by tests/test_paged_limits.py.
+// references bind to, and count the launches. Descriptors without data and grids beyond
+// the launch limits are refused before any launch. Built and run by tests/test_paged_limits.py.
 #include <hip/hip_runtime.h>
 
 #include <cstdio>
@@ -104,9 +104,25 @@ static void data() {
     gives(__LINE__, VXFA_OK, false, evict, CHANGED(c.k.data = c.v.data = c.w.data = nullptr; c.b.n_streams = 0));
 }
 
+// workgroups of an attention call: parts of streams (or tiles) by head groups, 2^23 - 1 at most
+static void grids() {
+    for (int64_t D : {64, 128}) {
+        // single tokens of 65535 streams, 128 and 129 kv heads: 8388480 and 8454015
+        GIVES(VXFA_OK, attend_only, Call(65535, 128, 128, 65535, 1, D));
+        GIVES(VXFA_UNSUPPORTED, attend_only, Call(65535, 129, 129, 65535, 1, D));
+        GIVES(VXFA_UNSUPPORTED, attend_only, Call(65535, 65535, 65535, 65535, 1, D));
+        // chunks: tiles of 256 (128) tokens, a head each
+        const int64_t bm = 2 * D;
+        GIVES(VXFA_OK, attend_only, Call(65535 * bm / 2, 255, 255, 1, 1 << 24, D));
+        GIVES(VXFA_UNSUPPORTED, attend_only, Call(65535 * bm / 2, 257, 257, 1, 1 << 24, D));
+        GIVES(VXFA_UNSUPPORTED, attend_only, Call(1 << 23, 60000, 60000, 1, 1 << 24, D));
+    }
+}
+
 int main() {
     g_ctx.ws = reinterpret_cast<char*>(0x7d0000000000ull);
     data();
+    grids();
     std::printf(g_bad ? "%d wrong\n" : "ok\n", g_bad);
     return g_bad != 0;
 }

@@ -190,8 +190,8 @@ hipError_t launch_paged_append(const PagedAppend& a, hipStream_t st);
 bool paged_rows_takes(const PagedAttn& a);
 // weighed: the accumulated weights are done, too (else launch_paged_weights)
 hipError_t launch_paged_rows(const PagedAttn& a, int head_dim, hipStream_t st, bool& weighed);
-// any chunks (hipErrorOutOfMemory, as from launch_paged_rows: the workspace does not
-// hold the work's tables)
+// any chunks (as from launch_paged_rows, before any launch: hipErrorOutOfMemory where the
+// workspace does not hold the work's tables, hipErrorNotSupported beyond the grid's limit)
 hipError_t launch_paged_chunk(const PagedAttn& a, int head_dim, hipStream_t st);
 hipError_t launch_paged_chunk64(const PagedAttn& a, hipStream_t st);
 // what the launches below take: workgroups along x

@@ -640,7 +640,7 @@ static hipError_t launch_chunk(const PagedAttn& a, hipStream_t st) {
     ca.tiles = reinterpret_cast<ChunkTile*>(a.ws);
     ca.rec = reinterpret_cast<float*>(a.ws + cb.table);
     const int64_t nwg = (int64_t)ca.p.items * ca.nhg;
-    if (nwg > 0xffffffffll / 512) return hipErrorInvalidValue;
+    if (nwg > 0xffffffffll / 512) return hipErrorNotSupported;
     if constexpr (HD == 64) {
         if (ca.p.kvg == 2) {
             if (a.q_f16) launch_pc<HD, 2, true>(ca, (unsigned)nwg, st);

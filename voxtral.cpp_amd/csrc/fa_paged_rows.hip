@@ -452,7 +452,7 @@ hipError_t launch_paged_rows(const PagedAttn& a, int head_dim, hipStream_t st, b
     ra.whole = ra.x && !ra.p.cuts && ra.groups == 1;
     ra.p.empty = ra.whole;
     const int64_t nwg = (int64_t)ra.items * nhg;
-    if (nwg > 0x7fffffff / 256) return hipErrorInvalidValue;
+    if (nwg > 0x7fffffff / 256) return hipErrorNotSupported;
     const dim3 grid((unsigned)nwg), block(64 * PR_WAVES);
     if (head_dim == 128) hipLaunchKernelGGL((paged_rows_kernel<128>), grid, block, 0, st, ra);
     else hipLaunchKernelGGL((paged_rows_kernel<64>), grid, block, 0, st, ra);
