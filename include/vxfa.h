@@ -357,11 +357,16 @@ int vxfa_paged_append(vxfa_ctx* ctx, const vxfa_tensor* k_new,
  * element (row, kv head, page) of every row of a stream becomes that of
  * weights_in plus the sum, over the tokens and the head's query heads, of the
  * softmax's weights. weights_in may be weights itself, another tensor of that
- * shape, or NULL (zeros). Streams that share a page leave one stream's sum
- * there. Rows of no stream are left as they were. Needs 4 * Hq * T bytes of
+ * shape, or NULL (zeros). Of a page that the call's tables name more than once
+ * (streams with a common prefix) the elements are left open: weights_in's plus
+ * the sum of one of its streams or of some of them, and not the same ones from
+ * call to call. Streams that share pages therefore take their weights in calls
+ * of their own, one after another, in place (weights_in = weights): their sums
+ * then add up in that order. Rows of no stream are left as they were. Needs 4 * Hq * T bytes of
  * the workspace (else VXFA_NO_WORKSPACE).
  *
- * The output is deterministic; asynchronous on `stream`. */
+ * dst is deterministic, and so are the weights of pages that are named once;
+ * asynchronous on `stream`. */
 int vxfa_flash_attn_ext_paged(vxfa_ctx* ctx, const vxfa_tensor* q,
                               const vxfa_tensor* k, const vxfa_tensor* v,
                               const vxfa_paged* batch, vxfa_tensor* dst,

@@ -328,7 +328,8 @@ class Context:
                              logit_softcap: float = 0.0, weights_in=None, weights=None, stream: int = 0,
                              check: bool = True) -> int:
         """The new tokens of all streams over their paged rows (batch: VxfaPaged), causal within each stream;
-        weights: accumulated attention weight of each row and kv head, on top of weights_in."""
+        weights: accumulated attention weight of each row and kv head, on top of weights_in. (Rows of a page that
+        two streams of the call share get the sum of one or both: calls of their own, in place, add up.)"""
         rc = self._lib.vxfa_flash_attn_ext_paged(self._h, q, k, v, batch, dst, scale, max_bias, logit_softcap,
                                                  weights_in, weights, stream)
         if check and rc != OK:
