@@ -296,9 +296,12 @@ int vxfa_flash_attn_ext_noalloc(const vxfa_tensor* q, const vxfa_tensor* k,
  *
  * The pool is two descriptors, k and v [D, page_size, Hkv, n_pages] F16 (rows
  * contiguous; any 16-byte multiples as nb[1..3], so [page][row][head] and
- * [page][head][row] both do), page_size a power of two from 16 to 65536. Row r
- * of stream s lies in row r % page_size of the page that entry
- * r / page_size of line s of the table names. An entry outside [0, n_pages)
+ * [page][head][row] both do, but the same ones for k and v, and nb[1] below
+ * 8 MiB), page_size a power of two from 16 to 65536. Pools of other strides, more
+ * than 65535 streams, heads or kv heads or 2^24 - 1 tokens, and sizes beyond a
+ * launch's grid give VXFA_UNSUPPORTED. Row r of stream s lies in row
+ * r % page_size of the page that entry r / page_size of line s of the table
+ * names. An entry outside [0, n_pages)
  * (-1, say) is an absent page: nothing is read there, its rows take no part,
  * and rows appended there are dropped. So pages that a window has left behind
  * can be freed at once.
@@ -311,8 +314,9 @@ int vxfa_flash_attn_ext_noalloc(const vxfa_tensor* q, const vxfa_tensor* k,
  * replay; the host gives bounds. Values out of range do no harm: n_kv is
  * taken as at most max_nkv (2^30 at most), q_start as within the call's tokens
  * and not decreasing, a row p below 0 takes no part, and tokens past max_nq of
- * a stream are left out; where chunks overlap, outputs may stay unwritten. Rows of q and dst behind the last stream's are neither
- * read nor written. */
+ * a stream are left out; where chunks overlap, outputs and weights may be
+ * anything. Rows of q and dst behind the last stream's are neither read nor
+ * written. */
 typedef struct vxfa_paged {
     const int32_t* pages;    /* device [n_streams][max_pages]                        */
     const int32_t* n_kv;     /* device [n_streams]: rows in use, the new ones included */
@@ -349,8 +353,10 @@ int vxfa_paged_append(vxfa_ctx* ctx, const vxfa_tensor* k_new,
  *   2^(-max_bias (2 (h - n) + 1) / (2 n)); 0 for max_bias = 0.
  * Sums and statistics are F32, the products f16 MFMA; a capped x is off by at
  * most 2^-22 of a cap of up to 64, by 2^-18 of itself with larger ones (which
- * take longer, chunks up to 1.5 times). A token that sees no row gets zeros. Rows that a window removes may still be read where a block of
- * 32 rows holds one that a token sees, and have to be finite there.
+ * take longer, chunks up to 1.5 times). A token that sees no row gets zeros.
+ * Rows that a token does not see (those of later tokens, those that a window
+ * removes) may still be read where a block of 32 rows holds one that it or
+ * another token of its chunk sees, and have to be finite there.
  *
  * weights (nullable) collects what each row is worth to the tokens:
  * F32 [page_size, Hkv, n_pages, 1], elements contiguous along ne[0];
@@ -362,8 +368,9 @@ int vxfa_paged_append(vxfa_ctx* ctx, const vxfa_tensor* k_new,
  * the sum of one of its streams or of some of them, and not the same ones from
  * call to call. Streams that share pages therefore take their weights in calls
  * of their own, one after another, in place (weights_in = weights): their sums
- * then add up in that order. Rows of no stream are left as they were. Needs 4 * Hq * T bytes of
- * the workspace (else VXFA_NO_WORKSPACE).
+ * then add up in that order. Rows of no stream are left as they were. Needs
+ * 4 * Hq * T bytes of the workspace beside the call's tables, 8 bytes a stream
+ * or 16 a tile of at least 32 tokens (else VXFA_NO_WORKSPACE).
  *
  * dst is deterministic, and so are the weights of pages that are named once;
  * asynchronous on `stream`. */
@@ -381,7 +388,7 @@ int vxfa_flash_attn_ext_paged(vxfa_ctx* ctx, const vxfa_tensor* q,
 typedef struct vxfa_evict {
     const int32_t* pages;   /* device [n_streams][max_pages]: where the kept rows go */
     int32_t max_pages;
-    int32_t budget;         /* rows kept of a stream, > 0                            */
+    int32_t budget;         /* rows kept of a stream, 1 .. 2^30                       */
     int32_t n_sink;         /* >= 0; n_sink + n_recent <= budget                     */
     int32_t n_recent;
     int32_t* kept;          /* device [n_streams][Hkv][budget]: row numbers kept,
@@ -394,12 +401,13 @@ typedef struct vxfa_evict {
  * of k, v and weights move, in their order, to rows 0, 1, .. of the pages that
  * evict->pages names, each at most once, pages of the same pool that no stream
  * of the call lies in (streams may share pages, which an eviction in place
- * would spoil for the others). The old pages are left as they were. batch->q_start, max_nq and
- * window are not looked at. Rows that lie in absent pages count as rows of
+ * would spoil for the others). The old pages are left as they were.
+ * batch->q_start is not read; max_nq and window, which may not be negative here
+ * either, have no effect. Rows that lie in absent pages count as rows of
  * weight NaN and of zeros. Afterwards row numbers are no longer token
  * positions: the distances and windows of further calls go by rows. Needs
- * 4 * Hkv * n_streams * min(budget, max_nkv) bytes of the workspace where kept is NULL (else
- * VXFA_NO_WORKSPACE). Asynchronous on `stream`. */
+ * 4 * Hkv * n_streams * min(budget, max_nkv) bytes of the workspace where kept
+ * is NULL (else VXFA_NO_WORKSPACE). Asynchronous on `stream`. */
 int vxfa_paged_evict(vxfa_ctx* ctx, vxfa_tensor* k, vxfa_tensor* v,
                      vxfa_tensor* weights, const vxfa_paged* batch,
                      const vxfa_evict* evict, void* stream);

@@ -1,7 +1,7 @@
 // Host check of the paged entry points as libvxfa.so has them, launchers and all,
 // without a GPU: the HIP calls are stand-ins of this program, which the library's
-// references bind to, and count the launches. Descriptors without data and grids beyond
-// the launch limits are refused before any launch. Built and run by tests/test_paged_limits.py.
+// references bind to, and count the launches. Descriptors without data, grids beyond
+// the launch limits and sizes beyond the documented ones are refused before any launch. Built and run by tests/test_paged_limits.py.
 #include <hip/hip_runtime.h>
 
 #include <cstdio>
@@ -119,10 +119,28 @@ static void grids() {
     }
 }
 
+// the sizes that the header names
+static void sizes() {
+    GIVES(VXFA_OK, append, Call(7, 65535));
+    GIVES(VXFA_UNSUPPORTED, append, Call(7, 65536));
+    GIVES(VXFA_UNSUPPORTED, attend_only, Call(7, 65536));
+    GIVES(VXFA_UNSUPPORTED, append, Call(1 << 24));
+    GIVES(VXFA_UNSUPPORTED, attend_only, Call(1 << 24));
+    for (auto run : {attend, append, evict}) {
+        GIVES(VXFA_UNSUPPORTED, run, Call(7, 65536, 65536));
+        GIVES(VXFA_UNSUPPORTED, run, Call(7, 8, 2, 65536));
+        // K and V pools share their strides, rows less than 8 MiB apart
+        GIVES(VXFA_UNSUPPORTED, run, CHANGED(c.v.nb[3] *= 2));
+        GIVES(VXFA_OK, run, CHANGED(c.k.nb[1] = c.v.nb[1] = (1 << 23) - 16));
+        GIVES(VXFA_UNSUPPORTED, run, CHANGED(c.k.nb[1] = c.v.nb[1] = 1 << 23));
+    }
+}
+
 int main() {
     g_ctx.ws = reinterpret_cast<char*>(0x7d0000000000ull);
     data();
     grids();
+    sizes();
     std::printf(g_bad ? "%d wrong\n" : "ok\n", g_bad);
     return g_bad != 0;
 }

@@ -193,14 +193,14 @@ int vxfa_paged_append(vxfa_ctx* c, const vxfa_tensor* k_new, const vxfa_tensor* 
         for (int d = 0; d < 4; ++d)
             if (q->ne[d] != q_out->ne[d]) return fail(c, VXFA_INVALID_ARG, "q and q_out shapes differ");
         if (missing(batch, q) || missing(batch, q_out)) return fail(c, VXFA_INVALID_ARG, "q and q_out: data is required");
-        if (q->ne[0] != D || q->ne[1] != T || q->ne[3] != 1 || q->ne[2] > 65535)
+        if (q->ne[0] != D || q->ne[1] != T || q->ne[3] != 1)
             return fail(c, VXFA_INVALID_ARG, "q must be [D, T, Hq, 1]");
         if (q->type != VXFA_TYPE_F32 || q_out->type != VXFA_TYPE_F16)
             return fail(c, VXFA_UNSUPPORTED, "q must be F32, q_out F16");
         if (!vector_rows(q, 4, 3) || !vector_rows(q_out, 2, 3))
             return fail(c, VXFA_UNSUPPORTED, "q and q_out rows must be contiguous and 16-byte aligned");
     }
-    if (T > kMaxTokens) return fail(c, VXFA_UNSUPPORTED, "sizes beyond the launch limits");
+    if (T > kMaxTokens || (q && q->ne[2] > 65535)) return fail(c, VXFA_UNSUPPORTED, "sizes beyond the launch limits");
     vxfa::PagedAppend a;
     memset(&a, 0, sizeof(a));
     a.b = batch_of(batch, k, T);
