@@ -28,7 +28,7 @@
 //   piece's blocks and a ring of its own, joined through LDS: alone on its CU a
 //   workgroup has one wavefront a SIMD, and the chain of a block's dependent steps
 //   takes 0.6 us (600 tokens on 3000 rows, 20 heads: 41.3 -> 35.5 us; with 320
-//   workgroups, two on some CUs either way, 41 -> 50).
+//   workgroups, of which the LDS of a CU holds one at 136 KiB each, 41 -> 50).
 // What bounds it, 32/8 heads of 128: 8192 tokens 554-579 us, 0.95-0.99 PFLOP/s (power,
 // as fa_prefill_group.hip; matrix pipe busy 49 % of the cycles); with slopes 565,
 // with a cap 750-775 (the VALU: exp2 and reciprocal a score more), with a wide one 1060
@@ -36,6 +36,8 @@
 // rows 53 us, 3 pieces: 38 blocks of ~0.9 us, ~8 before and after, 7 for the join.
 // 16 streams of up to 512 tokens and 4096 rows, half of them single tokens, cap and
 // slopes 208-220 us: 416 workgroups of 8 to 128 blocks, one a CU; VALU 56 % busy.
+// With a cap the hd 128 kernel takes all 256 VGPRs and spills 6 (a wide one 7): 28 (32)
+// bytes of scratch a lane.
 #pragma once
 
 #include "fa_paged.h"

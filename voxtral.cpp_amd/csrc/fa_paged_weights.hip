@@ -17,7 +17,11 @@
 // Bound by its VALU work (three instructions a score, and the masks of the blocks
 // on the diagonal and at a window's edge) and each workgroup's chain of loads: 8
 // streams of 250 tokens, window 750, 20 heads of 64, 22 us (a thread per row and
-// head, which this replaced, 331).
+// head, which this replaced, 331). Query rows are not split over workgroups: one stream's
+// 2000 tokens on as many rows are 128 workgroups, the first of which walks all 8000 query
+// rows, 125 steps, and the call takes 196 us (without weights 67).
+// Spills: F32 queries at hd 128 14 or 15 VGPRs (60 or 64 bytes of scratch a lane), F16
+// ones at hd 64 with a cap or slopes 3 (16 bytes).
 #include "fa_paged.h"
 
 namespace vxfa {
