@@ -298,7 +298,7 @@ int vxfa_flash_attn_ext_noalloc(const vxfa_tensor* q, const vxfa_tensor* k,
  * contiguous; any 16-byte multiples as nb[1..3], so [page][row][head] and
  * [page][head][row] both do, but the same ones for k and v, and nb[1] below
  * 8 MiB), page_size a power of two from 16 to 65536. Pools of other strides, more
- * than 65535 streams, heads or kv heads or 2^24 - 1 tokens, and sizes beyond a
+ * than 65535 streams, query or kv heads, or 2^24 - 1 tokens, and sizes beyond a
  * launch's grid give VXFA_UNSUPPORTED. Row r of stream s lies in row
  * r % page_size of the page that entry r / page_size of line s of the table
  * names. An entry outside [0, n_pages)

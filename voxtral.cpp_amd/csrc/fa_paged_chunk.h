@@ -19,9 +19,10 @@
 //   past the stream's last granule read a row of zeros.
 //   Scores. MOD 1: with the distance term, two FMAs a score where the plain
 //   softmax has one (slope j + (slope (kv0 - p) - m), then c s + that); MOD 2: with
-//   a cap, too, MOD 3 with one above kNarrowCap. These walk a tile's blocks from the last: far rows lie lower by
-//   the distance, so from the first on the running maximum would rise by more than
-//   2^8 in every block of a steep head, and every block's softmax be done twice.
+//   a cap, too, MOD 3 with one above kNarrowCap. These walk a tile's blocks from the
+//   last: far rows lie lower by the distance, so from the first on the running maximum
+//   would rise by more than 2^8 in every block of a steep head, and every block's
+//   softmax be done twice.
 //   The sum of P is taken in F32 before P is rounded: its logarithm is what the
 //   accumulated weights are divided by.
 //   hd 64, up to 256 workgroups: two groups of 4 wavefronts, each with half of the

@@ -186,9 +186,9 @@ constexpr int kChunkStreams = 64;   // more streams are not cut
 // A cut's time in blocks of 32 rows: `total` blocks of a head group, in `items`
 // workgroups (of each head group) of `lp` at most. A workgroup costs its blocks
 // (shared among kvg groups of wavefronts) and kWg, 256 run at once; a record costs
-// its traffic, and the joining of a walk's pieces goes one after another. The constants
-// were fitted to calls with the pieces given; chosen by them -> the best of 1 to 16 pieces,
-// us: 600 tokens on 3000 rows 61.4 -> 61.4 (3 pieces; 2 69.6, uncut 104), 300 on 7892 68.9 ->
+// its traffic, and the joining of a walk's pieces goes one after another. Measured,
+// pieces as chosen by it -> the best of 1 to 16 that were forced (VXFA_PAGED_PIECES), us:
+// 600 tokens on 3000 rows 61.4 -> 61.4 (3 pieces; 2 69.6, uncut 104), 300 on 7892 68.9 ->
 // 68.3, 100 on 8092 45.3 -> 44.9, 1200 on 1200 42.0 -> 42.4, 2 streams of 256 on 4000 57.6 ->
 // 56.8, 4 uneven ones of up to 500 on 4000 53.7 -> 56.0 (of one count for all); 20 heads of
 // 64: 600 on 3000 35.2 -> 33.9, 100 on 8092 29.3 -> 29.1.
