@@ -143,3 +143,10 @@ def test_the_bounds_hold_a_planted_error():
 def test_smallest_exponents_of_the_slopes(ctx, bias, hq, hkv, hd, t):
     """Slopes near 1 for all heads (max_bias over the number of heads may be 0 in F32: no less a slope)."""
     check(ctx, without_weights(Batch([(t, t), (97, t), (300, t)], hq, hkv, hd, seed=t + 1)), bias=bias)
+
+
+@pytest.mark.parametrize("hq,hkv,hd", [(8, 2, 128), (5, 5, 64)])
+def test_wide_caps_on_cut_walks_with_absent_pages(ctx, hq, hkv, hd):
+    absent = [(0, i) for i in (0, 31, 32, 63, 64, 65, 127, 128, 200, 218)] + [(1, i) for i in range(60, 70)]
+    check(ctx, without_weights(Batch([(3500, 70), (2100, 150), (40, 3)], hq, hkv, hd, absent=absent, seed=34)), cap=2e3, bias=2.0)
+    check(ctx, without_weights(Batch([(3500, 1), (2100, 1), (40, 1)], hq, hkv, hd, absent=absent, seed=35)), cap=2e3)

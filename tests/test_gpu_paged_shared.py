@@ -97,3 +97,13 @@ def test_a_call_for_each_stream(ctx, hq, hkv, hd, t):
         check_out(d.out(), out, err, True)
         assert bits is None or np.array_equal(bits.view(np.uint32), got.view(np.uint32))
         bits = got
+
+
+@pytest.mark.parametrize("hkv,hd", [(2, 128), (4, 64)])
+def test_eviction_of_streams_that_share_pages(ctx, hkv, hd):
+    """Each stream's choice among the shared rows is its own; the shared pages stay as they were."""
+    from test_gpu_paged import evict
+    c = Batch([(n, 0) for n, _ in SIZES], 2 * hkv, hkv, hd, seed=52, spare=3 * 3 + 1)
+    c.table[1:, :SHARED] = c.table[0, :SHARED]
+    evict(ctx, c, 40, 4, 8)
+    evict(ctx, c, 40, 0, 0, with_kept=False)
