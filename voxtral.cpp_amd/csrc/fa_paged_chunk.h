@@ -41,8 +41,8 @@
 // bytes of scratch a lane.
 #pragma once
 
-#include "fa_paged.h"
 #include "fa_paged_plan.h"
+#include "fa_paged_q8.h"
 
 #include <type_traits>
 
@@ -72,6 +72,7 @@ struct ChunkArgs {
     float* rec;                // records [head group][slot][wavefront]
     ChunkTile* tiles;          // what the joining launch needs of every tile; [0].s: their number first
     int32_t nhg;
+    PagedScales sc;            // of pages of 8 bits
 };
 
 static __device__ const char pc_zeros[256] = {0};
@@ -83,15 +84,18 @@ __device__ __forceinline__ void pc_wait_vm() {
 }
 
 // MOD: 1 the scores have a distance term, 2 a cap (and a slope, or 0), 3 a wide one. QF16: q is F16.
-template <int HD, int KVGROUPS, bool QF16, int MOD>
-__global__ __launch_bounds__((PC<HD, KVGROUPS>::NT), 2) void paged_chunk_kernel(ChunkArgs ca) {
+// KV8: pages of 8 bits.
+template <int HD, int KVGROUPS, bool QF16, int MOD, bool KV8>
+static __global__ __launch_bounds__((PC<HD, KVGROUPS>::NT), 2) void paged_chunk_kernel(ChunkArgs ca) {
     using P = PC<HD, KVGROUPS>;
     constexpr int D = P::D, KS = P::KS, DB = P::DB, BK = P::BK, ROW = P::ROW, BLK = P::BLK, STEP = P::STEP, NS = P::NS,
                   NW = P::NW, REC = P::REC;
     // K steps, V steps, and with 8 wavefronts half of the Q staging. The first block
     // past the ring is zeros from step 0 on: V of a block dead for a wavefront's rows.
     constexpr int ZERO = 2 * NS * STEP, KVG = P::KVG;
-    constexpr int REGION = ZERO + (NW == 8 ? 4 : 1) * BLK;     // a group's
+    // KV8: the scales of 32 steps' granules, with 8 wavefronts where the last one's Q was staged
+    constexpr int TAB = ZERO + (NW == 8 ? 3 : 1) * BLK;
+    constexpr int REGION = ZERO + (NW == 8 ? 4 : 1) * BLK + (KV8 && NW != 8 ? 2048 : 0);     // a group's
     constexpr bool REV = MOD != 0;                        // blocks from the last
     __shared__ __attribute__((aligned(16))) char smem_all[KVG * REGION];
 
@@ -178,13 +182,28 @@ __global__ __launch_bounds__((PC<HD, KVGROUPS>::NT), 2) void paged_chunk_kernel(
     int64_t offs = -1;
     int ids_from = 0;
     uint64_t there = 0, there_before = 0;
+    floatx4 scales = {1.f, 0.f, 1.f, 0.f};                // KV8: of the lane's granule K's, log2 of V's, 1 / V's
     auto load_ids = [&](int u0) {
         const int u = u0 + (lane >> 2), row = step_row(u) + 16 * (lane & 3);
         const int p = u < nstep && row < st.n ? paged_page(a.b, it.s, row >> lg) : -1;
         offs = p >= 0 ? a.kv.at(p, hk, row & ((1 << lg) - 1)) : -1;
+        if constexpr (KV8) {
+            scales = floatx4{1.f, 0.f, 1.f, 0.f};
+            if (wave == NW - 1 && p >= 0) {
+                const int64_t at = ca.sc.at(p, hk, row & ((1 << lg) - 1));
+                const float sv = scale_in_range(*(const float*)(ca.sc.v + at));
+                scales = floatx4{scale_in_range(*(const float*)(ca.sc.k + at)), __builtin_amdgcn_logf(sv), __builtin_amdgcn_rcpf(sv), 0.f};
+            }
+        }
         there_before = there;
         there = __ballot(p >= 0);
         ids_from = u0;
+    };
+    // (written by the last wavefront, 3 steps ahead of their use at least; the half that is
+    // overwritten was of the 16 steps before the last 16)
+    auto put_scales = [&](int u0) {
+        if constexpr (KV8)
+            if (wave == NW - 1) *(floatx4*)(smem + TAB + 1024 * ((u0 >> 4) & 1) + 16 * lane) = scales;
     };
     const uint32_t lds0 = lds_offset(smem);
     const int lrow = lane / CH;
@@ -241,7 +260,46 @@ __global__ __launch_bounds__((PC<HD, KVGROUPS>::NT), 2) void paged_chunk_kernel(
             for (int i = 0; i < 2; ++i) dma16(vp[i], ov[i], vd + RPI * (wave + NW * i) * ROW);
         }
     };
-    for (int u = 0; u < min(nstep, 2); ++u) issue(u);
+    // KV8: a lane's 16 bytes of K and V of a step (a row has CH / 2 lanes) go through its
+    // registers, a step long, and to the ring as f16: converted once, not by each wavefront
+    // that reads them.
+    constexpr int CH8 = D / 16, RPW = 64 / CH8;
+    static_assert(NW * RPW == 2 * BK && (16 % RPW == 0), "a wavefront's rows lie in one granule");
+    struct Raw {
+        u32x4 k, v;
+    };
+    auto load8 = [&](int u, Raw& w) {
+        if ((u & 15) == 0) {
+            load_ids(u);
+            if (u > 0) put_scales(u);
+        }
+        const int g = 4 * (u & 15) + RPW * wave / 16;
+        const int lo = __builtin_amdgcn_readlane((int)(uint32_t)offs, g), hi = __builtin_amdgcn_readlane((int)(offs >> 32), g);
+        const int64_t at = ((int64_t)hi << 32) | (uint32_t)lo;
+        // (absent: zeros, all rows the same ones)
+        const char *kp = hi < 0 ? pc_zeros : a.kv.k + at, *vp = hi < 0 ? pc_zeros : a.kv.v + at;
+        const uint32_t r = (uint32_t)(RPW * wave + lane / CH8) & (hi < 0 ? 0u : 15u);
+        const uint32_t off = r * (uint32_t)a.kv.nb1 + 16 * (lane % CH8);
+        w.k = *(const u32x4*)(kp + off);
+        w.v = *(const u32x4*)(vp + off);
+    };
+    auto store8 = [&](int u, const Raw& w) {
+        const int r = RPW * wave + lane / CH8, j = 2 * (lane % CH8);
+        char* const kd = smem + (u & (NS - 1)) * STEP + r * ROW;
+        char* const vd = kd + NS * STEP;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            *(half8*)(kd + (((j + i) ^ swz_k<D>(r)) * 16)) = half8_of_bytes(w.k[2 * i], w.k[2 * i + 1]);
+            *(half8*)(vd + (((j + i) ^ swz_v<D>(r)) * 16)) = half8_of_bytes(w.v[2 * i], w.v[2 * i + 1]);
+        }
+    };
+    Raw raw, raw1;
+    if constexpr (KV8) {
+        if (nstep > 0) load8(0, raw);
+        if (nstep > 1) load8(1, raw1);
+    } else {
+        for (int u = 0; u < min(nstep, 2); ++u) issue(u);
+    }
 
     // ---- Q operand: row qrow, dims 16 ks + 8 hh .. + 7, in f16; the sign of the
     // scale folded in (0 for scale 0) -----------------------------------------------
@@ -269,6 +327,12 @@ __global__ __launch_bounds__((PC<HD, KVGROUPS>::NT), 2) void paged_chunk_kernel(
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) qb[ks] = *(const half8*)(qs + nl * ROW + (((2 * ks + hh) ^ (nl % CH)) * 16));
         __builtin_amdgcn_wave_barrier();
+    }
+    if constexpr (KV8) {
+        put_scales(0);
+        if (nstep > 0) store8(0, raw);
+        if (nstep > 1) store8(1, raw1);
+        if (nstep > 2) load8(2, raw);
     }
     // the block of zeros (past the ring: by the wavefront whose rows it held)
     if constexpr (NW == 8) {
@@ -355,8 +419,22 @@ __global__ __launch_bounds__((PC<HD, KVGROUPS>::NT), 2) void paged_chunk_kernel(
     // MOD 2: cap - 2 cap / (1 + 2^(c s)) + slope (j - p); MOD 3: paged_wide_cap of c s + slope (j - p)
     const float slope = MOD ? __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, paged_slope(a, h)))) : 0.f;
     float m = -INFINITY, l = 0.f;
+    // KV8: the block's scales for the lane's granule: K's times c; log2 of V's, which is added to the
+    // scores (P are then the weights of whole numbers, and rounded as such whatever the scales);
+    // 1 / V's, which the sum of P takes back
+    float cs = c, lsv = 0.f, isv = 1.f;
+    auto scales_of = [&](int t) {
+        if constexpr (KV8) {
+            const int u = t >> 1;
+            const floatx4 x = *(const floatx4*)(smem + TAB + 1024 * ((u >> 4) & 1) + 16 * (4 * (u & 15) + 2 * (REV ? 1 - (t & 1) : t & 1) + hh));
+            cs = c * x[0];
+            lsv = x[1];
+            isv = x[2];
+        }
+    };
     // element j of block t, plus `base`
     auto terms = [&](int t, float base, float (&e)[2]) {
+        if constexpr (KV8) base += lsv;
         if constexpr (MOD == 0) {
             e[0] = e[1] = base;
         } else {
@@ -367,11 +445,11 @@ __global__ __launch_bounds__((PC<HD, KVGROUPS>::NT), 2) void paged_chunk_kernel(
         }
     };
     auto score = [&](float s, const float (&e)[2], int j) -> float {
-        if constexpr (MOD == 0) return fmaf(s, c, e[0]);
+        if constexpr (MOD == 0) return fmaf(s, cs, e[0]);
         const float tj = fmaf(slope, (float)j, e[j >> 3]);
-        if constexpr (MOD == 1) return fmaf(s, c, tj);
-        if constexpr (MOD == 3) return paged_wide_cap(s * c, a.cap, a.capk) + tj;
-        return fmaf(-2.f * a.cap, __builtin_amdgcn_rcpf(1.f + exp2_fast(s * c)), tj);
+        if constexpr (MOD == 1) return fmaf(s, cs, tj);
+        if constexpr (MOD == 3) return paged_wide_cap(s * cs, a.cap, a.capk) + tj;
+        return fmaf(-2.f * a.cap, __builtin_amdgcn_rcpf(1.f + exp2_fast(s * cs)), tj);
     };
     // a few scores at a time: with all 16 in flight the registers do not do
     auto few = [](int j) {
@@ -434,15 +512,17 @@ __global__ __launch_bounds__((PC<HD, KVGROUPS>::NT), 2) void paged_chunk_kernel(
             raise(block_max(sc, t));
             ls = exps(sc, p, t);
         }
-        l += ls;
+        l = KV8 ? fmaf(ls, isv, l) : l + ls;
     };
 
     // before step 0: steps 0 and 1 (step 2's loads may stay in flight)
-    if (nstep > 2) {
-        issue(2);
-        pc_wait_vm<4>();
-    } else {
-        pc_wait_vm<0>();
+    if constexpr (!KV8) {
+        if (nstep > 2) {
+            issue(2);
+            pc_wait_vm<4>();
+        } else {
+            pc_wait_vm<0>();
+        }
     }
     __syncthreads();
 
@@ -459,6 +539,7 @@ __global__ __launch_bounds__((PC<HD, KVGROUPS>::NT), 2) void paged_chunk_kernel(
         if (nb > 0) {
             read_k(0, kr);
             s_mfma(sa, kr);
+            scales_of(0);
             mask_test(0);
             mask_fix(sa, 0);
             m = block_max(sa, 0);
@@ -466,6 +547,7 @@ __global__ __launch_bounds__((PC<HD, KVGROUPS>::NT), 2) void paged_chunk_kernel(
         // half t: PV(t - 1), S(t + 1) and the softmax of S(t)
         auto half = [&](int t, floatx16& scur, floatx16& snext, half8 (&pcur)[2], half8 (&pprev)[2]) {
             const int va = mask_test(t);
+            scales_of(t);
             mask_fix(scur, t);
             read_k(t + 1, kr);
             pv_mfma(pprev, vr);
@@ -477,16 +559,24 @@ __global__ __launch_bounds__((PC<HD, KVGROUPS>::NT), 2) void paged_chunk_kernel(
         // (whole steps: a second block past nb has no live score, and the last
         // half's S is not used)
         for (int u = 0; u < (KVG == 1 ? nstep : steps); ++u) {
-            if (u + NS - 1 < nstep) issue(u + NS - 1);
+            if constexpr (KV8) {
+                // (step u - 2 had the slot, and has been read)
+                if (u + 2 < nstep) store8(u + 2, raw);
+                if (u + 3 < nstep) load8(u + 3, raw);
+            } else {
+                if (u + NS - 1 < nstep) issue(u + NS - 1);
+            }
             if (active && (KVG == 1 || u < nstep)) {
                 half(2 * u, sa, sb, pa, pb);
                 half(2 * u + 1, sb, sa, pb, pa);
             }
             // K of step u + 2 and V of step u + 1 have landed: at most the
             // loads of step u + 3 and V of step u + 2 are in flight
-            if (u + 3 < nstep) pc_wait_vm<6>();
-            else if (u + 2 < nstep) pc_wait_vm<2>();
-            else pc_wait_vm<0>();
+            if constexpr (!KV8) {
+                if (u + 3 < nstep) pc_wait_vm<6>();
+                else if (u + 2 < nstep) pc_wait_vm<2>();
+                else pc_wait_vm<0>();
+            }
             __syncthreads();
         }
         if (nb > 0) pv_mfma(pb, vr);
@@ -552,7 +642,7 @@ __global__ __launch_bounds__((PC<HD, KVGROUPS>::NT), 2) void paged_chunk_kernel(
 // Joins the pieces of a tile in order: a wavefront per 32 output dims of a
 // wavefront's tile, four records' loads in flight.
 template <int HD>
-__global__ __launch_bounds__(64 * PC<HD>::DB) void paged_chunk_combine(ChunkArgs ca) {
+static __global__ __launch_bounds__(64 * PC<HD>::DB) void paged_chunk_combine(ChunkArgs ca) {
     using P = PC<HD>;
     constexpr int D = P::D, NW = P::NW, REC = P::REC, UP = 4;
     const PagedAttn& a = ca.a;
@@ -618,20 +708,22 @@ __global__ __launch_bounds__(64 * PC<HD>::DB) void paged_chunk_combine(ChunkArgs
     if (a.lse && db == 0 && hh == 0) a.lse[row] = L == 0.f ? INFINITY : M + log2f(L);
 }
 
-template <int HD, int KVG, bool QF16>
+template <int HD, int KVG, bool QF16, bool KV8>
 static void launch_pc(const ChunkArgs& ca, unsigned nwg, hipStream_t st) {
     const dim3 grid(nwg), block(PC<HD, KVG>::NT);
-    if (ca.a.capk != 0.f) hipLaunchKernelGGL((paged_chunk_kernel<HD, KVG, QF16, 3>), grid, block, 0, st, ca);
-    else if (ca.a.cap != 0.f) hipLaunchKernelGGL((paged_chunk_kernel<HD, KVG, QF16, 2>), grid, block, 0, st, ca);
-    else if (ca.a.n2 != 0) hipLaunchKernelGGL((paged_chunk_kernel<HD, KVG, QF16, 1>), grid, block, 0, st, ca);
-    else hipLaunchKernelGGL((paged_chunk_kernel<HD, KVG, QF16, 0>), grid, block, 0, st, ca);
+    if (ca.a.capk != 0.f) hipLaunchKernelGGL((paged_chunk_kernel<HD, KVG, QF16, 3, KV8>), grid, block, 0, st, ca);
+    else if (ca.a.cap != 0.f) hipLaunchKernelGGL((paged_chunk_kernel<HD, KVG, QF16, 2, KV8>), grid, block, 0, st, ca);
+    else if (ca.a.n2 != 0) hipLaunchKernelGGL((paged_chunk_kernel<HD, KVG, QF16, 1, KV8>), grid, block, 0, st, ca);
+    else hipLaunchKernelGGL((paged_chunk_kernel<HD, KVG, QF16, 0, KV8>), grid, block, 0, st, ca);
 }
 
-template <int HD>
-static hipError_t launch_chunk(const PagedAttn& a, hipStream_t st) {
+// sc: of pages of 8 bits (null: F16)
+template <int HD, bool KV8>
+static hipError_t launch_chunk(const PagedAttn& a, const PagedScales* sc, hipStream_t st) {
     using P = PC<HD>;
     ChunkArgs ca;
     ca.a = a;
+    ca.sc = KV8 ? *sc : PagedScales{};
     uint32_t l2 = 0;
     while ((2 << l2) <= P::NW && (a.hq / a.hkv) % (2 << l2) == 0) ++l2;
     const int hpw = 1 << l2;
@@ -646,13 +738,13 @@ static hipError_t launch_chunk(const PagedAttn& a, hipStream_t st) {
     if (nwg > 0xffffffffll / 512) return hipErrorNotSupported;
     if constexpr (HD == 64) {
         if (ca.p.kvg == 2) {
-            if (a.q_f16) launch_pc<HD, 2, true>(ca, (unsigned)nwg, st);
-            else launch_pc<HD, 2, false>(ca, (unsigned)nwg, st);
+            if (a.q_f16) launch_pc<HD, 2, true, KV8>(ca, (unsigned)nwg, st);
+            else launch_pc<HD, 2, false, KV8>(ca, (unsigned)nwg, st);
         }
     }
     if (ca.p.kvg == 1) {
-        if (a.q_f16) launch_pc<HD, 1, true>(ca, (unsigned)nwg, st);
-        else launch_pc<HD, 1, false>(ca, (unsigned)nwg, st);
+        if (a.q_f16) launch_pc<HD, 1, true, KV8>(ca, (unsigned)nwg, st);
+        else launch_pc<HD, 1, false, KV8>(ca, (unsigned)nwg, st);
     }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || !ca.p.cuts) return e;

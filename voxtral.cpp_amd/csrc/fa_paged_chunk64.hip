@@ -3,6 +3,6 @@
 
 namespace vxfa {
 
-hipError_t launch_paged_chunk64(const PagedAttn& a, hipStream_t st) { return launch_chunk<64>(a, st); }
+hipError_t launch_paged_chunk64(const PagedAttn& a, hipStream_t st) { return launch_chunk<64, false>(a, nullptr, st); }
 
 }  // namespace vxfa

@@ -66,6 +66,26 @@ def weight_pages(n_pages: int, page_size: int, kv_heads: int):
     return ne, nb
 
 
+def scale_pages(n_pages: int, page_size: int, kv_heads: int, rows: int = 16):
+    """Scales beside a page pool of 8 bits (one per 16 rows and head), or beside the
+    bounds of its blocks of `rows`: F32 [page_size / rows, kv_heads, n_pages, 1].
+    Backing buffer: [n_pages][kv_heads][page_size / rows]."""
+    n = page_size // rows
+    ne = (n, kv_heads, n_pages, 1)
+    nb = (F32_SIZE, n * F32_SIZE, kv_heads * n * F32_SIZE, n_pages * kv_heads * n * F32_SIZE)
+    return ne, nb
+
+
+def bound_pages(n_pages: int, page_size: int, kv_heads: int, hd: int, block: int):
+    """Bounds of the keys of blocks of `block` rows beside a page pool, I8 [2 hd,
+    page_size / block, kv_heads, n_pages]. Backing buffer:
+    [n_pages][kv_heads][page_size / block][2][hd] (upper, lower)."""
+    n = page_size // block
+    ne = (2 * hd, n, kv_heads, n_pages)
+    nb = (1, 2 * hd, n * 2 * hd, kv_heads * n * 2 * hd)
+    return ne, nb
+
+
 def dst(hd: int, heads: int, n_tokens: int, batch: int = 1, elt: int = F32_SIZE):
     """Output of flash_attn_ext: F32 [hd, heads, n_tokens, batch], contiguous
     (already permuted; voxtral then applies cont + reshape, :1612, :1804).

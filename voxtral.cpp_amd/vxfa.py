@@ -13,7 +13,7 @@ import os
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libvxfa.so")
 
-F32, F16 = 0, 1  # equal to ggml's GGML_TYPE_F32 / GGML_TYPE_F16
+F32, F16, I8 = 0, 1, 24  # equal to ggml's GGML_TYPE_F32 / GGML_TYPE_F16 / GGML_TYPE_I8
 
 OK, UNSUPPORTED, INVALID_ARG, NO_WORKSPACE, HIP_ERROR = 0, 1, 2, 3, 4
 
@@ -35,6 +35,11 @@ EXPORTS = (
     "vxfa_paged_append",
     "vxfa_flash_attn_ext_paged",
     "vxfa_paged_evict",
+    "vxfa_paged_append_q8",
+    "vxfa_flash_attn_ext_paged_q8",
+    "vxfa_paged_bounds",
+    "vxfa_paged_select",
+    "vxfa_flash_attn_ext_paged_blocks",
     "vxfa_status_str",
     "vxfa_last_error",
     "vxfa_version",
@@ -142,6 +147,23 @@ def evict(pages_ptr: int, max_pages: int, budget: int, n_sink: int = 0, n_recent
     return e
 
 
+class VxfaBlocks(ctypes.Structure):
+    """vxfa_blocks: the blocks chosen for each token and kv head (device int32 pointer)."""
+    _fields_ = [
+        ("list", ctypes.c_void_p),
+        ("block", ctypes.c_int32),
+        ("top", ctypes.c_int32),
+        ("n_sink", ctypes.c_int32),
+        ("n_recent", ctypes.c_int32),
+    ]
+
+
+def blocks(list_ptr: int, block: int, top: int, n_sink: int = 0, n_recent: int = 0) -> VxfaBlocks:
+    b = VxfaBlocks()
+    b.list, b.block, b.top, b.n_sink, b.n_recent = list_ptr, block, top, n_sink, n_recent
+    return b
+
+
 class VxfaError(RuntimeError):
     def __init__(self, status: int, msg: str):
         super().__init__(f"vxfa status {status} ({status_str(status)}): {msg}")
@@ -202,6 +224,17 @@ def load() -> ctypes.CDLL:
     L.vxfa_flash_attn_ext_paged.restype = ctypes.c_int
     L.vxfa_paged_evict.argtypes = [ctypes.c_void_p, P, P, P, B, ctypes.POINTER(VxfaEvict), ctypes.c_void_p]
     L.vxfa_paged_evict.restype = ctypes.c_int
+    F, C = ctypes.c_float, ctypes.POINTER(VxfaBlocks)
+    L.vxfa_paged_append_q8.argtypes = [ctypes.c_void_p, P, P, B, P, P, P, P, ctypes.POINTER(VxfaRope), P, P, ctypes.c_void_p]
+    L.vxfa_paged_append_q8.restype = ctypes.c_int
+    L.vxfa_flash_attn_ext_paged_q8.argtypes = [ctypes.c_void_p, P, P, P, P, P, B, P, F, F, F, ctypes.c_void_p]
+    L.vxfa_flash_attn_ext_paged_q8.restype = ctypes.c_int
+    L.vxfa_paged_bounds.argtypes = [ctypes.c_void_p, P, P, B, P, P, ctypes.c_void_p]
+    L.vxfa_paged_bounds.restype = ctypes.c_int
+    L.vxfa_paged_select.argtypes = [ctypes.c_void_p, P, P, P, B, C, ctypes.c_void_p]
+    L.vxfa_paged_select.restype = ctypes.c_int
+    L.vxfa_flash_attn_ext_paged_blocks.argtypes = [ctypes.c_void_p, P, P, P, P, P, B, C, P, F, F, F, ctypes.c_void_p]
+    L.vxfa_flash_attn_ext_paged_blocks.restype = ctypes.c_int
     L.vxfa_status_str.argtypes = [ctypes.c_int]
     L.vxfa_status_str.restype = ctypes.c_char_p
     L.vxfa_last_error.argtypes = [ctypes.c_void_p]
@@ -339,6 +372,48 @@ class Context:
     def paged_evict(self, k, v, weights, batch, evict_desc, stream: int = 0, check: bool = True) -> int:
         """Each stream's rows of the largest weights (VxfaEvict), per kv head, moved to other pages."""
         rc = self._lib.vxfa_paged_evict(self._h, k, v, weights, batch, evict_desc, stream)
+        if check and rc != OK:
+            raise VxfaError(rc, self.last_error())
+        return rc
+
+    def paged_append_q8(self, k_new, v_new, batch, k, k_scale, v, v_scale, rope=None, q=None, q_out=None,
+                        stream: int = 0, check: bool = True) -> int:
+        """paged_append into pages of 8 bits with a scale for each 16 rows and head."""
+        rc = self._lib.vxfa_paged_append_q8(self._h, k_new, v_new, batch, k, k_scale, v, v_scale, rope, q, q_out, stream)
+        if check and rc != OK:
+            raise VxfaError(rc, self.last_error())
+        return rc
+
+    def flash_attn_ext_paged_q8(self, q, k, k_scale, v, v_scale, batch, dst, scale: float, max_bias: float = 0.0,
+                                logit_softcap: float = 0.0, stream: int = 0, check: bool = True) -> int:
+        """flash_attn_ext_paged (without weights) over pages of 8 bits."""
+        rc = self._lib.vxfa_flash_attn_ext_paged_q8(self._h, q, k, k_scale, v, v_scale, batch, dst, scale, max_bias,
+                                                    logit_softcap, stream)
+        if check and rc != OK:
+            raise VxfaError(rc, self.last_error())
+        return rc
+
+    def paged_bounds(self, k, k_scale, batch, bounds, bounds_scale, stream: int = 0, check: bool = True) -> int:
+        """Bounds of the keys of the blocks with new rows (k_scale: None for an F16 pool)."""
+        rc = self._lib.vxfa_paged_bounds(self._h, k, k_scale, batch, bounds, bounds_scale, stream)
+        if check and rc != OK:
+            raise VxfaError(rc, self.last_error())
+        return rc
+
+    def paged_select(self, q, bounds, bounds_scale, batch, blocks_desc, stream: int = 0, check: bool = True) -> int:
+        """Blocks for each new token and kv head by their bounds, into blocks_desc's list (VxfaBlocks)."""
+        rc = self._lib.vxfa_paged_select(self._h, q, bounds, bounds_scale, batch, blocks_desc, stream)
+        if check and rc != OK:
+            raise VxfaError(rc, self.last_error())
+        return rc
+
+    def flash_attn_ext_paged_blocks(self, q, k, k_scale, v, v_scale, batch, blocks_desc, dst, scale: float,
+                                    max_bias: float = 0.0, logit_softcap: float = 0.0, stream: int = 0,
+                                    check: bool = True) -> int:
+        """flash_attn_ext_paged (without weights) over the rows of chosen blocks alone (VxfaBlocks); F16 pools
+        (k_scale and v_scale None) or of 8 bits."""
+        rc = self._lib.vxfa_flash_attn_ext_paged_blocks(self._h, q, k, k_scale, v, v_scale, batch, blocks_desc, dst,
+                                                        scale, max_bias, logit_softcap, stream)
         if check and rc != OK:
             raise VxfaError(rc, self.last_error())
         return rc
