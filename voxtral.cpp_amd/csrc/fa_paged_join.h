@@ -1,9 +1,11 @@
-// fa_paged_join.h — the parts that the rows of a stream's few tokens are cut into: their
-// records, and the launch that joins them (for fa_paged_rows.hip and fa_paged_walk.hip).
+// fa_paged_join.h — what fa_paged_rows.hip and fa_paged_walk.hip share: the parts that the
+// rows of a stream's few tokens are cut into, their records, the launch that joins them;
+// loads to LDS.
 #pragma once
 
 #include "fa_paged.h"
 #include "fa_paged_plan.h"
+#include "fa_paged_q8.h"
 
 namespace vxfa {
 
@@ -24,6 +26,19 @@ struct RowsArgs {
     int32_t whole;            // no stream is cut and no group shared: the weights need no launch of their own
 };
 
+// dma16 with a nontemporal hint: rows are read once
+__device__ __forceinline__ void dma16_nt(const char* base, uint32_t off, uint32_t lds) {
+    asm volatile("global_load_lds_dwordx4 %0, %1 nt" ::"v"(off), "s"(base), "{m0}"(lds) : "memory");
+}
+
+template <int N>
+__device__ __forceinline__ void pr_wait_vm() {
+    static_assert(N >= 0 && N < 64, "vmcnt range");
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+// LDS reads done: their slot may be written again
+__device__ __forceinline__ void pr_wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
 __device__ __forceinline__ float quad_max(float x) {   // over lanes l ^ 16, l ^ 32
     const int xi = __builtin_bit_cast(int, x);
     const auto r = __builtin_amdgcn_permlane16_swap(xi, xi, false, false);
@@ -37,19 +52,29 @@ __device__ __forceinline__ float quad_sum(float x) {
 
 // Joins the parts of a stream: a wavefront per (token, query head, 32 dims), 8
 // lanes of 4 dims for every eighth part, all loads of 8 parts a lane at once.
-template <int D>
-static __global__ __launch_bounds__(64) void paged_rows_combine(RowsArgs ra) {
+// TOKENS: each packed token has `parts` of its own.
+template <int D, bool TOKENS>
+static __global__ __launch_bounds__(64) void paged_rows_combine(RowsArgs ra, int parts) {
     const PagedAttn& a = ra.a;
     const int lane = (int)threadIdx.x, f = lane & 7, grp = lane >> 3;
     // kv head fastest, as in the kernel that wrote the records
     const int hk = (int)blockIdx.x % a.hkv, rest = (int)blockIdx.x / a.hkv;
     const int g = rest / (D / 32), sl = rest % (D / 32);
-    const int i = (int)blockIdx.y, s = (int)blockIdx.z;
-    const PagedStream st = paged_stream(a.b, s);
+    const int i = TOKENS ? 0 : (int)blockIdx.y, s = (int)blockIdx.z;
+    PagedStream st;
+    int2 cut;
     // (one stream's parts begin at 0: its records are on their way before their number
     // is known)
-    const bool one = a.b.n_streams == 1;
-    const int2 cut = ra.cut[s];
+    bool one = a.b.n_streams == 1;
+    if constexpr (TOKENS) {
+        const int t = (int)blockIdx.y;
+        st = PagedStream{t, paged_token(a.b, t).s >= 0 ? 1 : 0, 0};
+        cut = int2{t * parts, parts};
+        one = false;
+    } else {
+        st = paged_stream(a.b, s);
+        cut = ra.cut[s];
+    }
     if (!one && (i >= min(st.t, a.b.max_nq) || cut.y <= 1)) return;
     const int first = one ? 0 : cut.x, nload = one ? ra.items : cut.y;
     const int sub = (int)ra.hpw.div((uint32_t)g), r = i * (int)ra.hpw.d + g - sub * (int)ra.hpw.d;

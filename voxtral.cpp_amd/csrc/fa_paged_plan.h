@@ -87,9 +87,14 @@ __device__ __forceinline__ int rows_first(const PagedStream& s, int window) {
 
 // rows of a part, given all streams' rows: whole rounds of four tiles
 __host__ __device__ __forceinline__ int rows_chunk(const RowsPlan& p, int64_t total) {
-    int64_t c = (total + p.small - 1) / p.small;
+    // (a division of 64 bits takes a hundred instructions: only where it has to be one)
+    auto parts_of = [&](int32_t n) -> int64_t {
+        if (total <= 0x40000000) return (int64_t)(((uint32_t)total + (uint32_t)n - 1) / (uint32_t)n);
+        return (total + n - 1) / n;
+    };
+    int64_t c = parts_of(p.small);
     if (c > p.limit) {
-        c = (total + p.large - 1) / p.large;
+        c = parts_of(p.large);
         if (c < p.limit) c = p.limit;
     }
     c = (c + 63) & ~(int64_t)63;
@@ -100,7 +105,8 @@ __host__ __device__ __forceinline__ int rows_chunk(const RowsPlan& p, int64_t to
 __host__ __device__ __forceinline__ int64_t rows_total(int64_t tiles, int n_streams) { return 16 * tiles + 15 * (int64_t)n_streams; }
 // parts of a stream of len rows
 __host__ __device__ __forceinline__ int rows_parts(const RowsPlan& p, int len, int chunk) {
-    return p.cuts && len > chunk ? (int)(((int64_t)len + chunk - 1) / chunk) : 1;
+    // (both at most 2^30)
+    return p.cuts && len > chunk ? (int)(((uint32_t)len + (uint32_t)chunk - 1) / (uint32_t)chunk) : 1;
 }
 
 #ifdef __HIPCC__

@@ -87,16 +87,20 @@ __host__ __device__ __forceinline__ int exp_for(float x) {
 // that rows which no token sees (whose scales may be anything) take part as zeros.
 __device__ __forceinline__ float scale_in_range(float s) { return fminf(fmaxf(s, two_to(kMinExp)), two_to(kMaxExp)); }
 
-// Two whole numbers in the low bytes of 16-bit halves (high bytes 0) as f16: with the
-// sign bit turned over and 0x64 above, byte b is the f16 number 1024 + (b + 128), exact, from
-// which 1152 leaves b.
-__device__ __forceinline__ half2 halves_of_bytes(uint32_t w) {
-    return __builtin_bit_cast(half2, w ^ 0x64806480u) - half2{(_Float16)1152.f, (_Float16)1152.f};
-}
-// the four bytes of w, in order
+// The four bytes of w, in order, as f16: with the sign bit turned over (b + 128) and 0x64 above
+// it a byte is the f16 number 1024 + (b + 128), exact, from which 1152 leaves b.
 __device__ __forceinline__ half4 half4_of_bytes(uint32_t w) {
-    const half2 lo = halves_of_bytes(__builtin_amdgcn_perm(0u, w, 0x0C010C00u)), hi = halves_of_bytes(__builtin_amdgcn_perm(0u, w, 0x0C030C02u));
+    const uint32_t u = w ^ 0x80808080u;
+    const half2 off = {(_Float16)1152.f, (_Float16)1152.f};
+    const half2 lo = __builtin_bit_cast(half2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - off;
+    const half2 hi = __builtin_bit_cast(half2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - off;
     return half4{lo[0], lo[1], hi[0], hi[1]};
+}
+// Two bytes b + 128 in the low halves' bits (the high bytes 0) as f16 numbers b / 512: as f16 the bits are
+// (b + 128) 2^-24, subnormal and exact; one multiply-add.
+__device__ __forceinline__ half2 halves_over_512(uint32_t w) {
+    const half2 f = {(_Float16)32768.f, (_Float16)32768.f}, off = {(_Float16)-0.25f, (_Float16)-0.25f};
+    return __builtin_elementwise_fma(__builtin_bit_cast(half2, w), f, off);
 }
 __device__ __forceinline__ half8 half8_of_bytes(uint32_t w0, uint32_t w1) {
     const half4 lo = half4_of_bytes(w0), hi = half4_of_bytes(w1);

@@ -41,19 +41,6 @@ namespace vxfa {
 constexpr int PR_WAVES = 4;
 constexpr int PR_TILE = 16;
 
-// dma16 with a nontemporal hint: rows are read once
-__device__ __forceinline__ void dma16_nt(const char* base, uint32_t off, uint32_t lds) {
-    asm volatile("global_load_lds_dwordx4 %0, %1 nt" ::"v"(off), "s"(base), "{m0}"(lds) : "memory");
-}
-
-template <int N>
-__device__ __forceinline__ void pr_wait_vm() {
-    static_assert(N >= 0 && N < 64, "vmcnt range");
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
-}
-// LDS reads done: their slot may be written again
-__device__ __forceinline__ void pr_wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
-
 template <int D>
 __global__ __launch_bounds__(64 * PR_WAVES, 2) void paged_rows_kernel(RowsArgs ra) {
     constexpr int KS = D / 32;                 // k steps of the first product
@@ -363,8 +350,8 @@ hipError_t launch_paged_rows(const PagedAttn& a, int head_dim, hipStream_t st, b
     if (e != hipSuccess) return e;
     if (ra.p.cuts) {
         const dim3 cg((unsigned)(a.hq * (head_dim / 32)), (unsigned)a.b.max_nq, (unsigned)a.b.n_streams);
-        if (head_dim == 128) hipLaunchKernelGGL((paged_rows_combine<128>), cg, dim3(64), 0, st, ra);
-        else hipLaunchKernelGGL((paged_rows_combine<64>), cg, dim3(64), 0, st, ra);
+        if (head_dim == 128) hipLaunchKernelGGL((paged_rows_combine<128, false>), cg, dim3(64), 0, st, ra, 0);
+        else hipLaunchKernelGGL((paged_rows_combine<64, false>), cg, dim3(64), 0, st, ra, 0);
         e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
