@@ -93,9 +93,9 @@ static __global__ __launch_bounds__((PC<HD, KVGROUPS>::NT), 2) void paged_chunk_
     // K steps, V steps, and with 8 wavefronts half of the Q staging. The first block
     // past the ring is zeros from step 0 on: V of a block dead for a wavefront's rows.
     constexpr int ZERO = 2 * NS * STEP, KVG = P::KVG;
-    // KV8: the scales of 32 steps' granules, with 8 wavefronts where the last one's Q was staged
-    constexpr int TAB = ZERO + (NW == 8 ? 3 : 1) * BLK;
-    constexpr int REGION = ZERO + (NW == 8 ? 4 : 1) * BLK + (KV8 && NW != 8 ? 2048 : 0);     // a group's
+    // KV8: the whole numbers of a step, and the scales of 32 steps' granules
+    constexpr int RAW = ZERO + BLK, TAB = RAW + 2 * NW * 1024;
+    constexpr int REGION = KV8 ? TAB + 2048 : ZERO + (NW == 8 ? 4 : 1) * BLK;     // a group's
     constexpr bool REV = MOD != 0;                        // blocks from the last
     __shared__ __attribute__((aligned(16))) char smem_all[KVG * REGION];
 
@@ -199,7 +199,7 @@ static __global__ __launch_bounds__((PC<HD, KVGROUPS>::NT), 2) void paged_chunk_
         there = __ballot(p >= 0);
         ids_from = u0;
     };
-    // (written by the last wavefront, 3 steps ahead of their use at least; the half that is
+    // (written by the last wavefront, 3 steps ahead of their use; the half that is
     // overwritten was of the 16 steps before the last 16)
     auto put_scales = [&](int u0) {
         if constexpr (KV8)
@@ -260,15 +260,18 @@ static __global__ __launch_bounds__((PC<HD, KVGROUPS>::NT), 2) void paged_chunk_
             for (int i = 0; i < 2; ++i) dma16(vp[i], ov[i], vd + RPI * (wave + NW * i) * ROW);
         }
     };
-    // KV8: a lane's 16 bytes of K and V of a step (a row has CH / 2 lanes) go through its
-    // registers, a step long, and to the ring as f16: converted once, not by each wavefront
-    // that reads them.
+    // KV8: a lane's 16 bytes of K and V of a step (a row has CH / 2 lanes) go to LDS as they are,
+    // and a step later through its registers to the ring as f16: converted once, not
+    // by each wavefront that reads them. (Kept in registers for that step they cost 4 to 20 spills; five steps ahead
+    // in LDS, with a ring of three slots, 8192 tokens took 591 us instead of 581.)
     constexpr int CH8 = D / 16, RPW = 64 / CH8;
     static_assert(NW * RPW == 2 * BK && (16 % RPW == 0), "a wavefront's rows lie in one granule");
+    const uint32_t raw0 = RAW + 2048 * wave;
     struct Raw {
         u32x4 k, v;
     };
-    auto load8 = [&](int u, Raw& w) {
+    // where the wavefront's rows of step u lie (absent: zeros, all rows the same ones)
+    auto find8 = [&](int u, const char*& kp, const char*& vp) -> uint32_t {
         if ((u & 15) == 0) {
             load_ids(u);
             if (u > 0) put_scales(u);
@@ -276,27 +279,40 @@ static __global__ __launch_bounds__((PC<HD, KVGROUPS>::NT), 2) void paged_chunk_
         const int g = 4 * (u & 15) + RPW * wave / 16;
         const int lo = __builtin_amdgcn_readlane((int)(uint32_t)offs, g), hi = __builtin_amdgcn_readlane((int)(offs >> 32), g);
         const int64_t at = ((int64_t)hi << 32) | (uint32_t)lo;
-        // (absent: zeros, all rows the same ones)
-        const char *kp = hi < 0 ? pc_zeros : a.kv.k + at, *vp = hi < 0 ? pc_zeros : a.kv.v + at;
-        const uint32_t r = (uint32_t)(RPW * wave + lane / CH8) & (hi < 0 ? 0u : 15u);
-        const uint32_t off = r * (uint32_t)a.kv.nb1 + 16 * (lane % CH8);
+        kp = hi < 0 ? pc_zeros : a.kv.k + at;
+        vp = hi < 0 ? pc_zeros : a.kv.v + at;
+        int ln = lane;
+        asm volatile("" : "+v"(ln));                      // (worked out here rather than held across the loop)
+        return ((uint32_t)(RPW * wave + ln / CH8) & (hi < 0 ? 0u : 15u)) * (uint32_t)a.kv.nb1 + 16 * (ln % CH8);
+    };
+    auto load8 = [&](int u, Raw& w) {
+        const char *kp, *vp;
+        const uint32_t off = find8(u, kp, vp);
         w.k = *(const u32x4*)(kp + off);
         w.v = *(const u32x4*)(vp + off);
     };
+    auto issue8 = [&](int u) {
+        const char *kp, *vp;
+        const uint32_t off = find8(u, kp, vp);
+        dma16(kp, off, lds0 + raw0);
+        dma16(vp, off, lds0 + raw0 + 1024);
+    };
     auto store8 = [&](int u, const Raw& w) {
-        const int r = RPW * wave + lane / CH8, j = 2 * (lane % CH8);
+        int ln = lane;
+        asm volatile("" : "+v"(ln));
+        const int r = RPW * wave + ln / CH8, j = 2 * (ln % CH8);
         char* const kd = smem + (u & (NS - 1)) * STEP + r * ROW;
         char* const vd = kd + NS * STEP;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            *(half8*)(kd + (((j + i) ^ swz_k<D>(r)) * 16)) = half8_of_bytes(w.k[2 * i], w.k[2 * i + 1]);
-            *(half8*)(vd + (((j + i) ^ swz_v<D>(r)) * 16)) = half8_of_bytes(w.v[2 * i], w.v[2 * i + 1]);
-        }
+        for (int i = 0; i < 2; ++i) *(half8*)(kd + (((j + i) ^ swz_k<D>(r)) * 16)) = half8_of_bytes(w.k[2 * i], w.k[2 * i + 1]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) *(half8*)(vd + (((j + i) ^ swz_v<D>(r)) * 16)) = half8_of_bytes(w.v[2 * i], w.v[2 * i + 1]);
     };
-    Raw raw, raw1;
+    Raw first0, first1;
     if constexpr (KV8) {
-        if (nstep > 0) load8(0, raw);
-        if (nstep > 1) load8(1, raw1);
+        if (nstep > 0) load8(0, first0);
+        if (nstep > 1) load8(1, first1);
+        if (nstep > 2) issue8(2);
     } else {
         for (int u = 0; u < min(nstep, 2); ++u) issue(u);
     }
@@ -308,9 +324,9 @@ static __global__ __launch_bounds__((PC<HD, KVGROUPS>::NT), 2) void paged_chunk_
     {
         const float sg = a.c < 0.f ? -1.0f : (a.c > 0.f ? 1.0f : 0.0f);
         // 16-byte chunk j of row r at j ^ (r % CH); wavefronts 0-3 in ring slot 3
-        // (filled from step 0 on), 4-7 past the ring
-        char* qs = smem + (wave < 2 ? 3 * STEP + wave * BLK
-                                    : (wave < 4 ? (NS + 3) * STEP + (wave - 2) * BLK : 2 * NS * STEP + (wave - 4) * BLK));
+        // (filled from step 0 on), 4-7 past the ring (KV8: in slot 2, which is, too)
+        const int w2 = wave & 1, slot = KV8 && wave >= 4 ? 2 : 3;
+        char* qs = smem + (wave >= 4 && !KV8 ? 2 * NS * STEP + (wave - 4) * BLK : ((wave & 2) ? NS + slot : slot) * STEP + w2 * BLK);
 #pragma unroll
         for (int u = 0; u < QL; ++u) {
             const int r = (64 / QCH) * u + lane / QCH, j = lane % QCH;
@@ -330,9 +346,8 @@ static __global__ __launch_bounds__((PC<HD, KVGROUPS>::NT), 2) void paged_chunk_
     }
     if constexpr (KV8) {
         put_scales(0);
-        if (nstep > 0) store8(0, raw);
-        if (nstep > 1) store8(1, raw1);
-        if (nstep > 2) load8(2, raw);
+        if (nstep > 0) store8(0, first0);
+        if (nstep > 1) store8(1, first1);
     }
     // the block of zeros (past the ring: by the wavefront whose rows it held)
     if constexpr (NW == 8) {
@@ -441,12 +456,20 @@ static __global__ __launch_bounds__((PC<HD, KVGROUPS>::NT), 2) void paged_chunk_
             const int d0 = block_row(t) - prow;
             if constexpr (MOD == 2) base += a.cap;
             e[0] = fmaf(slope, (float)(d0 + (hh ? 24 : 0)), base);
-            e[1] = fmaf(slope, (float)(d0 + (hh ? 8 : 0)), base);
+            e[1] = fmaf(slope, (float)(d0 + (hh ? 8 : 0) + (KV8 ? 8 : 0)), base);   // (KV8: of element 8, not 0)
         }
     };
     auto score = [&](float s, const float (&e)[2], int j) -> float {
         if constexpr (MOD == 0) return fmaf(s, cs, e[0]);
-        const float tj = fmaf(slope, (float)j, e[j >> 3]);
+        float tj;
+        if constexpr (KV8) {
+            // (multiples that are constants of the instruction: 3, 5, 6 and 7 would each take a register)
+            const float e4 = (j & 7) < 3 ? e[j >> 3] : fmaf(slope, 4.f, e[j >> 3]), e8 = (j & 7) < 7 ? e4 : fmaf(slope, 4.f, e4);
+            constexpr float f[8] = {0.f, 1.f, 2.f, -1.f, 0.f, 1.f, 2.f, -1.f};
+            tj = f[j & 7] == 0.f ? e4 : fmaf(slope, f[j & 7], e8);
+        } else {
+            tj = fmaf(slope, (float)j, e[j >> 3]);
+        }
         if constexpr (MOD == 1) return fmaf(s, cs, tj);
         if constexpr (MOD == 3) return paged_wide_cap(s * cs, a.cap, a.capk) + tj;
         return fmaf(-2.f * a.cap, __builtin_amdgcn_rcpf(1.f + exp2_fast(s * cs)), tj);
@@ -549,6 +572,16 @@ static __global__ __launch_bounds__((PC<HD, KVGROUPS>::NT), 2) void paged_chunk_
             const int va = mask_test(t);
             scales_of(t);
             mask_fix(scur, t);
+            if constexpr (KV8 && MOD >= 2) {
+                // (a cap's softmax takes the registers: S(t + 1) after it)
+                pv_mfma(pprev, vr);
+                softmax(scur, pcur, t);
+                __builtin_amdgcn_sched_barrier(0);
+                read_v(va, vr);
+                read_k(t + 1, kr);
+                s_mfma(snext, kr);
+                return;
+            }
             read_k(t + 1, kr);
             pv_mfma(pprev, vr);
             __builtin_amdgcn_sched_barrier(0x6);   // VALU and SALU may cross
@@ -561,8 +594,18 @@ static __global__ __launch_bounds__((PC<HD, KVGROUPS>::NT), 2) void paged_chunk_
         for (int u = 0; u < (KVG == 1 ? nstep : steps); ++u) {
             if constexpr (KV8) {
                 // (step u - 2 had the slot, and has been read)
-                if (u + 2 < nstep) store8(u + 2, raw);
-                if (u + 3 < nstep) load8(u + 3, raw);
+                if (u + 2 < nstep) {
+                    pc_wait_vm<0>();
+                    asm volatile("" ::: "memory");
+                    Raw w;
+                    w.k = *(const u32x4*)(smem + raw0 + 16 * lane);
+                    w.v = *(const u32x4*)(smem + raw0 + 1024 + 16 * lane);
+                    store8(u + 2, w);
+                    // (the whole numbers have been read: the next ones may come)
+                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                    if (u + 3 < nstep) issue8(u + 3);
+                }
+                __builtin_amdgcn_sched_barrier(0);
             } else {
                 if (u + NS - 1 < nstep) issue(u + NS - 1);
             }
