@@ -505,9 +505,11 @@ typedef struct vxfa_blocks {
  * negative scale of the attention turns its meaning around.) q [D, T, Hq, 1] F16 or F32. Tokens
  * of no stream leave the list as it was. bounds_scale: powers of two from 2^-64 to 2^64 (others: the
  * choice may differ from the formula's). At most 262144 blocks of a stream
- * (max_nkv), else VXFA_UNSUPPORTED. Needs 8 bytes of the workspace for each token, kv head
- * and one of min(top, 4096) blocks, where streams have more than 4096 blocks (fewer
- * where kv heads have fewer than 4 query heads: 1024 for 1), for every 4096 (1024) blocks (else VXFA_NO_WORKSPACE).
+ * (max_nkv; else VXFA_UNSUPPORTED). Where streams have more than 4096 blocks (with 16 / n
+ * tokens of a stream at once for kv heads of n query heads, n rounded up to a power of
+ * two, 16384 by that many), and with few tokens from 512 on, the call leaves the best of segments of
+ * blocks in the workspace, 8 bytes times top for each token, kv head and segment (else
+ * VXFA_NO_WORKSPACE).
  * Asynchronous on `stream`. */
 int vxfa_paged_select(vxfa_ctx* ctx, const vxfa_tensor* q,
                       const vxfa_tensor* bounds, const vxfa_tensor* bounds_scale,

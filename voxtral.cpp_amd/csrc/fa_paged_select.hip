@@ -5,7 +5,10 @@
 // q is larger than sum_d max(q_d lo_d, q_d hi_d) = sum_d max(q_d, 0) hi_d + min(q_d, 0) lo_d.
 // With bounds and queries in 8 bits at scales that are powers of two that is one
 // product of whole numbers, of length 2 D, on v_mfma_i32_16x16x64_i8: exact, so the choice depends on
-// no order of sums. Bound by the bytes of the bounds: 2 D + 4 a block and kv head.
+// no order of sums. The choice is bound by the chain of its loads (sizes, pages, bounds), each of
+// about a microsecond, and the search: one stream of 128 blocks 8.7 us in a graph, of 512 12.9, 32 uneven ones of up
+// to 512 18 (19 MB of bounds: 4 us at what a large copy reaches), of up to 2048 41 (76 MB). Bounds of
+// a token's blocks 6.2 us, of 8192 tokens' keys of 16 bits in blocks of 32 4.9.
 #include "fa_paged_q8.h"
 
 namespace vxfa {
@@ -97,16 +100,17 @@ hipError_t launch_paged_bounds(const PagedBounds& a, hipStream_t st) {
 }
 
 // ---- choice ------------------------------------------------------------------------
-// A workgroup per tile of tokens of one stream, kv head and segment of blocks. Columns
-// of the product: tokens x query heads of the group (padded to a power of two, gp;
-// groups above 16 in passes), rows: 16 blocks a wavefront and step. Scores, as
-// unsigned keys that order as they do, go to LDS; a wavefront per token finds the key of
-// the last block to be chosen, bit by bit from the highest in which two keys
-// differ, counting keys by ballots, and stops where a threshold leaves just as many
-// as are wanted; then it lists them in order. Streams of more blocks than a segment: each
-// segment leaves its best (key, block) and paged_select_join chooses among those.
+// A workgroup of 16 wavefronts per tile of tokens of one stream, kv head and segment of
+// blocks. Columns of the product: tokens x query heads of the group (padded to a power of two,
+// gp; groups above 16 in passes), rows: 16 blocks a wavefront and step, two steps' loads in
+// flight. Scores, as unsigned keys that order as they do, go to LDS. The key of the last block to be
+// chosen is found bit by bit from the highest in which two keys differ, by counting keys
+// (ballots), and the search stops where a threshold leaves just as many as are wanted; then
+// they are listed in order: by a wavefront per token where there are several and few blocks, else by all
+// of them, token by token. Streams of more blocks than a segment: each segment leaves its best
+// (key, block) and paged_select_join chooses among those.
 
-constexpr int SL_NT = 512;
+constexpr int SL_WAVES = 16;                           // wavefronts of a workgroup at most
 constexpr uint32_t kForced = 0xFFFFFFFFu;              // a first or last block
 struct SelectArgs {
     PagedSelect a;
@@ -123,20 +127,32 @@ __device__ __forceinline__ uint32_t score_key(float x) {
     return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 
-// One wavefront: of n keys key(i) (0: no candidate) the `want` largest, of equal ones the first;
-// put(rank, i) of each, in order. Returns how many. REGS: 64 REGS keys or fewer, kept in registers.
-template <int REGS, class K, class P>
-__device__ __forceinline__ int wave_choose(int n, int want, int lane, K key, P put) {
+// LDS of the wavefronts that choose together.
+struct ChooseRoom {
+    uint32_t cnt[3][8];        // counts of keys from seven thresholds on, in turn
+    uint32_t first[4][SL_WAVES], over[SL_WAVES], same[SL_WAVES];
+};
+
+__device__ __forceinline__ uint32_t wave_largest(uint32_t x) { return (uint32_t)wave_max((int)(x ^ 0x80000000u)) ^ 0x80000000u; }
+
+// Of n keys key(i) (0: no candidate) the `want` largest, of equal ones the first; put(rank, i) of each,
+// in order. Returns how many. TEAM: all that many wavefronts of the workgroup, each with keys 64 REGS wave .. in
+// registers, three bits of the threshold a round (a round is a barrier); 0:
+// one wavefront, a bit a round, REGS 0: any number of keys, read again each time.
+template <int TEAM, int REGS, class K, class P>
+__device__ __forceinline__ int choose(ChooseRoom* room, int wave, int lane, int n, int want, K key, P put) {
+    constexpr int NT = TEAM > 0 ? TEAM : 1;
+    const int at = TEAM ? 64 * REGS * wave : 0;
     uint32_t reg[REGS > 0 ? REGS : 1];
     if constexpr (REGS > 0) {
 #pragma unroll
-        for (int c = 0; c < REGS; ++c) reg[c] = 64 * c + lane < n ? key(64 * c + lane) : 0u;
+        for (int c = 0; c < REGS; ++c) reg[c] = at + 64 * c + lane < n ? key(at + 64 * c + lane) : 0u;
     }
     auto each = [&](auto f) {
         if constexpr (REGS > 0) {
 #pragma unroll
             for (int c = 0; c < REGS; ++c)
-                if (64 * c < n) f(64 * c + lane, reg[c]);
+                if (at + 64 * c < n) f(at + 64 * c + lane, reg[c]);
         } else {
             for (int i = 0; i < n; i += 64) f(i + lane, i + lane < n ? key(i + lane) : 0u);
         }
@@ -155,6 +171,19 @@ __device__ __forceinline__ int wave_choose(int n, int want, int lane, K key, P p
         hi = max(hi, in ? k : 0u);
         lo = min(lo, in ? k : 0xFFFFFFFFu);
     });
+    hi = wave_largest(hi);
+    lo = ~wave_largest(~lo);
+    if constexpr (TEAM > 0) {
+        __syncthreads();       // (the keys are here; the room is free)
+        if (lane < 4) room->first[lane][wave] = lane == 0 ? (uint32_t)all : (lane == 1 ? (uint32_t)forced : (lane == 2 ? hi : lo));
+        if (wave == 0 && lane < 24) (&room->cnt[0][0])[lane] = 0;
+        __syncthreads();
+        const int w = lane & (NT - 1);
+        all = wave_sum(lane < NT ? (int)room->first[0][w] : 0);
+        forced = wave_sum(lane < NT ? (int)room->first[1][w] : 0);
+        hi = wave_largest(room->first[2][w]);
+        lo = ~wave_largest(~room->first[3][w]);
+    }
     uint32_t t = 1;            // chosen: keys above t, and `eq` of those that are t
     int eq = 0x7fffffff;
     if (all > want) {
@@ -162,23 +191,71 @@ __device__ __forceinline__ int wave_choose(int n, int want, int lane, K key, P p
             t = kForced;
             eq = want;
         } else {
-            // (unsigned maximum and minimum over the lanes, as signed ones)
-            hi = (uint32_t)wave_max((int)(hi ^ 0x80000000u)) ^ 0x80000000u;
-            lo = ~((uint32_t)wave_max((int)(~lo ^ 0x80000000u)) ^ 0x80000000u);
             const uint32_t diff = hi ^ lo;
             int bit = diff ? 31 - __builtin_clz(diff) : -1;
             t = bit >= 31 ? 0u : hi >> (bit + 1) << (bit + 1);
-            for (; bit >= 0; --bit) {
-                const uint32_t c = t | 1u << bit;
-                const int m = count(c);
-                if (m >= want) t = c;
-                if (m == want) break;
+            bool exact = false;
+            if constexpr (TEAM > 0) {
+                // m: keys from t on
+                int m = all, turn = 0;
+                for (; bit >= 0 && !exact; bit -= 3, turn = turn == 2 ? 0 : turn + 1) {
+                    const int sh = max(bit - 2, 0);
+                    uint32_t mine = 0;
+#pragma unroll
+                    for (int j = 0; j < 7; ++j) {
+                        const uint32_t c = (uint32_t)count(t + ((uint32_t)(j + 1) << sh));
+                        mine = lane == j ? c : mine;
+                    }
+                    if (lane < 7) atomicAdd(&room->cnt[turn][lane], mine);
+                    __syncthreads();
+                    const int c = lane < 7 ? (int)room->cnt[turn][lane] : 0;
+                    // (the counts fall from threshold to threshold; those past the remaining bits
+                    // count first and last blocks only)
+                    const int best = __popcll(__ballot(lane < 7 && c >= want));
+                    if (best > 0) {
+                        t += (uint32_t)best << sh;
+                        m = __builtin_amdgcn_readlane(c, best > 0 ? best - 1 : 0);
+                    }
+                    exact = m == want;
+                    // (read before the last barrier but one, written after the next)
+                    if (wave == 0 && lane < 8) room->cnt[turn == 0 ? 2 : turn - 1][lane] = 0;
+                }
+            } else {
+                for (; bit >= 0 && !exact; --bit) {
+                    const uint32_t c = t | 1u << bit;
+                    const int m = count(c);
+                    if (m >= want) t = c;
+                    exact = m == want;
+                }
             }
-            if (bit < 0) eq = want - (t == 0xFFFFFFFFu ? 0 : count(t + 1));
+            if (!exact) {
+                eq = want - count(t + 1);              // (t is below kForced)
+                if constexpr (TEAM > 0) {
+                    __syncthreads();
+                    if (lane == 0) room->over[wave] = (uint32_t)(want - eq);
+                    __syncthreads();
+                    eq = want - wave_sum(lane < NT ? (int)room->over[lane & (NT - 1)] : 0);
+                }
+            }
         }
     }
-    int done = 0, eqs = 0;
     const uint64_t below = lane ? ~0ull >> (64 - lane) : 0ull;
+    int eqs = 0, done = 0;
+    if constexpr (TEAM > 0) {
+        // what the wavefronts before this one take
+        int same = 0, over = 0;
+        each([&](int, uint32_t k) {
+            same += __popcll(__ballot(k == t && k != 0));
+            over += __popcll(__ballot(k > t));
+        });
+        __syncthreads();
+        if (lane == 0) { room->over[wave] = (uint32_t)over; room->same[wave] = (uint32_t)same; }
+        __syncthreads();
+        const int w = lane & (NT - 1);
+        const int o = lane < wave ? (int)room->over[w] : 0, e = lane < wave ? (int)room->same[w] : 0;
+        eqs = wave_sum(e);
+        done = wave_sum(o) + min(eqs, eq);
+    }
     each([&](int i, uint32_t k) {
         const uint64_t same = __ballot(k == t && k != 0);
         const bool take = k != 0 && (k > t || (k == t && eqs + __popcll(same & below) < eq));
@@ -187,19 +264,31 @@ __device__ __forceinline__ int wave_choose(int n, int want, int lane, K key, P p
         eqs += __popcll(same);
         done += __popcll(b);
     });
-    return done;
+    return min(all, want);
 }
 template <class K, class P>
-__device__ __forceinline__ int wave_choose_any(int n, int want, int lane, K key, P put) {
-    if (n <= 256) return wave_choose<4>(n, want, lane, key, put);
-    if (n <= 1024) return wave_choose<16>(n, want, lane, key, put);
-    return wave_choose<0>(n, want, lane, key, put);
+__device__ __forceinline__ int wave_choose(int n, int want, int lane, K key, P put) {
+    if (n <= 256) return choose<0, 4>(nullptr, 0, lane, n, want, key, put);
+    if (n <= 512) return choose<0, 8>(nullptr, 0, lane, n, want, key, put);
+    if (n <= 1024) return choose<0, 16>(nullptr, 0, lane, n, want, key, put);
+    return choose<0, 0>(nullptr, 0, lane, n, want, key, put);
 }
 
-template <int D>
-__global__ __launch_bounds__(SL_NT) void paged_select_blocks(SelectArgs sa) {
-    constexpr int KS = 2 * D / 64, QS = D / 64;       // k steps of the product, of a query
+// the largest over the gp columns of a token, in each of them (gp: 1, 2, 4, 8 or 16 neighbouring lanes)
+__device__ __forceinline__ float columns_max(float x, int gp) {
+    auto with = [](float y, auto ctl) { return fmaxf(y, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, y), decltype(ctl)::value, 0xF, 0xF, true))); };
+    if (gp > 1) x = with(x, std::integral_constant<int, 0xB1>{});     // lane ^ 1
+    if (gp > 2) x = with(x, std::integral_constant<int, 0x4E>{});     // lane ^ 2
+    if (gp > 4) x = with(x, std::integral_constant<int, 0x141>{});    // the other 4 of 8
+    if (gp > 8) x = with(x, std::integral_constant<int, 0x140>{});    // the other 8 of 16
+    return x;
+}
+
+template <int D, int NW>
+__global__ __launch_bounds__(64 * NW) void paged_select_blocks(SelectArgs sa) {
+    constexpr int KS = 2 * D / 64, QS = D / 64, U = 2;   // k steps of the product, of a query; steps in flight
     extern __shared__ uint32_t keys[];                // [token][segment]
+    __shared__ ChooseRoom room;
     const PagedSelect& a = sa.a;
     const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int hk = (int)blockIdx.x % a.hkv, rest = (int)blockIdx.x / a.hkv;
@@ -211,15 +300,27 @@ __global__ __launch_bounds__(SL_NT) void paged_select_blocks(SelectArgs sa) {
     const int p0 = u.st.n - u.st.t + i0;              // row of the first token
     auto low_of = [&](int p) -> int { return a.window > 0 ? max(p - a.window + 1, 0) >> lg : 0; };
     const int end = ((p0 + ntok - 1) >> lg) + 1;      // blocks seen by any token (none: 0 or less)
-    const int sb = low_of(p0) + seg * sa.seg, n = min(end - sb, sa.seg);   // this segment's
+    const int sb = low_of(p0) + seg * sa.seg, n = max(min(end - sb, sa.seg), 0);   // this segment's
     const int G = a.hq / a.hkv, gp = 1 << sa.gp_log2;
 
-    // ---- queries in 8 bits: column lane % 16, dims 64 ks + 16 (lane / 16) .. ----------
+    // the lane's block of steps t0, t0 + NW, ..: its page and place (asked for a round ahead)
     const int col = lane & 15, quad = lane >> 4;
+    const int nt = (n + 15) / 16;
+    int page[U], place[U];
+    auto find = [&](int t0) {
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            const int b = max(min(sb + 16 * (t0 + NW * j) + col, end - 1), 0);
+            page[j] = nt > 0 ? paged_page(a.b, u.s, b >> bpp) : -1;
+            place[j] = b & ((1 << bpp) - 1);
+        }
+    };
+    find(wave);
+
+    // ---- queries in 8 bits: column lane % 16, dims 64 ks + 16 (lane / 16) .. ----------
     const int tk = col >> sa.gp_log2, g0 = col & (gp - 1);
     const int passes = (G + gp - 1) >> sa.gp_log2;
     const int p = p0 + tk, low = low_of(p), last = p >> lg;
-    const int nt = (max(n, 0) + 15) / 16;
     for (int pass = 0; pass < passes; ++pass) {
         const int g = g0 + (pass << sa.gp_log2);
         const bool valid = tk < ntok && g < G;
@@ -245,80 +346,113 @@ __global__ __launch_bounds__(SL_NT) void paged_select_blocks(SelectArgs sa) {
         for (int ks = 0; ks < QS; ++ks)
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-                uint32_t up = 0, dn = 0;
+                uint32_t r[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    r[i] = (uint32_t)(int)__builtin_amdgcn_fmed3f(rintf((float)q[2 * ks + (w >> 1)][4 * (w & 1) + i] * f), -127.f, 127.f);
+                const uint32_t lo = __builtin_amdgcn_perm(r[1], r[0], 0x0C0C0400u), hi = __builtin_amdgcn_perm(r[3], r[2], 0x04000C0Cu), x = lo | hi;
+                // bytes of all ones where a number is below 0
+                const uint32_t below = ((x >> 7) & 0x01010101u) * 255u;
+                qb[ks][w] = (int)(x & ~below);
+                qb[QS + ks][w] = (int)(x & below);
+            }
+        for (int t0 = wave; t0 < nt; t0 += U * NW) {
+            intx4 kb[U][KS];
+            float s[U];
+            int there[U];
+#pragma unroll
+            for (int j = 0; j < U; ++j) {
+                there[j] = page[j];
+                const char* const src = a.in.b + max(page[j], 0) * a.in.nb3 + hk * a.in.nb2 + place[j] * a.in.nb1 + 16 * quad;
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) kb[j][ks] = *(const intx4*)(src + 64 * ks);
+                s[j] = *(const float*)(a.in.s + max(page[j], 0) * a.in.s_nb3 + hk * a.in.s_nb2 + 4 * (int64_t)place[j]);
+            }
+            find(t0 + U * NW < nt ? t0 + U * NW : wave);   // (the next pass begins again)
+#pragma unroll
+            for (int j = 0; j < U; ++j) {
+                const int t = t0 + NW * j;
+                if (t >= nt) break;
+                intx4 acc = {0, 0, 0, 0};
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(kb[j][ks], qb[ks], acc, 0, 0, 0);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float x = (float)q[2 * ks + (w >> 1)][4 * (w & 1) + i] * f;
-                    const int r = x == x ? (int)fminf(fmaxf(rintf(x), -127.f), 127.f) : 0;
-                    up |= (uint32_t)(max(r, 0) & 255) << (8 * i);
-                    dn |= (uint32_t)(min(r, 0) & 255) << (8 * i);
+                    // block of the result's row, its scale and page from the lane that read it
+                    const int r = 4 * quad + i, at = 16 * t + r, bl = sb + at;
+                    const float sr = __shfl(s[j], r, 64);
+                    const int pr = __shfl(there[j], r, 64);
+                    const float y = columns_max(valid ? (float)acc[i] * fs : -INFINITY, gp);
+                    if (g0 != 0 || tk >= ntok || at >= n) continue;
+                    uint32_t key = pr < 0 ? 0u : score_key(y * sr);
+                    if (pass > 0) key = max(key, keys[tk * sa.seg + at]);
+                    if (pass + 1 == passes) {
+                        if (bl < low + a.n_sink || bl > last - a.n_recent) key = kForced;
+                        if (bl < low || bl > last) key = 0u;
+                    }
+                    keys[tk * sa.seg + at] = key;
                 }
-                qb[ks][w] = (int)up;
-                qb[QS + ks][w] = (int)dn;
-            }
-        for (int t = wave; t < nt; t += SL_NT / 64) {
-            // the lane's row of the operand: block b
-            const int b = min(sb + 16 * t + col, end - 1);
-            const int page = paged_page(a.b, u.s, b >> bpp), bi = b & ((1 << bpp) - 1);
-            const char* const src = a.in.b + max(page, 0) * a.in.nb3 + hk * a.in.nb2 + bi * a.in.nb1 + 16 * quad;
-            intx4 kb[KS], acc = {0, 0, 0, 0};
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) kb[ks] = *(const intx4*)(src + 64 * ks);
-            const float s = *(const float*)(a.in.s + max(page, 0) * a.in.s_nb3 + hk * a.in.s_nb2 + 4 * (int64_t)bi);
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(kb[ks], qb[ks], acc, 0, 0, 0);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                // block of the result's row, its scale and page from the lane that read it
-                const int r = 4 * quad + i, at = 16 * t + r, bl = sb + at;
-                const float sr = __shfl(s, r, 64);
-                const int pr = __shfl(page, r, 64);
-                float y = valid ? (float)acc[i] * fs : -INFINITY;
-                for (int k = 1; k < gp; k *= 2) y = fmaxf(y, shfl_xor(y, k));
-                if (g0 != 0 || tk >= ntok || at >= n) continue;
-                uint32_t key = pr < 0 ? 0u : score_key(y * sr);
-                if (pass > 0) key = max(key, keys[tk * sa.seg + at]);
-                if (pass + 1 == passes) {
-                    if (bl < low + a.n_sink || bl > last - a.n_recent) key = kForced;
-                    if (bl < low || bl > last) key = 0u;
-                }
-                keys[tk * sa.seg + at] = key;
             }
         }
     }
     __syncthreads();
-    for (int t = wave; t < ntok; t += SL_NT / 64) {
+    const int want = sa.segs == 1 ? a.top : sa.keep;
+    auto lists = [&](int t, auto choice, int lane0, int step) {
         const uint32_t* const key = keys + t * sa.seg;
         const int64_t row = (int64_t)(u.st.q0 + i0 + t) * a.hkv + hk;
         auto get = [&](int i) -> uint32_t { return key[i]; };
         if (sa.segs == 1) {
             int32_t* const out = a.list + row * a.top;
-            const int k = wave_choose_any(max(n, 0), a.top, lane, get, [&](int r, int i) { out[r] = sb + i; });
-            for (int r = k + lane; r < a.top; r += 64) out[r] = -1;
+            const int k = choice(get, [&](int r, int i) { out[r] = sb + i; });
+            for (int r = k + lane0; r < a.top; r += step) out[r] = -1;
         } else {
             uint2* const out = sa.pairs + (row * sa.segs + seg) * sa.keep;
-            const int k = wave_choose_any(max(n, 0), sa.keep, lane, get, [&](int r, int i) { out[r] = uint2{key[i], (uint32_t)(sb + i)}; });
-            for (int r = k + lane; r < sa.keep; r += 64) out[r] = uint2{0u, 0u};
+            const int k = choice(get, [&](int r, int i) { out[r] = uint2{key[i], (uint32_t)(sb + i)}; });
+            for (int r = k + lane0; r < sa.keep; r += step) out[r] = uint2{0u, 0u};
         }
+    };
+    // a wavefront per token, or all of them for one after another
+    if (NW < SL_WAVES || n <= 512 || (ntok >= 4 && n <= 1024)) {
+        for (int t = wave; t < ntok; t += NW) lists(t, [&](auto get, auto put) { return wave_choose(n, want, lane, get, put); }, lane, 64);
+    } else if constexpr (NW == SL_WAVES) {
+        for (int t = 0; t < ntok; ++t)
+            lists(t, [&](auto get, auto put) { return choose<NW, kSelectSeg / (64 * NW)>(&room, wave, lane, n, want, get, put); }, (int)threadIdx.x, 64 * NW);
     }
 }
 
-// Among the segments' best: a wavefront per token and kv head.
-__global__ __launch_bounds__(256) void paged_select_join(SelectArgs sa) {
+// Among the segments' best: a workgroup per token and kv head, of one wavefront (up to 1024 pairs) or 16
+// (up to 16384; beyond, one of them reads the pairs again and again).
+template <int NW>
+__global__ __launch_bounds__(64 * NW) void paged_select_join(SelectArgs sa) {
+    __shared__ ChooseRoom room;
     const PagedSelect& a = sa.a;
-    const int lane = (int)threadIdx.x & 63;
-    const int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    if (row >= (int64_t)a.b.tokens * a.hkv) return;
+    const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int64_t row = blockIdx.x;
     if (paged_token(a.b, (int)(row / a.hkv)).s < 0) return;
-    const uint2* const in = sa.pairs + row * sa.segs * sa.keep;
+    const int n = sa.segs * sa.keep;
+    const uint2* const in = sa.pairs + row * n;
     int32_t* const out = a.list + row * a.top;
-    const int k = wave_choose_any(sa.segs * sa.keep, a.top, lane, [&](int i) -> uint32_t { return in[i].x; },
-                                  [&](int r, int i) { out[r] = (int32_t)in[i].y; });
-    for (int r = k + lane; r < a.top; r += 64) out[r] = -1;
+    auto get = [&](int i) -> uint32_t { return in[i].x; };
+    auto put = [&](int r, int i) { out[r] = (int32_t)in[i].y; };
+    int k;
+    if constexpr (NW == 1) {
+        k = wave_choose(n, a.top, lane, get, put);
+    } else if (n <= 4096) {
+        k = choose<NW, 4>(&room, wave, lane, n, a.top, get, put);
+    } else if (n <= 16384) {
+        k = choose<NW, 16>(&room, wave, lane, n, a.top, get, put);
+    } else {
+        if (wave > 0) return;
+        k = wave_choose(n, a.top, lane, get, put);
+        for (int r = k + lane; r < a.top; r += 64) out[r] = -1;
+        return;
+    }
+    for (int r = k + (int)threadIdx.x; r < a.top; r += 64 * NW) out[r] = -1;
 }
 
 hipError_t launch_paged_select(const PagedSelect& a, hipStream_t st) {
     if (a.b.tokens <= 0 || a.b.n_streams <= 0 || a.b.max_nq <= 0 || a.hq <= 0) return hipSuccess;
+    if (a.d != 128 && a.d != 64) return hipErrorInvalidValue;
     SelectArgs sa;
     sa.a = a;
     const int G = a.hq / a.hkv;
@@ -332,6 +466,22 @@ hipError_t launch_paged_select(const PagedSelect& a, hipStream_t st) {
     const int64_t nb = (rows + (1 << a.in.lg) - 1) >> a.in.lg;
     int64_t most = 16384 / sa.tiles / 16 * 16;          // (64 KiB of keys)
     if (most > kSelectSeg) most = kSelectSeg;
+    const int64_t per = ((int64_t)a.b.max_nq + sa.tiles - 1) / sa.tiles;
+    int64_t tiles = (int64_t)a.b.tokens / sa.tiles + a.b.n_streams;
+    if (tiles > per * a.b.n_streams) tiles = per * a.b.n_streams;
+    if (tiles > a.b.tokens) tiles = a.b.tokens;
+    // Few workgroups with many blocks: segments of 128 and more, for up to a workgroup a CU, and no more
+    // pairs than one wavefront of the join holds. Whole -> cut, a stream, 8 kv heads of 128: 512
+    // blocks 16.1 -> 12.9 us, 2048 32.2 -> 20.9 (segments of 256: 16.1, 19.3), 8192 50 -> 24.9 (with
+    // segments of 256 alone, whose pairs the join read again and again, 115); 8 streams of 512 16.1 -> 13.5.
+    constexpr int64_t kSeg = 128;
+    if (nb >= 4 * kSeg && tiles * a.hkv < 128) {
+        int64_t cuts = 256 / (tiles * a.hkv);
+        if (cuts > 1024 / a.top) cuts = 1024 / a.top;
+        int64_t seg = cuts > 1 ? (nb + cuts - 1) / cuts : nb;
+        if (seg < kSeg) seg = kSeg;
+        if (seg < most) most = seg;
+    }
     sa.segs = (int32_t)((nb + most - 1) / most);
     if (sa.segs < 1) sa.segs = 1;
     sa.seg = (int32_t)(((nb + sa.segs - 1) / sa.segs + 15) / 16 * 16);
@@ -339,19 +489,23 @@ hipError_t launch_paged_select(const PagedSelect& a, hipStream_t st) {
     sa.keep = a.top < sa.seg ? a.top : sa.seg;
     sa.pairs = reinterpret_cast<uint2*>(a.ws);
     if (sa.segs > 1 && (double)a.b.tokens * a.hkv * sa.segs * sa.keep * sizeof(uint2) > (double)a.ws_bytes) return hipErrorOutOfMemory;
-    const int64_t per = ((int64_t)a.b.max_nq + sa.tiles - 1) / sa.tiles;
-    int64_t tiles = (int64_t)a.b.tokens / sa.tiles + a.b.n_streams;
-    if (tiles > per * a.b.n_streams) tiles = per * a.b.n_streams;
-    if (tiles > a.b.tokens) tiles = a.b.tokens;
-    const int64_t grid = tiles * sa.segs * a.hkv, jgrid = ((int64_t)a.b.tokens * a.hkv + 3) / 4;
-    if (grid > kMaxGridX / 2 || jgrid > kMaxGridX) return hipErrorNotSupported;
+    const int64_t grid = tiles * sa.segs * a.hkv, jgrid = (int64_t)a.b.tokens * a.hkv;
+    if (grid > kMaxGridX / 4 || (sa.segs > 1 && jgrid > kMaxGridX / 4)) return hipErrorNotSupported;
     const size_t lds = (size_t)sa.tiles * sa.seg * sizeof(uint32_t);
-    if (a.d == 128) hipLaunchKernelGGL((paged_select_blocks<128>), dim3((unsigned)grid), dim3(SL_NT), lds, st, sa);
-    else if (a.d == 64) hipLaunchKernelGGL((paged_select_blocks<64>), dim3((unsigned)grid), dim3(SL_NT), lds, st, sa);
-    else return hipErrorInvalidValue;
+    // (Each wavefront forms all the columns' queries: with several tokens to choose for, 4 of them, 256
+    // tokens over 256 blocks 23.6 -> 16.7 us; with one token 16, whose loads are all in flight at once, 512
+    // blocks of 32 streams 23.9 -> 18.1.)
+    if (sa.tiles >= 4 && sa.seg <= 512) {
+        if (a.d == 128) hipLaunchKernelGGL((paged_select_blocks<128, 4>), dim3((unsigned)grid), dim3(256), lds, st, sa);
+        else hipLaunchKernelGGL((paged_select_blocks<64, 4>), dim3((unsigned)grid), dim3(256), lds, st, sa);
+    } else {
+        if (a.d == 128) hipLaunchKernelGGL((paged_select_blocks<128, SL_WAVES>), dim3((unsigned)grid), dim3(64 * SL_WAVES), lds, st, sa);
+        else hipLaunchKernelGGL((paged_select_blocks<64, SL_WAVES>), dim3((unsigned)grid), dim3(64 * SL_WAVES), lds, st, sa);
+    }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || sa.segs == 1) return e;
-    hipLaunchKernelGGL(paged_select_join, dim3((unsigned)jgrid), dim3(256), 0, st, sa);
+    if (sa.segs * sa.keep <= 1024) hipLaunchKernelGGL((paged_select_join<1>), dim3((unsigned)jgrid), dim3(64), 0, st, sa);
+    else hipLaunchKernelGGL((paged_select_join<SL_WAVES>), dim3((unsigned)jgrid), dim3(64 * SL_WAVES), 0, st, sa);
     return hipGetLastError();
 }
 
