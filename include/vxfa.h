@@ -429,7 +429,9 @@ int vxfa_paged_evict(vxfa_ctx* ctx, vxfa_tensor* k, vxfa_tensor* v,
  * any scales from 2^-64 to 2^64 (others count as the nearer end, NaN as 2^-64). */
 
 /* vxfa_paged_append into pages of 8 bits: arguments, rotation, queries and
- * absent pages as there. Of every 16 rows (of a page) and head that new rows come
+ * absent pages as there, but for the angles: they are formed in 64 bits (a
+ * running product in F32, as there and in ggml, is off by up to 1e-3 at position
+ * 8192, which F16 hides less and less the further a position is). Of every 16 rows (of a page) and head that new rows come
  * into, K's scale and V's become the least 2^e (-64 <= e <= 64) with
  * max |x| <= 127 * 2^e over the new rows, or stay what they are where rows
  * ahead of the new ones have a larger one (which has to be such a power). New rows

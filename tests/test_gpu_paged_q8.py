@@ -144,40 +144,40 @@ def test_append_token_by_token(ctx):
 
 @pytest.mark.parametrize("hd,dims", [(128, 128), (64, 64), (128, 64), (64, 2)])
 def test_append_turned(ctx, hd, dims):
-    """Keys and queries turned as by the append into F16 pages: queries bit for bit, keys to the roundings of both."""
-    import torch
-    from gpu_util import guarded, vxfa
+    """Keys and queries turned, at far positions too, against 64 bits: an element is off by the roundings of cos and
+    sin (1e-6 each) and of three operations in F32, all of |x0| + |x1| of its pair, then by half a step of its type."""
     sizes = [(1, 1), (40, 40), (100, 3), (8000, 17), (30, 0), (64, 16)]
-    c8 = Batch8(sizes, 6, 3, hd, page=32, seed=dims, absent=[(3, 249)], behind=2)
-    c16 = Batch(sizes, 6, 3, hd, page=32, seed=dims, absent=[(3, 249)], behind=2)
+    c = Batch8(sizes, 6, 3, hd, page=32, seed=dims, absent=[(3, 249)], behind=2)
     rng = np.random.default_rng(dims)
-    T = c8.T + 2
+    T = c.T + 2
     k_new, v_new = (rng.standard_normal((T, 3, hd)).astype(np.float32) for _ in "kv")
     q = rng.standard_normal((T, 6, hd)).astype(np.float32)
     pos = np.concatenate([np.arange(n - t, n) for n, t in sizes] + [[5, 6]]).astype(np.int32)
-    d8 = store(ctx, c8, k_new, v_new, rope=(pos, dims), q=q)
-    d16 = Device8(c16)
-    w = 3 * hd
-    new = [guarded(x) for x in (k_new, v_new)]
-    nd = [vxfa.desc(t.data_ptr(), vxfa.F32, (w, T, 1, 1), (4, 4 * w, 4 * w * T, 4 * w * T)) for t in new]
-    pt, qt, qo = guarded(pos), guarded(q), guarded(np.zeros(q.shape, np.float16))
-    ctx.paged_append(*nd, d16.batch, d16.k, d16.v, rope=vxfa.rope(pt.data_ptr(), dims, 1e6),
-                     q=vxfa.desc(qt.data_ptr(), vxfa.F32, *d16.views.decoder_q(T, 6, hd)),
-                     q_out=vxfa.desc(qo.data_ptr(), vxfa.F16, *d16.views.decoder_q(T, 6, hd, 2)), stream=current())
-    finish()
-    assert np.array_equal(d8.q_out.view(np.uint16), qo.cpu().numpy().view(np.uint16).reshape(T, 6, hd))
-    assert (d8.q_out[c8.T:] == 0).all()
-    for name in "kv":
-        ints, scales = d8.ints(name), d8.scale(name)
-        pool = d16.pool(name)
+    pos[:c.T] += 100000 * (np.arange(c.T) % 3 == 0)      # (positions need not be the rows' numbers)
+    d = store(ctx, c, k_new, v_new, rope=(pos, dims), q=q)
+
+    def turned(x):
+        y, err = x.astype(np.float64), np.zeros(x.shape)
+        a = pos[:, None, None] * 1e6 ** (-2.0 / dims * np.arange(dims // 2))[None, None]
+        x0, x1 = y[..., 0:dims:2].copy(), y[..., 1:dims:2].copy()
+        y[..., 0:dims:2], y[..., 1:dims:2] = x0 * np.cos(a) - x1 * np.sin(a), x0 * np.sin(a) + x1 * np.cos(a)
+        err[..., 0:dims:2] = err[..., 1:dims:2] = (np.abs(x0) + np.abs(x1)) * (1e-6 + 3 * 2.0 ** -24)
+        return y, err
+
+    want, err = turned(q)
+    assert (np.abs(d.q_out[:c.T] - want[:c.T]) <= err[:c.T] + HALF * np.abs(want[:c.T]) * 1.001 + 2.0 ** -25).all()
+    assert (d.q_out[c.T:] == 0).all()
+    k_want, k_err = turned(k_new)
+    for name, want, err in (("k", k_want, k_err), ("v", v_new.astype(np.float64), np.zeros(v_new.shape))):
+        ints, scales = d.ints(name), d.scale(name)
         for s, (n, t) in enumerate(sizes):
             for r in range(n - t, n):
-                p = c8.table[s, r // 32]
-                if not 0 <= p < c8.n_pages:
+                p = c.table[s, r // 32]
+                if not 0 <= p < c.n_pages:
                     continue
                 step = scales[p, :, r % 32 // 16].astype(np.float64)[:, None]
-                want = pool[c16.table[s, r // 32], r % 32].astype(np.float64)
-                assert (np.abs(ints[p, r % 32] * step - want) <= 0.5 * step + HALF * np.abs(want) * 1.001 + 2.0 ** -25).all()
+                i = c.q_start[s] + r - (n - t)
+                assert (np.abs(ints[p, r % 32] * step - want[i]) <= 0.5 * step + err[i]).all()
 
 
 # ---- attention over all rows -------------------------------------------------------------

@@ -315,15 +315,14 @@ constexpr uint32_t kMaxGridX = (1u << 24) - 1;   // workgroups of 256 threads al
 // x0' = x0 cos - x1 sin, x1' = x0 sin + x1 cos; dims at or past n_dims are
 // left as they are.
 //
-// (cos, sin) of a float angle: reduced by the nearest multiple q of pi / 2 in
+// (cos, sin) of an angle (mostly a float one): reduced by the nearest multiple q of pi / 2 in
 // double precision (error ~1e-12 at the angles rotary embeddings reach), sin
 // and cos of the remainder r (|r| <= pi / 4) by their Taylor series through
 // r^11 and r^12 (truncation below 1e-11, float rounding a few ulp), then the
 // quadrant q mod 4 swaps and negates them. Straight-line code: the library's
 // sincosf carries a large-argument path whose code, repeated for every pair a
 // lane rotates, cost more than the arithmetic.
-__host__ __device__ __forceinline__ float2 rope_cs_of_angle(float th) {
-    const double td = (double)th;
+__host__ __device__ __forceinline__ float2 rope_cs_of_angle(double td) {
     const double qd = __builtin_rint(td * 0.63661977236758134);   // 2 / pi
     const float r = (float)__builtin_fma(-qd, 1.5707963267948966, td);
     const int q = (int)(long long)qd & 3;

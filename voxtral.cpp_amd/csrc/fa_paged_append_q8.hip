@@ -11,7 +11,9 @@
 // stores 4 bytes a lane. So each element is read once, and rows of one block are in one
 // wavefront, whatever order they came in. Queries, which have no scales, have workgroups of
 // their own, a wavefront per token. The angles' cos / sin are formed once for
-// all heads.
+// all heads. Bound by HBM: 8192 tokens of 32 + 8 + 8 heads of 128 53 us, 5.4 TB/s read and
+// written (four wavefronts a SIMD: 55.8 -> 53.1; eight of a token's query loads in flight: 61 -> 55.8); 32
+// tokens 5.4 us in a graph.
 #include "fa_paged_q8.h"
 
 namespace vxfa {
@@ -28,8 +30,20 @@ __device__ __forceinline__ uint32_t bytes_of(floatx4 x, float f) {
     return byte_of(x[0] * f) | byte_of(x[1] * f) << 8 | byte_of(x[2] * f) << 16 | byte_of(x[3] * f) << 24;
 }
 
+// cos / sin of pair j < 64 at position p, the angle p ts^j in 64 bits: as a running product in F32
+// (which f16 values hide) it is off by up to 1e-3 at position 8192, and as many whole numbers by one.
+__device__ __forceinline__ float2 rope_cs_far(int p, int j, double ts) {
+    double th = (double)p;
+#pragma unroll
+    for (int b = 0; b < 6; ++b) {
+        th *= (j >> b) & 1 ? ts : 1.0;
+        ts *= ts;
+    }
+    return rope_cs_of_angle(th);
+}
+
 template <int D>
-__global__ __launch_bounds__(256) void paged_append_q8_kernel(PagedAppend8 p, int units) {
+__global__ __launch_bounds__(256, 4) void paged_append_q8_kernel(PagedAppend8 p, int units) {
     constexpr int PER = D / 4, RPI = 64 / PER, NI = kScaleRows / RPI;   // lanes of a row, rows of a load, loads
     const PagedAppend& a = p.a;
     __shared__ float2 cs[kScaleRows][D / 2];
@@ -40,18 +54,30 @@ __global__ __launch_bounds__(256) void paged_append_q8_kernel(PagedAppend8 p, in
         if (t >= a.b.tokens) return;
         const PagedUnit u = paged_token(a.b, t);
         if (u.s < 0) return;
-        if (lane < D / 2) cs[wave][lane] = rope_cs_chain<D / 2>(a.rope_pos[t], lane, a.rope_ts);
+        if (lane < D / 2) cs[wave][lane] = rope_cs_far(a.rope_pos[t], lane, p.rope_ts);
         __builtin_amdgcn_wave_barrier();   // (a wavefront's LDS accesses run in order)
-        for (int c = lane; c < a.hq * (D / 8); c += 64) {
-            const int h = c / (D / 8), d = 8 * (c % (D / 8));
-            const char* src = (const char*)a.q + (int64_t)t * a.q_nb1 + (int64_t)h * a.q_nb2 + 4 * d;
-            const floatx4 x0 = __builtin_nontemporal_load((const floatx4*)src), x1 = __builtin_nontemporal_load((const floatx4*)src + 1);
-            float x[8] = {x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]};
-            rope8_tab(x, d, cs[wave], a.rope_dims);
-            half8 y;
+        constexpr int U = 4;                           // 16-byte pairs in flight
+        const int n = a.hq * (D / 8);
+        for (int c0 = lane; c0 < n; c0 += 64 * U) {
+            floatx4 x0[U], x1[U];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) y[j] = (_Float16)x[j];
-            *(half8*)((char*)a.q_out + (int64_t)t * a.qo_nb1 + (int64_t)h * a.qo_nb2 + 2 * d) = y;
+            for (int j = 0; j < U; ++j) {
+                const int c = min(c0 + 64 * j, n - 1), h = c / (D / 8), d = 8 * (c % (D / 8));
+                const char* src = (const char*)a.q + (int64_t)t * a.q_nb1 + (int64_t)h * a.q_nb2 + 4 * d;
+                x0[j] = __builtin_nontemporal_load((const floatx4*)src);
+                x1[j] = __builtin_nontemporal_load((const floatx4*)src + 1);
+            }
+#pragma unroll
+            for (int j = 0; j < U; ++j) {
+                const int c = c0 + 64 * j, h = c / (D / 8), d = 8 * (c % (D / 8));
+                if (c >= n) continue;
+                float x[8] = {x0[j][0], x0[j][1], x0[j][2], x0[j][3], x1[j][0], x1[j][1], x1[j][2], x1[j][3]};
+                rope8_tab(x, d, cs[wave], a.rope_dims);
+                half8 y;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) y[i] = (_Float16)x[i];
+                *(half8*)((char*)a.q_out + (int64_t)t * a.qo_nb1 + (int64_t)h * a.qo_nb2 + 2 * d) = y;
+            }
         }
         return;
     }
@@ -69,7 +95,7 @@ __global__ __launch_bounds__(256) void paged_append_q8_kernel(PagedAppend8 p, in
     if (turn) {
         for (int i = tid; i < kScaleRows * 64; i += 256) {
             const int r = i >> 6, j = i & 63;
-            if (j < D / 2 && r >= r0 && r < r1) cs[r][j] = rope_cs_chain<D / 2>(a.rope_pos[tok0 + r], j, a.rope_ts);
+            if (j < D / 2 && r >= r0 && r < r1) cs[r][j] = rope_cs_far(a.rope_pos[tok0 + r], j, p.rope_ts);
         }
         __syncthreads();
     }

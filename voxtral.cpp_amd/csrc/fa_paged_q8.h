@@ -21,6 +21,7 @@ struct PagedScales {
 struct PagedAppend8 {
     PagedAppend a;
     PagedScales sc;
+    double rope_ts;                                   // a.rope_ts in 64 bits
 };
 
 // Bounds of blocks: rows [block of the page] of 2 D bytes at b + page nb3 + head nb2 +

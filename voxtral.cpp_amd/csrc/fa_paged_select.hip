@@ -8,7 +8,8 @@
 // no order of sums. The choice is bound by the chain of its loads (sizes, pages, bounds), each of
 // about a microsecond, and the search: one stream of 128 blocks 8.7 us in a graph, of 512 12.9, 32 uneven ones of up
 // to 512 18 (19 MB of bounds: 4 us at what a large copy reaches), of up to 2048 41 (76 MB). Bounds of
-// a token's blocks 6.2 us, of 8192 tokens' keys of 16 bits in blocks of 32 4.9.
+// a token's block 4.3 us, of 8192 tokens' keys of 16 bits in blocks of 32 4.6 (17 MB: 3.4).
+#include "fa_paged_join.h"
 #include "fa_paged_q8.h"
 
 namespace vxfa {
@@ -16,11 +17,13 @@ namespace vxfa {
 typedef int intx4 __attribute__((ext_vector_type(4)));
 
 // ---- bounds ------------------------------------------------------------------------
-// A wavefront per block and kv head: rows of 16-byte chunks, a lane's dims' extremes in
-// registers, joined over the lanes that have the same dims.
-template <int D, bool I8>
+// A wavefront per block and kv head. A lane has 4 dims of every second (D 64: fourth) row, their
+// extremes in registers (of the smallest, the negative's largest), which one lane swap (two) joins:
+// with 16 dims a lane the joining took most of the time (8192 tokens in blocks of 16 rows of 8 bits
+// 9.7 us, not 5.1). ROWS: of a round, whose loads are in flight together.
+template <int D, bool I8, int ROWS>
 __global__ __launch_bounds__(256) void paged_bounds_kernel(PagedBounds a) {
-    constexpr int DPL = I8 ? 16 : 8, CH = D / DPL, RPI = 64 / CH;   // dims of a lane, lanes of a row, rows of a load
+    constexpr int CH = D / 4, RPI = 64 / CH, U = ROWS / RPI;   // lanes of a row, rows of a load, loads of a round
     const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int nh = (a.hkv + 3) / 4, lg = a.out.lg;
     const int h = (int)blockIdx.x % nh * 4 + wave;
@@ -30,71 +33,73 @@ __global__ __launch_bounds__(256) void paged_bounds_kernel(PagedBounds a) {
     const int page = paged_page(a.b, u.s, row0 >> a.b.ps_log2);
     if (page < 0) return;
     const int at = row0 & ((1 << a.b.ps_log2) - 1);
-    const char* const src = a.kv.k + a.kv.at(page, h, at) + 16 * (lane % CH);
-    float hi[DPL], lo[DPL];
+    const char* const src = a.kv.k + a.kv.at(page, h, at) + (I8 ? 4 : 8) * (lane % CH);
+    float hi[4], lo[4];
 #pragma unroll
-    for (int i = 0; i < DPL; ++i) { hi[i] = -INFINITY; lo[i] = INFINITY; }
-    constexpr int U = 4;
-    for (int r0 = 0; r0 < rows; r0 += U * RPI) {
-        u32x4 w[U];
-        float s[U];
+    for (int i = 0; i < 4; ++i) hi[i] = lo[i] = -INFINITY;
+    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+    for (int r0 = 0; r0 < rows; r0 += ROWS) {
+        u32x2 w[U];
+        float s[ROWS / 16];
 #pragma unroll
         for (int j = 0; j < U; ++j) {
             // (rows past the last read that one again)
-            const int rb = min(r0 + RPI * j, rows - 1), r = min(r0 + RPI * j + lane / CH, rows - 1);
-            w[j] = *(const u32x4*)(src + (int64_t)r * a.kv.nb1);
-            s[j] = 1.f;
-            if constexpr (I8) s[j] = scale_in_range(*(const float*)(a.sc.k + a.sc.at(page, h, at + rb)));   // (16 rows hold the load's)
+            const char* const from = src + (int64_t)min(r0 + RPI * j + lane / CH, rows - 1) * a.kv.nb1;
+            if constexpr (I8) w[j][0] = *(const uint32_t*)from;
+            else w[j] = *(const u32x2*)from;
+        }
+        if constexpr (I8) {
+#pragma unroll
+            for (int j = 0; j < ROWS / 16; ++j) s[j] = scale_in_range(*(const float*)(a.sc.k + a.sc.at(page, h, at + min(r0 + 16 * j, rows - 1))));
         }
 #pragma unroll
         for (int j = 0; j < U; ++j)
 #pragma unroll
-            for (int i = 0; i < DPL; ++i) {
+            for (int i = 0; i < 4; ++i) {
                 float x;
-                if constexpr (I8) x = (float)((int)(w[j][i >> 2] << (24 - 8 * (i & 3))) >> 24) * s[j];
-                else x = (float)__builtin_bit_cast(half8, w[j])[i];
+                // (16 rows hold a load's; those past the last are of the scale of the last one's 16)
+                if constexpr (I8) x = (float)((int)(w[j][0] << (24 - 8 * i)) >> 24) * s[RPI * j / 16];
+                else x = (float)__builtin_bit_cast(half4, w[j])[i];
                 hi[i] = fmaxf(hi[i], x);
-                lo[i] = fminf(lo[i], x);
+                lo[i] = fmaxf(lo[i], -x);
             }
     }
     float m = 0.f;
 #pragma unroll
-    for (int i = 0; i < DPL; ++i) {
-#pragma unroll
-        for (int k = CH; k < 64; k *= 2) {
-            hi[i] = fmaxf(hi[i], shfl_xor(hi[i], k));
-            lo[i] = fminf(lo[i], shfl_xor(lo[i], k));
-        }
+    for (int i = 0; i < 4; ++i) {
+        hi[i] = CH == 32 ? pair32_max(hi[i]) : quad_max(hi[i]);
+        lo[i] = -(CH == 32 ? pair32_max(lo[i]) : quad_max(lo[i]));
         m = fmaxf(m, fmaxf(fabsf(hi[i]), fabsf(lo[i])));
     }
     const int e = exp_for(__builtin_bit_cast(float, wave_max(__builtin_bit_cast(int, m))));
     const float f = two_to(-e);
-    uint32_t bh[DPL / 4], bl[DPL / 4];
+    uint32_t bh = 0, bl = 0;
 #pragma unroll
-    for (int i = 0; i < DPL; ++i) {
-        const uint32_t x = (uint32_t)(int)fminf(fmaxf(ceilf(hi[i] * f), -127.f), 127.f) & 255u;
-        const uint32_t y = (uint32_t)(int)fminf(fmaxf(floorf(lo[i] * f), -127.f), 127.f) & 255u;
-        bh[i / 4] = (i & 3) ? bh[i / 4] | x << (8 * (i & 3)) : x;
-        bl[i / 4] = (i & 3) ? bl[i / 4] | y << (8 * (i & 3)) : y;
+    for (int i = 0; i < 4; ++i) {
+        bh |= ((uint32_t)(int)fminf(fmaxf(ceilf(hi[i] * f), -127.f), 127.f) & 255u) << (8 * i);
+        bl |= ((uint32_t)(int)fminf(fmaxf(floorf(lo[i] * f), -127.f), 127.f) & 255u) << (8 * i);
     }
     const int bi = at >> lg;
-    if (lane < CH) {
-        uint32_t* const dh = (uint32_t*)(a.out.b + page * a.out.nb3 + h * a.out.nb2 + bi * a.out.nb1 + DPL * lane);
-#pragma unroll
-        for (int i = 0; i < DPL / 4; ++i) { dh[i] = bh[i]; dh[D / 4 + i] = bl[i]; }
-    }
+    uint32_t* const dst = (uint32_t*)(a.out.b + page * a.out.nb3 + h * a.out.nb2 + bi * a.out.nb1);
+    // (the second half of the lanes, or the second row of them, has the same: it stores the lower ones)
+    if (lane < 2 * CH) dst[lane] = lane < CH ? bh : bl;
     if (lane == 0) *(float*)(a.out.s + page * a.out.s_nb3 + h * a.out.s_nb2 + 4 * (int64_t)bi) = two_to(e);
+}
+
+template <int D, bool I8>
+static void launch_bounds(const PagedBounds& a, unsigned grid, hipStream_t st) {
+    if (a.out.lg >= 6) hipLaunchKernelGGL((paged_bounds_kernel<D, I8, 64>), dim3(grid), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((paged_bounds_kernel<D, I8, 16>), dim3(grid), dim3(256), 0, st, a);
 }
 
 hipError_t launch_paged_bounds(const PagedBounds& a, hipStream_t st) {
     if (a.b.tokens <= 0 || a.b.n_streams <= 0 || a.b.max_nkv <= 0) return hipSuccess;
     const int64_t grid = blocks_bound(a.b, a.out.lg) * ((a.hkv + 3) / 4);
     if (grid > kMaxGridX) return hipErrorNotSupported;
-    const dim3 g((unsigned)grid), b(256);
-    if (a.d == 128 && a.sc.k) hipLaunchKernelGGL((paged_bounds_kernel<128, true>), g, b, 0, st, a);
-    else if (a.d == 128) hipLaunchKernelGGL((paged_bounds_kernel<128, false>), g, b, 0, st, a);
-    else if (a.d == 64 && a.sc.k) hipLaunchKernelGGL((paged_bounds_kernel<64, true>), g, b, 0, st, a);
-    else if (a.d == 64) hipLaunchKernelGGL((paged_bounds_kernel<64, false>), g, b, 0, st, a);
+    if (a.d == 128 && a.sc.k) launch_bounds<128, true>(a, (unsigned)grid, st);
+    else if (a.d == 128) launch_bounds<128, false>(a, (unsigned)grid, st);
+    else if (a.d == 64 && a.sc.k) launch_bounds<64, true>(a, (unsigned)grid, st);
+    else if (a.d == 64) launch_bounds<64, false>(a, (unsigned)grid, st);
     else return hipErrorInvalidValue;
     return hipGetLastError();
 }

@@ -100,6 +100,7 @@ int vxfa_paged_append_q8(vxfa_ctx* c, const vxfa_tensor* k_new, const vxfa_tenso
     int rc = check_pool8(k, k_scale, v, v_scale, batch, a.sc, &why);
     if (rc != VXFA_OK) return fail(c, rc, "%s", why);
     if ((rc = append_of(c, k_new, v_new, batch, k, v, rope, q, q_out, a.a)) != VXFA_OK) return rc;
+    a.rope_ts = rope ? pow((double)rope->freq_base, -2.0 / (double)rope->n_dims) : 1.0;
     OnDevice on(c->device);
     if (on.e != hipSuccess) return fail(c, VXFA_HIP_ERROR, "hipSetDevice: %s", hipGetErrorString(on.e));
     return launched(c, vxfa::launch_paged_append_q8(a, reinterpret_cast<hipStream_t>(stream)), "paged append");
