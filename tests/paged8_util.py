@@ -55,7 +55,8 @@ class Batch8(paged_util.Batch):
         there = (p >= 0) & (p < self.n_pages)
         p = np.where(there, p, 0)
         scale = (self.ks if pool is self.k else self.vs)[p, h, r % self.page // 16].astype(np.float64)
-        x = pool[p, r % self.page, h] * scale[:, None]
+        with np.errstate(invalid="ignore"):     # (rows of absent pages; a line below)
+            x = pool[p, r % self.page, h] * scale[:, None]
         return np.where(there[:, None], x, 0.0), there
 
 

@@ -462,6 +462,145 @@ def test_blocks_are_all_rows(ctx):
     attend_blocks(ctx, c, 16, 32, lists=lists)
 
 
+@pytest.mark.parametrize("kind", [Batch, Batch8])
+def test_blocks_lists_longer_than_the_lanes(ctx, kind):
+    """Whole lists of more than 32 steps a wavefront, whose pages are read 32 steps at a time."""
+    attend_blocks(ctx, kind([(6000, 70)], 8, 8, 64, 16, seed=12), 16, 300)
+
+
+def test_whole_streams_longer_than_the_lanes(ctx):
+    """Streams that the workspace's records leave whole (1024 query heads), of more than 32 steps a wavefront."""
+    attend(ctx, Batch8([(5000, 1)] + [(3, 1)] * 59, 1024, 64, 64, 16, seed=13))
+
+
+def test_many_rows_of_neighbouring_heads(ctx):
+    """The bounds' rows where a workgroup takes four heads, with short streams and long ones, absent pages, a window."""
+    sizes = [(n, 1) for n in (1, 17, 200, 5000, 9000, 33, 64, 1000, 2, 3000, 700, 40)]
+    attend(ctx, Batch8(sizes, 8, 8, 64, 16, seed=14, absent=[(3, 0), (4, 100), (4, 562)]))
+    attend(ctx, Batch8(sizes, 32, 8, 128, 32, seed=15), window=2500, cap=20.0, bias=4.0)
+
+
+# ---- memory and streams ----------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("kind", [Batch, Batch8])
+@pytest.mark.parametrize("hd", [128, 64])
+def test_pages_past_4_gib(ctx, kind, hd):
+    """Pages 2 GiB and more apart: offsets within the pool pass 32 bits."""
+    import torch
+    from gpu_util import guarded, vxfa
+    c = kind([(60, 1), (100, 40)], 4, 2, hd, 64, seed=hd)
+    d = Device8(c, block=16)
+    far = (2 ** 31 + 4096)
+    e = 1 if kind is Batch8 else 2
+    page = 64 * 2 * hd * e
+    for name in "kv":
+        big = torch.empty(far * (c.n_pages - 1) + page, dtype=torch.uint8, device="cuda")
+        small = d.pools[name][0].view(c.n_pages, page)
+        for i in range(c.n_pages):
+            big[far * i:far * i + page] = small[i]
+        d.pools[name] = (big, vxfa.desc(big.data_ptr(), vxfa.I8 if e == 1 else vxfa.F16, (hd, 64, 2, c.n_pages), (e, 2 * hd * e, hd * e, far)))
+    d.k, d.v = d.pools["k"][1], d.pools["v"][1]
+    if e == 1:
+        ctx.flash_attn_ext_paged_q8(d.q, d.k, d.ks, d.v, d.vs, d.batch, d.dst, 0.1, stream=current())
+        finish()
+        want, err = p8.reference(c, 0.1)
+        check_out(d.out(), want, err, True)
+        d.dt.fill_(0xA5)
+    ctx.paged_bounds(d.k, d.ks, d.batch, d.b, d.bs, stream=current())
+    finish()
+    b, bs = p8.bounds(c, 16, d.b_np, d.bs_np)
+    assert np.array_equal(d.bounds()[0], b) and np.array_equal(d.bounds()[1], bs)
+    lists = some_blocks(c, 16, 5, np.random.default_rng(1))
+    d.set_list(lists, 16)
+    ctx.flash_attn_ext_paged_blocks(d.q, d.k, d.ks, d.v, d.vs, d.batch, d.blocks, d.dst, 0.1, stream=current())
+    finish()
+    want, err = p8.reference(c, 0.1, lists=lists)
+    check_out(d.out(), want, err, True)
+    if e == 1:
+        rng = np.random.default_rng(2)
+        new = [rng.standard_normal((c.T, 2, hd)).astype(np.float32) for _ in "kv"]
+        t = [guarded(x) for x in new]
+        w = 2 * hd
+        nd = [vxfa.desc(x.data_ptr(), vxfa.F32, (w, c.T, 1, 1), (4, 4 * w, 4 * w * c.T, 4 * w * c.T)) for x in t]
+        ctx.paged_append_q8(*nd, d.batch, d.k, d.ks, d.v, d.vs, stream=current())
+        finish()
+        for name, x in zip("kv", new):
+            ints, scales = p8.append(c, getattr(c, name), getattr(c, name + "s"), x)
+            got = np.stack([d.pools[name][0][far * i:far * i + page].cpu().numpy().view(np.int8) for i in range(c.n_pages)])
+            assert np.array_equal(got.reshape(ints.shape), ints) and np.array_equal(d.scale(name), scales, equal_nan=True)
+
+
+@pytest.mark.parametrize("kind", [Batch, Batch8])
+def test_a_pool_without_pages(ctx, kind):
+    """Zeros, and no choice; nothing of the pool is read."""
+    import torch
+    c = kind([(60, 1), (100, 40)], 4, 2, 64, 64, seed=1)
+    d = Device8(c, block=32)
+    lists = some_blocks(c, 32, 3, np.random.default_rng(1))
+    d.set_list(lists, 32)
+    for t in (d.k, d.v, d.ks, d.vs, d.b, d.bs):
+        if t is not None:
+            t.ne[2 if t.type == d.vxfa.F32 else 3] = 0
+            t.data = None
+    ctx.flash_attn_ext_paged_blocks(d.q, d.k, d.ks, d.v, d.vs, d.batch, d.blocks, d.dst, 0.1, stream=current())
+    finish()
+    assert (d.out() == 0).all()
+    if kind is Batch8:
+        ctx.flash_attn_ext_paged_q8(d.q, d.k, d.ks, d.v, d.vs, d.batch, d.dst, 0.1, stream=current())
+        finish()
+        assert (d.out() == 0).all()
+    ctx.paged_bounds(d.k, d.ks, d.batch, d.b, d.bs, stream=current())
+    ctx.paged_select(d.q, d.b, d.bs, d.batch, d.blocks, stream=current())
+    finish()
+    assert (d.list() == -1).all()
+
+
+def test_two_contexts_at_once(ctx):
+    """Two streams, a context each, one in a graph and one eager, several times: each as alone."""
+    import torch
+    from gpu_util import vxfa
+    cs = [Batch8([(3000, 1), (700, 1), (90, 1)], 8, 2, 128, 32, seed=s) for s in (1, 2)]
+    ds = [Device8(c, block=32) for c in cs]
+    streams, ctxs = [torch.cuda.Stream() for _ in cs], [vxfa.Context(0) for _ in cs]
+    for d, c in zip(ds, cs):
+        d.set_list(np.zeros((3, 2, 9), np.int32), 32, 1, 2)
+
+    def step(i, st):
+        d = ds[i]
+        ctxs[i].paged_bounds(d.k, d.ks, d.batch, d.b, d.bs, stream=st)
+        ctxs[i].paged_select(d.q, d.b, d.bs, d.batch, d.blocks, stream=st)
+        ctxs[i].flash_attn_ext_paged_blocks(d.q, d.k, d.ks, d.v, d.vs, d.batch, d.blocks, d.dst, 0.1, stream=st)
+
+    try:
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=streams[0]):
+            step(0, streams[0].cuda_stream)
+        want = []
+        for i in range(2):
+            step(i, current())
+            finish()
+            want.append((ds[i].out(), ds[i].list().copy()))
+            full, err = p8.reference(cs[i], 0.1, lists=want[i][1], block=32)
+            check_out(want[i][0], full, err, True)
+        for _ in range(20):
+            for d in ds:
+                d.dt.fill_(0xA5)
+                d.lt.zero_()
+            torch.cuda.synchronize()
+            with torch.cuda.stream(streams[0]):
+                graph.replay()
+            for _ in range(3):
+                step(1, streams[1].cuda_stream)
+            torch.cuda.synchronize()
+            for d, w in zip(ds, want):
+                assert np.array_equal(d.out(), w[0]) and np.array_equal(d.list(), w[1])
+    finally:
+        for x in ctxs:
+            x.close()
+
+
 # ---- together -------------------------------------------------------------------------------
 
 

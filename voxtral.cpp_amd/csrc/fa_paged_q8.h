@@ -123,7 +123,8 @@ __device__ __forceinline__ PagedUnit paged_unit(const PagedBatch& b, int item, F
     for (int s0 = 0; s0 < b.n_streams; s0 += 64) {
         PagedStream s{0, 0, 0};
         if (s0 + lane < b.n_streams) s = paged_stream(b, s0 + lane);
-        const int n = s.t > 0 ? count(s) : 0;
+        // (no grid has more: sizes that break the bounds do not overflow the sums)
+        const int n = s.t > 0 ? min(count(s), 1 << 24) : 0;
         const int incl = wave_scan(n);
         const uint64_t hit = __ballot(before + incl > item);
         if (hit) {

@@ -96,6 +96,7 @@ static __global__ __launch_bounds__(64 * NW, I8 ? 4 : (NW == 8 ? 2 : 3)) void pa
         np = wa.parts;
         tb = wa.tiles * piece + min(piece, wa.longer);
         te = tb + wa.tiles + (piece < wa.longer ? 1 : 0);
+        if (a.b.n_pages == 0) te = tb;                // (no page that tiles which are not there could read)
     } else {
         const Part part = rows_locate(a.b, ra.p, a.window, item);
         if (part.s < 0) return;

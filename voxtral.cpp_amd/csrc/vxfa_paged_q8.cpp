@@ -160,8 +160,9 @@ int vxfa_paged_select(vxfa_ctx* c, const vxfa_tensor* q, const vxfa_tensor* boun
     const char* why = "";
     if (!bounds || !bounds_scale || !batch || !blocks) return fail(c, VXFA_INVALID_ARG, "bounds, their scales, batch and blocks are required");
     if (!sane(bounds, true)) return fail(c, VXFA_INVALID_ARG, "bounds: unknown type, negative ne or absurd nb");
-    if (bounds->ne[0] % 2 || blocks->block < 16 || bounds->ne[1] > (1 << 16))
+    if (bounds->ne[0] % 2 || blocks->block < 16 || bounds->ne[1] < 1 || bounds->ne[1] > (1 << 16) || (bounds->ne[1] & (bounds->ne[1] - 1)))
         return fail(c, VXFA_INVALID_ARG, "bounds must be [2 D, page_size / block, Hkv, n_pages], blocks of 16 rows at least");
+    if (blocks->block & (blocks->block - 1)) return fail(c, VXFA_INVALID_ARG, "blocks: a power of two from 16 to the page size");
     // (the pool itself is not looked at: its page size is the blocks of a page times their rows)
     vxfa_tensor k = *bounds;
     k.type = VXFA_TYPE_I8;
