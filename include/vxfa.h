@@ -416,32 +416,37 @@ int vxfa_paged_evict(vxfa_ctx* ctx, vxfa_tensor* k, vxfa_tensor* v,
 
 /* ---- Paged K/V cache of 8 bits ------------------------------------------------
  *
- * The same pool with half the bytes: k, v [D, page_size, Hkv, n_pages] I8, laid
- * out as above (strides of 16-byte multiples, the same ones for k and v), and
- * beside each its scales, F32 [page_size / 16, Hkv, n_pages, 1], elements
+ * The same pool with half the bytes: k, v [D, page_size, Hkv, n_pages] I8,
+ * laid out as above (strides of 16-byte multiples, the same ones for k and v),
+ * and beside each its scales, F32 [page_size / 16, Hkv, n_pages, 1], elements
  * contiguous along ne[0], the same strides for k_scale and v_scale. Row r of a
  * page and head holds the values scale[r / 16] * k[r]. No counterpart in the
  * reference, whose cache is F16 or F32 (src/voxtral.cpp:1126-1136).
  *
- * The scales that vxfa_paged_append_q8 writes are powers of two 2^e, -64 <= e <=
- * 64; the whole numbers go from -127 to 127. So the product with a scale is exact,
- * and the numbers of a block whose scale has to grow are shifted. Attention takes
- * any scales from 2^-64 to 2^64 (others count as the nearer end, NaN as 2^-64). */
+ * The scales that vxfa_paged_append_q8 writes are powers of two 2^e, -64 <= e
+ * <= 64; the whole numbers go from -127 to 127. So the product with a scale is
+ * exact, and the numbers of a block whose scale has to grow are shifted.
+ * Attention takes any scales from 2^-64 to 2^64 (others count as the nearer
+ * end, NaN as 2^-64). Rows under a scale of V that is less than 2^-96 of the
+ * largest one that the token sees may be missing from the sum of its softmax
+ * (rows of zeros have the least scale, 2^-64: so it takes elements of V beyond
+ * 127 * 2^32). */
 
 /* vxfa_paged_append into pages of 8 bits: arguments, rotation, queries and
  * absent pages as there, but for the angles: they are formed in 64 bits (a
- * running product in F32, as there and in ggml, is off by up to 1e-3 at position
- * 8192, which F16 hides less and less the further a position is). Of every 16 rows (of a page) and head that new rows come
- * into, K's scale and V's become the least 2^e (-64 <= e <= 64) with
- * max |x| <= 127 * 2^e over the new rows, or stay what they are where rows
- * ahead of the new ones have a larger one (which has to be such a power). New rows
- * are stored as x / 2^e rounded to nearest even (NaN as 0; beyond 127 as 127); the
- * rows ahead are rounded again, to nearest even, where the scale grows: a value is off by at
- * most half a step of the final scale for its own rounding, and the same again for every
- * time that its block's scale has grown, by a factor of 2 at least, since. Rows of
- * the 16 behind the new ones keep their numbers and are worth nothing
- * until a later append. Streams whose new rows lie in the same 16 rows of a page leave
- * any values there. One launch; asynchronous on `stream`. */
+ * running product in F32, as there and in ggml, is off by up to 1e-3 at
+ * position 8192, which F16 hides less and less the further a position is). Of
+ * every 16 rows (of a page) and head that new rows come into, K's scale and
+ * V's become the least 2^e (-64 <= e <= 64) with max |x| <= 127 * 2^e over the
+ * new rows, or stay what they are where rows ahead of the new ones have a
+ * larger one (which has to be such a power). New rows are stored as x / 2^e
+ * rounded to nearest even (NaN as 0; beyond 127 as 127); the rows ahead are
+ * rounded again, to nearest even, where the scale grows: a value is off by at
+ * most half a step of the final scale for its own rounding, and the same again
+ * for every time that its block's scale has grown, by a factor of 2 at least,
+ * since. Rows of the 16 behind the new ones keep their numbers and are worth
+ * nothing until a later append. Streams whose new rows lie in the same 16 rows
+ * of a page leave any values there. One launch; asynchronous on `stream`. */
 int vxfa_paged_append_q8(vxfa_ctx* ctx, const vxfa_tensor* k_new,
                          const vxfa_tensor* v_new, const vxfa_paged* batch,
                          vxfa_tensor* k, vxfa_tensor* k_scale, vxfa_tensor* v,
@@ -449,10 +454,10 @@ int vxfa_paged_append_q8(vxfa_ctx* ctx, const vxfa_tensor* k_new,
                          const vxfa_tensor* q, vxfa_tensor* q_out,
                          void* stream);
 
-/* vxfa_flash_attn_ext_paged over pages of 8 bits, without accumulated weights. The
- * products are of f16 (in which the whole numbers are exact) and scales
- * are applied to the scores and sums in F32, so nothing is rounded more than there.
- * Rows that a token does not see may hold anything. */
+/* vxfa_flash_attn_ext_paged over pages of 8 bits, without accumulated weights.
+ * The products are of f16 (in which the whole numbers are exact) and scales
+ * are applied to the scores and sums in F32, so nothing is rounded more than
+ * there. Rows that a token does not see may hold anything. */
 int vxfa_flash_attn_ext_paged_q8(vxfa_ctx* ctx, const vxfa_tensor* q,
                                  const vxfa_tensor* k, const vxfa_tensor* k_scale,
                                  const vxfa_tensor* v, const vxfa_tensor* v_scale,
@@ -464,22 +469,26 @@ int vxfa_flash_attn_ext_paged_q8(vxfa_ctx* ctx, const vxfa_tensor* q,
  *
  * A token of a long stream looks at a few blocks of its rows only: those whose
  * keys may have the largest products with its queries. Bounds of every block's
- * keys are kept beside the pool (of F16 or 8 bits) and brought up to date after
- * each append; a call chooses blocks for every new token and kv head by
- * them; a call attends over the chosen ones. A block is 16, 32, .. rows, up to a
- * page: block b of a stream is its rows b * block .. (b + 1) * block - 1.
+ * keys are kept beside the pool (of F16 or 8 bits) and brought up to date
+ * after each append; a call chooses blocks for every new token and kv head by
+ * them; a call attends over the chosen ones. A block is 16, 32, .. rows, up to
+ * a page: block b of a stream is its rows b * block .. (b + 1) * block - 1.
  *
- * Bounds: I8 [2 D, page_size / block, Hkv, n_pages], rows contiguous, strides of
- * 16-byte multiples, and their scales, F32 [page_size / block, Hkv, n_pages, 1],
- * contiguous along ne[0]. Of a block and head with keys k: 2^e the least power (-64 <= e
- * <= 64) with max |k| <= 127 * 2^e; element d < D the largest k_d / 2^e, rounded up,
- * element D + d the smallest, rounded down. (NaN among keys is passed over; what lies beyond
- * 127 * 2^64, as infinities do, counts as that.) */
+ * Bounds: I8 [2 D, page_size / block, Hkv, n_pages], rows contiguous, strides
+ * of 16-byte multiples, and their scales, F32 [page_size / block, Hkv,
+ * n_pages, 1], contiguous along ne[0]. Of a block and head with keys k: 2^e
+ * the least power (-64 <= e <= 64) with max |k| <= 127 * 2^e; element d < D
+ * the largest k_d / 2^e, rounded up, element D + d the smallest, rounded down.
+ * (NaN among keys is passed over; what lies beyond 127 * 2^64, as infinities
+ * do, counts as that.) */
 
 /* Bounds of the blocks that the batch's new tokens lie in, over the streams'
- * rows in them. k_scale: of a pool of 8 bits; NULL for F16. max_nq bounds the new
- * tokens as elsewhere; the window has no effect. Blocks of absent pages are left
- * out. One launch; asynchronous on `stream`. */
+ * rows in them. k_scale: of a pool of 8 bits; NULL for F16. max_nq bounds the
+ * new tokens as elsewhere; the window has no effect. Blocks of absent pages
+ * are left out. The new tokens need not be new: a batch whose chunks are as
+ * long as its streams brings all their bounds up to date, as after
+ * vxfa_paged_evict, which moves rows and not their bounds. One launch;
+ * asynchronous on `stream`. */
 int vxfa_paged_bounds(vxfa_ctx* ctx, const vxfa_tensor* k,
                       const vxfa_tensor* k_scale, const vxfa_paged* batch,
                       vxfa_tensor* bounds, vxfa_tensor* bounds_scale,
@@ -494,38 +503,40 @@ typedef struct vxfa_blocks {
     int32_t n_recent;
 } vxfa_blocks;
 
-/* Choose blocks for the batch's new tokens: blocks->list of token i and kv head h
- * becomes, of the blocks with rows that the token sees (within the window), the
- * first n_sink, the last n_recent, and of the others those of the largest scores
- * (of equal ones the first), `top` in all or as many as there are; ascending,
- * then -1. Blocks in absent pages are no candidates, but count among the first and last.
- * The score of a block is the largest, over the kv head's query heads, of
+/* Choose blocks for the batch's new tokens: blocks->list of token i and kv
+ * head h becomes, of the blocks with rows that the token sees (within the
+ * window), the first n_sink, the last n_recent, and of the others those of the
+ * largest scores (of equal ones the first), `top` in all or as many as there
+ * are; ascending, then -1. Blocks in absent pages are no candidates, but count
+ * among the first and last. The score of a block is the largest, over the kv
+ * head's query heads, of
  *   2^(e + f) sum_d (r_d > 0 ? r_d hi_d : r_d lo_d)
- * with the block's bounds hi, lo at scale 2^e and the head's query (as F16) in 8
- * bits, r_d = q_d / 2^f rounded to nearest even, f as for bounds. It is exact in F32, and the
- * choice the same everywhere. (No cap or slope changes it; a
- * negative scale of the attention turns its meaning around.) q [D, T, Hq, 1] F16 or F32. Tokens
- * of no stream leave the list as it was. bounds_scale: powers of two from 2^-64 to 2^64 (others: the
- * choice may differ from the formula's). At most 262144 blocks of a stream
- * (max_nkv; else VXFA_UNSUPPORTED). Where streams have more than 4096 blocks (with 16 / n
- * tokens of a stream at once for kv heads of n query heads, n rounded up to a power of
- * two, 16384 by that many), and with few tokens from 512 on, the call leaves the best of segments of
- * blocks in the workspace, 8 bytes times top for each token, kv head and segment (else
- * VXFA_NO_WORKSPACE).
- * Asynchronous on `stream`. */
+ * with the block's bounds hi, lo at scale 2^e and the head's query (as F16) in
+ * 8 bits, r_d = q_d / 2^f rounded to nearest even, f as for bounds. It is
+ * exact in F32, and the choice the same everywhere. (No cap or slope changes
+ * it; a negative scale of the attention turns its meaning around.) q [D, T,
+ * Hq, 1] F16 or F32. Tokens of no stream leave the list as it was.
+ * bounds_scale: powers of two from 2^-64 to 2^64 (others: the choice may
+ * differ from the formula's). At most 262144 blocks of a stream (max_nkv; else
+ * VXFA_UNSUPPORTED). Where streams have more than 4096 blocks (with 16 / n
+ * tokens of a stream at once for kv heads of n query heads, n rounded up to a
+ * power of two, 16384 by that many), and with few tokens from 512 on, the call
+ * leaves the best of segments of blocks in the workspace, 8 bytes times top
+ * for each token, kv head and segment (else VXFA_NO_WORKSPACE). Asynchronous
+ * on `stream`. */
 int vxfa_paged_select(vxfa_ctx* ctx, const vxfa_tensor* q,
                       const vxfa_tensor* bounds, const vxfa_tensor* bounds_scale,
                       const vxfa_paged* batch, const vxfa_blocks* blocks,
                       void* stream);
 
-/* vxfa_flash_attn_ext_paged, without accumulated weights, over the rows of chosen
- * blocks only: token i, kv head h over the rows of blocks->list[i][h], as far as the token sees
- * them (j <= p, the window). Numbers of blocks in any order; those
- * below 0, or of rows that the token does not see, count for nothing, one that
- * is listed twice counts twice. n_sink and n_recent are not looked at. The pool is F16 (k_scale and v_scale NULL)
- * or of 8 bits. A token without a row gets zeros. In an F16 pool rows
- * of a token's blocks that it does not see have to be finite, within 16 rows of one that it
- * sees. */
+/* vxfa_flash_attn_ext_paged, without accumulated weights, over the rows of
+ * chosen blocks only: token i, kv head h over the rows of blocks->list[i][h],
+ * as far as the token sees them (j <= p, the window). Numbers of blocks in any
+ * order; those below 0, or of rows that the token does not see, count for
+ * nothing, one that is listed twice counts twice. n_sink and n_recent are not
+ * looked at. The pool is F16 (k_scale and v_scale NULL) or of 8 bits. A token
+ * without a row gets zeros. In an F16 pool rows of a token's blocks that it
+ * does not see have to be finite, within 16 rows of one that it sees. */
 int vxfa_flash_attn_ext_paged_blocks(vxfa_ctx* ctx, const vxfa_tensor* q,
                                      const vxfa_tensor* k, const vxfa_tensor* k_scale,
                                      const vxfa_tensor* v, const vxfa_tensor* v_scale,

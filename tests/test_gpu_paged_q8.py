@@ -237,6 +237,18 @@ def test_chunk_types(ctx, dst, q):
         attend(ctx, Batch8([(50, 50), (200, 50)], hd=64, q_type=q, seed=5), dst=dst, **opt)
 
 
+@pytest.mark.parametrize("sizes", [[(1, 1), (77, 1), (500, 1), (3000, 1)], [(50, 50), (777, 40), (1200, 200)]])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_scales_as_far_apart_as_they_may_be(ctx, hd, sizes):
+    """V's scales from 2^-64 to 2^32. (Exponents of two numbers behind the comma: a weight of F32 reaches 2^-126.)"""
+    c = Batch8(sizes, hd=hd, spread=50, seed=17)
+    ok = (c.vs > 0) & (c.vs < 2.0 ** 60)
+    with np.errstate(invalid="ignore", over="ignore"):
+        e = np.where(ok, np.log2(np.where(ok, c.vs, 1)), 0)
+        c.vs = np.where(ok, 2.0 ** np.rint(-64 + (e + 55) * 96 / 50), c.vs).astype(np.float32)
+    attend(ctx, c, dst="f32")
+
+
 @pytest.mark.parametrize("hd", [64, 128])
 def test_chunk_scales_far_apart(ctx, hd):
     attend(ctx, Batch8([(50, 50), (777, 40), (1200, 200)], hd=hd, spread=50, seed=7), dst="f32")
@@ -310,6 +322,40 @@ def test_bounds(ctx, kind, hkv, hd, page, block, layout):
     assert np.array_equal(gots, wants), np.argwhere(gots != wants)[0]
     assert np.array_equal(got, want), np.argwhere(got != want)[0]
     d.check_guards()
+
+
+@pytest.mark.parametrize("max_nq", [1, 30])
+def test_bounds_of_chunks_longer_than_max_nq(ctx, max_nq):
+    """Tokens past max_nq are left out, and the others stay in the rows that q_start gives them, in however many
+    streams; the host knows no count of all tokens."""
+    from gpu_util import vxfa
+    c = Batch8([(100, 90), (70, 10), (130, 64), (40, 1)], 2, 2, 64, 64, seed=max_nq)
+    d = Device8(c, block=16)
+    batch = vxfa.paged(d.table.data_ptr(), d.n_kv.data_ptr(), d.q_start.data_ptr(), 4, c.max_pages, max_nq)
+    ctx.paged_bounds(d.k, d.ks, batch, d.b, d.bs, stream=current())
+    finish()
+    want, wants = d.b_np.copy(), d.bs_np.copy()
+    full, fulls = p8.bounds(c, 16, d.b_np, d.bs_np)
+    for s, (n, t) in enumerate(c.sizes):
+        for i in range((n - t) // 16, (n - t + min(t, max_nq) - 1) // 16 + 1):
+            page, b = c.table[s, i // 4], i % 4
+            want[page, :, b], wants[page, :, b] = full[page, :, b], fulls[page, :, b]
+    got, gots = d.bounds()
+    assert np.array_equal(got, want) and np.array_equal(gots, wants)
+    d.check_guards()
+
+
+def test_bounds_of_all_rows_again(ctx):
+    """Chunks as long as the streams, with bounds of the host's far above them."""
+    from gpu_util import vxfa
+    c = Batch8([(100, 100), (1, 1), (300, 300)], 2, 2, 128, 64, seed=3)
+    d = Device8(c, block=32)
+    batch = vxfa.paged(d.table.data_ptr(), d.n_kv.data_ptr(), d.q_start.data_ptr(), 3, c.max_pages, 2 ** 31 - 1)
+    ctx.paged_bounds(d.k, d.ks, batch, d.b, d.bs, stream=current())
+    finish()
+    want, wants = p8.bounds(c, 32, d.b_np, d.bs_np)
+    got, gots = d.bounds()
+    assert np.array_equal(got, want) and np.array_equal(gots, wants)
 
 
 def test_bounds_of_nan_and_infinite_keys(ctx):
@@ -599,6 +645,43 @@ def test_two_contexts_at_once(ctx):
     finally:
         for x in ctxs:
             x.close()
+
+
+@pytest.mark.parametrize("max_nq", [1, 3, 20])
+def test_chunks_longer_than_max_nq(ctx, max_nq):
+    """Tokens past max_nq are left out by each call; the others keep their rows."""
+    from gpu_util import vxfa
+    rng = np.random.default_rng(max_nq)
+    sizes = [(90, 40), (33, 33), (200, 1), (64, 5)]
+    kept = [(n - t + min(t, max_nq), min(t, max_nq)) for n, t in sizes]
+    c = Batch8(sizes, 8, 2, 128, 32, seed=max_nq)
+    live = np.concatenate([np.arange(t) < max_nq for _, t in sizes])
+    d = Device8(c, block=16)
+    d.batch = vxfa.paged(d.table.data_ptr(), d.n_kv.data_ptr(), d.q_start.data_ptr(), 4, c.max_pages, max_nq)
+    # attention, over all rows and over lists
+    want, err = p8.reference(c, 0.1)
+    before = d.out().copy()
+    ctx.flash_attn_ext_paged_q8(d.q, d.k, d.ks, d.v, d.vs, d.batch, d.dst, 0.1, stream=current())
+    finish()
+    check_out(d.out()[:c.T][live], want[live], err[live], True)
+    assert np.array_equal(d.out()[:c.T][~live], before[:c.T][~live], equal_nan=True)
+    b, bs = p8.bounds(c, 16, d.b_np, d.bs_np)
+    d.set_bounds(b, bs, 16)
+    d.set_list(np.full((c.T, 2, 3), -7, np.int32), 16, 1, 1)
+    ctx.paged_select(d.q, d.b, d.bs, d.batch, d.blocks, stream=current())
+    finish()
+    lists = p8.select(c, 16, b, bs, 3, 1, 1)
+    assert np.array_equal(d.list()[live], lists[live]) and (d.list()[~live] == -7).all()
+    want, err = p8.reference(c, 0.1, lists=lists, block=16)
+    ctx.flash_attn_ext_paged_blocks(d.q, d.k, d.ks, d.v, d.vs, d.batch, d.blocks, d.dst, 0.1, stream=current())
+    finish()
+    check_out(d.out()[:c.T][live], want[live], err[live], True)
+    assert np.array_equal(d.out()[:c.T][~live], before[:c.T][~live], equal_nan=True)
+    # appends
+    k_new, v_new = rows_of(rng, c, c.T), rows_of(rng, c, c.T)
+    store(ctx, c, k_new, v_new, d)
+    c.sizes = kept
+    same_stored(c, d, k_new, v_new)
 
 
 # ---- together -------------------------------------------------------------------------------

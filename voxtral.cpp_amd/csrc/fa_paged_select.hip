@@ -9,6 +9,8 @@
 // about a microsecond, and the search: one stream of 128 blocks 8.7 us in a graph, of 512 12.9, 32 uneven ones of up
 // to 512 18 (19 MB of bounds: 4 us at what a large copy reaches), of up to 2048 41 (76 MB). Bounds of
 // a token's block 4.3 us, of 8192 tokens' keys of 16 bits in blocks of 32 4.6 (17 MB: 3.4).
+#include <algorithm>
+
 #include "fa_paged_join.h"
 #include "fa_paged_q8.h"
 
@@ -93,8 +95,10 @@ static void launch_bounds(const PagedBounds& a, unsigned grid, hipStream_t st) {
 }
 
 hipError_t launch_paged_bounds(const PagedBounds& a, hipStream_t st) {
-    if (a.b.tokens <= 0 || a.b.n_streams <= 0 || a.b.max_nkv <= 0) return hipSuccess;
-    const int64_t grid = blocks_bound(a.b, a.out.lg) * ((a.hkv + 3) / 4);
+    if (a.b.max_nq <= 0 || a.b.n_streams <= 0 || a.b.max_nkv <= 0) return hipSuccess;
+    // (max_nq rows, wherever they begin, or all)
+    const int64_t per = std::min((((int64_t)a.b.max_nq - 2) >> a.out.lg) + 2, (((int64_t)a.b.max_nkv - 1) >> a.out.lg) + 1);
+    const int64_t grid = a.b.n_streams * per * ((a.hkv + 3) / 4);
     if (grid > kMaxGridX) return hipErrorNotSupported;
     if (a.d == 128 && a.sc.k) launch_bounds<128, true>(a, (unsigned)grid, st);
     else if (a.d == 128) launch_bounds<128, false>(a, (unsigned)grid, st);

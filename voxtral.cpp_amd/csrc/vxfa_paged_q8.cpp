@@ -141,10 +141,8 @@ int vxfa_paged_bounds(vxfa_ctx* c, const vxfa_tensor* k, const vxfa_tensor* k_sc
     if (!bounds || !bounds_scale) return fail(c, VXFA_INVALID_ARG, "bounds and their scales are required");
     if (!sane(bounds, true)) return fail(c, VXFA_INVALID_ARG, "bounds: unknown type, negative ne or absurd nb");
     if ((rc = check_bounds(bounds, bounds_scale, k, batch, a.out, &why)) != VXFA_OK) return fail(c, rc, "%s", why);
-    // (the tokens are on the device: as many as the streams' bounds allow)
-    int64_t tokens = (int64_t)batch->n_streams * batch->max_nq;
-    if (tokens > 0x7fffffff) tokens = 0x7fffffff;
-    a.b = batch_of(batch, k, tokens);
+    // (how many tokens there are is on the device alone: chunks are as long as q_start has it)
+    a.b = batch_of(batch, k, 0x7fffffff);
     a.kv = pool_of(k, k);
     a.d = (int32_t)k->ne[0];
     a.hkv = (int32_t)k->ne[2];
