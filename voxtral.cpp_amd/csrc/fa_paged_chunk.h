@@ -1,6 +1,6 @@
 // fa_paged_chunk.h — attention of chunks of new tokens over a paged cache, a
-// ragged batch in one launch, for gfx950. (A translation unit per head dim:
-// fa_paged_chunk.hip, fa_paged_chunk64.hip.)
+// ragged batch in one launch, for gfx950. (A translation unit per head dim and
+// type of the pages: fa_paged_chunk.hip, fa_paged_chunk64.hip; of 8 bits _q8.)
 //
 // The paged form of fa_prefill_group.hip, whose loop it has: a workgroup of 8
 // (hd 64: 4) wavefronts of 32 query rows, the heads of a kv group by as many row
@@ -37,8 +37,27 @@
 // rows 53 us, 3 pieces: 38 blocks of ~0.9 us, ~8 before and after, 7 for the join.
 // 16 streams of up to 512 tokens and 4096 rows, half of them single tokens, cap and
 // slopes 208-220 us: 416 workgroups of 8 to 128 blocks, one a CU; VALU 56 % busy.
-// With a cap the hd 128 kernel takes all 256 VGPRs and spills 6 (a wide one 7): 28 (32)
-// bytes of scratch a lane.
+// With a cap the hd 128 kernel takes all 256 VGPRs and spills 6: 28 bytes of scratch
+// a lane.
+//
+// KV8: pages of 8 bits, value = scale[granule] whole number. Whole numbers are exact
+// in f16, so the products stay those above, on whole numbers, and the scales are
+// applied in F32: K's multiplies the score; V's goes into the exponent, P' = 2^(x +
+// log2 s - m), so that f16 rounds P s as it rounds P whatever the granules' scales,
+// and the sum adds P' / s. A step's bytes come by global_load_lds a step ahead into a
+// region of their own, and each is turned into f16 once, when the workgroup stores
+// the step to the ring (v_perm_b32, one f16 operation for two): in every wavefront's
+// fragments it would be done 8 times. The scales of 32 steps' granules lie in a table
+// in LDS. With a cap the softmax of a block stands ahead of the next block's S, whose
+// registers it then has: 223 VGPRs, no scratch.
+// The conversions are VALU work beside MFMAs, and the stores of the ring meet bank
+// conflicts (8 cycles a store of 16 bytes a lane; storing the two halves in turn by row
+// changed neither the count nor the time). Graph, F16 -> 8 bits on one card: 8192 tokens 574-582 -> 605-610 us
+// (0.91 PFLOP/s), 600 on 3000 rows 55.7 -> 57, 100 on 8192 44 -> 39; the mixed batch above
+// 264 -> 300 on one set of lengths (215 on the shortest); 2000 on 4000 with a cap 181 ->
+// 203, wide 261 -> 270; hd 64, 4000 tokens 72 -> 83. Raw numbers in registers instead of LDS:
+// spills of 4 to 42; five steps ahead with a ring of three slots 581 -> 591; the reciprocal
+// scale read again at its use 605 -> 619.
 #pragma once
 
 #include "fa_paged_plan.h"
