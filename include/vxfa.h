@@ -487,8 +487,10 @@ int vxfa_flash_attn_ext_paged_q8(vxfa_ctx* ctx, const vxfa_tensor* q,
  * new tokens as elsewhere; the window has no effect. Blocks of absent pages
  * are left out. The new tokens need not be new: a batch whose chunks are as
  * long as its streams brings all their bounds up to date, as after
- * vxfa_paged_evict, which moves rows and not their bounds. One launch;
- * asynchronous on `stream`. */
+ * vxfa_paged_evict, which moves rows and not their bounds. Streams with
+ * different numbers of rows in one block of a page that they share leave any
+ * values there (whole blocks of a common prefix may be written by all). One
+ * launch; asynchronous on `stream`. */
 int vxfa_paged_bounds(vxfa_ctx* ctx, const vxfa_tensor* k,
                       const vxfa_tensor* k_scale, const vxfa_paged* batch,
                       vxfa_tensor* bounds, vxfa_tensor* bounds_scale,

@@ -265,6 +265,37 @@ def test_chunks_of_absent_pages_and_many_tiles(ctx, hd):
     attend(ctx, Batch8([(400, 100)] * 12, 16, 8, hd, page=64, seed=11), bias=1.0)
 
 
+FEW_AMONG_CHUNKS = [(3000, 1), (2500, 300), (700, 4), (0, 0), (900, 5), (64, 3), (2048, 1), (33, 33), (2, 6), (600, 2)]
+
+
+@pytest.mark.parametrize("opt", [dict(), dict(cap=30.0, bias=8.0), dict(window=500)], ids=str)
+@pytest.mark.parametrize("hq,hkv,hd", [(8, 2, 128), (5, 1, 128), (32, 1, 128), (7, 7, 64), (40, 2, 64)])
+def test_few_tokens_among_chunks(ctx, opt, hq, hkv, hd):
+    """Streams of a few tokens beside chunks: either kernel's streams, and nobody else's rows of dst."""
+    attend(ctx, Batch8(FEW_AMONG_CHUNKS, hq, hkv, hd, seed=hq, behind=3, absent=[(0, 0), (0, 100), (1, 5)]), **opt)
+
+
+def test_few_tokens_among_chunks_in_pieces(pieces):
+    attend(pieces, Batch8(FEW_AMONG_CHUNKS, 8, 2, 128, seed=3), bias=2.0)
+
+
+def test_few_tokens_among_chunks_of_many_streams(ctx):
+    """More streams than lanes; no chunks at all under a bound that allows them; chunks alone."""
+    rng = np.random.default_rng(5)
+    sizes = [(int(n), int(t)) for n, t in zip(rng.integers(1, 700, 150), rng.choice([0, 1, 1, 2, 4, 5, 40], 150))]
+    attend(ctx, Batch8(sizes, 8, 2, 64, 64, seed=6))
+    from gpu_util import vxfa
+    for sizes in ([(900, 1), (30, 1), (700, 2), (600, 4)], [(900, 100), (700, 30), (600, 5), (10, 7)]):
+        c = Batch8(sizes, 8, 2, 128, seed=7)
+        d = Device8(c)
+        d.batch = vxfa.paged(d.table.data_ptr(), d.n_kv.data_ptr(), d.q_start.data_ptr(), 4, c.max_pages, 100)
+        ctx.flash_attn_ext_paged_q8(d.q, d.k, d.ks, d.v, d.vs, d.batch, d.dst, 0.1, stream=current())
+        finish()
+        want, err = p8.reference(c, 0.1)
+        check_out(d.out(), want, err, True)
+        d.check_guards()
+
+
 @pytest.mark.parametrize("layout", ["row", "head"])
 @pytest.mark.parametrize("page", [16, 128, 1024])
 def test_chunk_pages_and_strides(ctx, page, layout):
