@@ -37,14 +37,26 @@ struct RowsPlan {
 // 117.4. Over 196 mixes of heads, streams and rows (half of them even, half uneven)
 // the rule is 0.5 % off the better choice on average, 15 % at worst: 1 stream
 // that is shorter than its bound of 512.
-inline bool rows_whole(const PagedBatch& b, int nhg, int head_dim) {
+// i8: pages of 8 bits, by another kernel, which gains more by a cut: a workgroup alone
+// 7.5 ns a row (hd 64: 5), and none whole beyond 1024 rows. Cut -> whole, 8 kv heads of
+// 128: 1 stream of 256 rows 7.7 -> 6.0, of 512 7.5 -> 8.2; 4 uneven ones of 1024 8.8 ->
+// 12.5; 16 of 512 12.1 -> 10.4; 32 uneven ones of 512 12.8 -> 10.4, of 2048 24.6 -> 31.5;
+// 20 heads of 64: 8 of 512 10.8 -> 9.4, of 1024 13.5 -> 15.9, 32 of 2048 44.9 -> 56.8. Over
+// 195 mixes 0.5 % off the better choice, 31 % at worst (2 streams that are shorter than
+// their bound of 512); by the rule for F16 3.3 %, 52 %.
+inline bool rows_whole(const PagedBatch& b, int nhg, int head_dim, bool i8) {
+    if (i8) {
+        const double n = 1e-3 * b.max_nkv, alone = head_dim == 128 ? 7.5 : 5.0;
+        const double together = (double)b.n_streams * nhg * 2 * head_dim / 5600;
+        return b.max_nkv <= 1024 && n * (alone > 0.7 * together ? alone : 0.7 * together) < 2.5 + 0.6 * n * together;
+    }
     const double n = 1e-3 * b.max_nkv, alone = head_dim == 128 ? 10.5 : 6.5;
     const double together = 0.7 * (double)b.n_streams * nhg * 4 * head_dim / 5600;
     return b.max_nkv <= 2048 && 4.5 + n * (alone > together ? alone : together) < 7.5 + 1.05 * n * together;
 }
 
 // The grid of a call: `items` parts per head group.
-inline RowsPlan rows_plan(const PagedBatch& b, int nhg, int head_dim, int64_t room, int32_t& items) {
+inline RowsPlan rows_plan(const PagedBatch& b, int nhg, int head_dim, int64_t room, int32_t& items, bool i8 = false) {
     RowsPlan p;
     p.empty = 0;
     p.small = 512 / nhg > 0 ? 512 / nhg : 1;
@@ -60,7 +72,7 @@ inline RowsPlan rows_plan(const PagedBatch& b, int nhg, int head_dim, int64_t ro
         else p.cuts = 0;
     }
     if (p.small > p.large) p.small = p.large;
-    if (rows_whole(b, nhg, head_dim)) p.cuts = 0;
+    if (rows_whole(b, nhg, head_dim, i8)) p.cuts = 0;
     items = b.n_streams;
     if (p.cuts) {
         const int64_t by_rows = (int64_t)b.n_streams * ((b.max_nkv + 63) / 64);

@@ -471,7 +471,7 @@ hipError_t launch_paged_rows_q8(const PagedBlocks& pb, int head_dim, hipStream_t
     ra.cut = reinterpret_cast<int2*>(a.ws);
     ra.recs = reinterpret_cast<float*>(a.ws + cut);
     const int64_t room = (int64_t)((a.ws_bytes - cut) / ((size_t)ra.rec * sizeof(float))) / nhg;
-    ra.p = rows_plan(a.b, nhg, head_dim, room, ra.items);
+    ra.p = rows_plan(a.b, nhg, head_dim, room, ra.items, true);
     const bool wide = ra.p.cuts && rows_wide(a.b, nhg) && 4096 / nhg + 1 + (int64_t)a.b.n_streams <= room;
     if (wide) {
         ra.p.small = 2048 / nhg > 0 ? 2048 / nhg : 1;
