@@ -447,6 +447,20 @@ def test_choice_of_equal_scores(ctx):
         choose(ctx, c, 16, 20, 1, 1, b=(b, np.full((c.n_pages, c.hkv, 1), 0.5, np.float32)))
 
 
+@pytest.mark.parametrize("q_type", ["f16", "f32"])
+def test_choice_by_queries_of_all_sizes(ctx, q_type):
+    """Queries of zeros, of the least f16 numbers, of the largest, one head far above the others; F32 ones are rounded to f16."""
+    c = Batch8([(500, 6), (300, 1), (900, 20)], 8, 2, 128, 32, q_type=q_type, seed=3)
+    rng = np.random.default_rng(4)
+    c.q[0] = 0
+    c.q[1] = rng.choice([-1, 0, 1], c.q[1].shape) * 2.0 ** -24
+    c.q[2] = rng.choice([-65504, 65504], c.q[2].shape)
+    c.q[3, 0] *= 1000
+    c.q[4, :, 1:] = 0
+    c.q[6] *= 2.0 ** -13
+    choose(ctx, c, 16, 5, 1, 1)
+
+
 def test_choice_of_many_blocks(ctx):
     """Streams of more blocks than a segment, scores of either sign."""
     rng = np.random.default_rng(5)
