@@ -518,8 +518,9 @@ typedef struct vxfa_blocks {
  * exact in F32, and the choice the same everywhere. (No cap or slope changes
  * it; a negative scale of the attention turns its meaning around.) q [D, T,
  * Hq, 1] F16 or F32. Tokens of no stream leave the list as it was.
- * bounds_scale: powers of two from 2^-64 to 2^64 (others: the choice may
- * differ from the formula's). At most 262144 blocks of a stream (max_nkv; else
+ * bounds_scale: powers of two from 2^-64 to 2^64 (what lies outside counts as
+ * the nearer end, NaN as 2^-64; by others the choice may differ from the
+ * formula's). At most 262144 blocks of a stream (max_nkv; else
  * VXFA_UNSUPPORTED). Where streams have more than 4096 blocks (with 16 / n
  * tokens of a stream at once for kv heads of n query heads, n rounded up to a
  * power of two, 16384 by that many), and with few tokens from 512 on, the call

@@ -375,7 +375,8 @@ __global__ __launch_bounds__(64 * NW) void paged_select_blocks(SelectArgs sa) {
                 const char* const src = a.in.b + max(page[j], 0) * a.in.nb3 + hk * a.in.nb2 + place[j] * a.in.nb1 + 16 * quad;
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) kb[j][ks] = *(const intx4*)(src + 64 * ks);
-                s[j] = *(const float*)(a.in.s + max(page[j], 0) * a.in.s_nb3 + hk * a.in.s_nb2 + 4 * (int64_t)place[j]);
+                // (no NaN: of some the keys lie so high that the search's thresholds pass 32 bits)
+                s[j] = scale_in_range(*(const float*)(a.in.s + max(page[j], 0) * a.in.s_nb3 + hk * a.in.s_nb2 + 4 * (int64_t)place[j]));
             }
             find(t0 + U * NW < nt ? t0 + U * NW : wave);   // (the next pass begins again)
 #pragma unroll
