@@ -349,7 +349,9 @@ __global__ __launch_bounds__(64 * NW) void paged_select_blocks(SelectArgs sa) {
         m = fmaxf(m, shfl_xor(m, 16));
         m = fmaxf(m, shfl_xor(m, 32));
         const int e = exp_for(m);
-        const float f = two_to(-e), fs = valid ? two_to(e) : 0.f;
+        // (scores times 2^-32, which leaves their order: with infinities in query and keys they reach 2^150, of the
+        // least numbers 2^-94)
+        const float f = two_to(-e), fs = valid ? two_to(e - 32) : 0.f;
         intx4 qb[KS];
 #pragma unroll
         for (int ks = 0; ks < QS; ++ks)
