@@ -479,8 +479,8 @@ int vxfa_flash_attn_ext_paged_q8(vxfa_ctx* ctx, const vxfa_tensor* q,
  * n_pages, 1], contiguous along ne[0]. Of a block and head with keys k: 2^e
  * the least power (-64 <= e <= 64) with max |k| <= 127 * 2^e; element d < D
  * the largest k_d / 2^e, rounded up, element D + d the smallest, rounded down.
- * (NaN among keys is passed over; what lies beyond 127 * 2^64, as infinities
- * do, counts as that.) */
+ * (NaN among keys is passed over, a dim without a number counts as 0; what
+ * lies beyond 127 * 2^64, as infinities do, counts as that.) */
 
 /* Bounds of the blocks that the batch's new tokens lie in, over the streams'
  * rows in them. k_scale: of a pool of 8 bits; NULL for F16. max_nq bounds the

@@ -71,6 +71,7 @@ __global__ __launch_bounds__(256) void paged_bounds_kernel(PagedBounds a) {
     for (int i = 0; i < 4; ++i) {
         hi[i] = CH == 32 ? pair32_max(hi[i]) : quad_max(hi[i]);
         lo[i] = -(CH == 32 ? pair32_max(lo[i]) : quad_max(lo[i]));
+        if (hi[i] < lo[i]) hi[i] = lo[i] = 0.f;           // (no number among the block's keys: all NaN)
         m = fmaxf(m, fmaxf(fabsf(hi[i]), fabsf(lo[i])));
     }
     const int e = exp_for(__builtin_bit_cast(float, wave_max(__builtin_bit_cast(int, m))));
