@@ -63,9 +63,11 @@ static __global__ __launch_bounds__(64) void paged_rows_combine(RowsArgs ra, int
     const int i = TOKENS ? 0 : (int)blockIdx.y, s = (int)blockIdx.z;
     PagedStream st;
     int2 cut;
-    // (one stream's parts begin at 0: its records are on their way before their number
-    // is known)
-    bool one = a.b.n_streams == 1;
+    // (One stream's parts begin at 0: its records are on their way before their number is known, as
+    // far as a round of the lanes takes them. Of a bound far above the rows there are up to 513: read
+    // ahead -> not, 32/8 heads of 128, bound 131072: 8 bits 8192 rows 11.6 -> 9.8 us, four heads a workgroup 15.3
+    // -> 11.1 and 300 rows 14.2 -> 9.4; F16 pages, 8192 rows 13.6 -> 11.9. Up to 128 records the two are even.)
+    bool one = a.b.n_streams == 1 && ra.items <= 64;
     if constexpr (TOKENS) {
         const int t = (int)blockIdx.y;
         st = PagedStream{t, paged_token(a.b, t).s >= 0 ? 1 : 0, 0};
