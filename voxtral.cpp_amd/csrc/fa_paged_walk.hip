@@ -456,10 +456,16 @@ static void launch_walk(const WalkArgs& wa, dim3 grid, hipStream_t st) {
 // Whether a workgroup's wavefronts take four neighbouring heads, each all rows of the part, or one
 // head's rows in turn: neighbouring heads' rows are neighbouring lines, which memory gives
 // faster at once, but a wavefront's walk is four times as long. By the bounds' rows x heads; one -> four heads,
-// 8 kv heads of 128: 1 stream of 8192 8.8 -> 15.2 us, 32768 18.0 -> 24.5; 8 even ones of 8192 (half a million)
-// 31.6 -> 33.0, 16 of them 60.2 -> 51.7, 32 uneven ones of up to 2500 25.8 -> 26.1, of 8192 69.8 -> 63.1;
-// 20 heads of 64: 8 uneven ones of 1500 21.6 -> 21.6, 32 of 2500 43.3 -> 36.2, of 8192 127 -> 107.
-static bool rows_wide(const PagedBatch& b, int nhg) { return nhg % 4 == 0 && (double)b.n_streams * b.max_nkv * nhg >= 786432.0; }
+// 8 kv heads of 128: 8 even streams of 8192 (half a million) 31.5 -> 33.0 us, 12 of them 43.8 -> 43.4, 16 58.6 -> 50.5,
+// 4 of 32768 59.3 -> 49.9; 32 uneven ones of up to 2048 24.0 -> 24.4, of 8192 60.4 -> 56.3; 20 heads of 64: 8 uneven ones of
+// 1500 21.6 -> 21.6, 32 of 2048 35.3 -> 28.7, of 8192 117 -> 84; one stream of 32768 31 -> 29, of 131072 109 -> 83.
+// Rows far below their bounds, whose parts are short, lose by it: at hd 128 2 streams of 512 8.0 -> 9.8, 4 of 8192
+// 19 -> 23, 16 of 2048 20.5 -> 23.7, 32 of 512 14.9 -> 16.6; at hd 64 2 to 32 of 512 10 % more to 10 % less. So one
+// stream of 128 keeps one head a workgroup: it would gain at 131072 rows (56 -> 51), but lose below its
+// bound: 8192 rows 9.8 -> 11.1, 300 7.6 -> 9.4 (hd 64: 13.2 -> 13.5, 7.4 -> 8.2).
+static bool rows_wide(const PagedBatch& b, int nhg, int head_dim) {
+    return nhg % 4 == 0 && (b.n_streams > 1 || head_dim == 64) && (double)b.n_streams * b.max_nkv * nhg >= 786432.0;
+}
 
 hipError_t launch_paged_rows_q8(const PagedBlocks& pb, int head_dim, hipStream_t st) {
     const PagedAttn& a = pb.a;
@@ -478,7 +484,7 @@ hipError_t launch_paged_rows_q8(const PagedBlocks& pb, int head_dim, hipStream_t
     ra.recs = reinterpret_cast<float*>(a.ws + cut);
     const int64_t room = (int64_t)((a.ws_bytes - cut) / ((size_t)ra.rec * sizeof(float))) / nhg;
     ra.p = rows_plan(a.b, nhg, head_dim, room, ra.items, true);
-    const bool wide = ra.p.cuts && rows_wide(a.b, nhg) && 4096 / nhg + 1 + (int64_t)a.b.n_streams <= room;
+    const bool wide = ra.p.cuts && rows_wide(a.b, nhg, head_dim) && 4096 / nhg + 1 + (int64_t)a.b.n_streams <= room;
     if (wide) {
         ra.p.small = 2048 / nhg > 0 ? 2048 / nhg : 1;
         ra.p.large = 4096 / nhg > 0 ? 4096 / nhg : 1;
