@@ -7,6 +7,7 @@ import subprocess
 import pytest
 
 from conftest import ROOT, load_package
+from paged8_choices import LONG
 
 LIB = load_package().vxfa.LIB_PATH
 pytestmark = pytest.mark.skipif(not os.path.exists(LIB), reason="libvxfa.so not built")
@@ -54,3 +55,32 @@ def test_many_rows_take_four_heads_a_workgroup(routes):
         assert heads_of_a_workgroup(routes("attend", hq=32, hkv=8, hd=hd, streams=2, max_pages=65536 // 64)) == 4
         assert heads_of_a_workgroup(routes("attend", hq=32, hkv=8, hd=hd, streams=11, max_pages=8192 // 64)) == 1
         assert heads_of_a_workgroup(routes("attend", hq=6, hkv=6, hd=hd, streams=32, max_pages=8192 // 64)) == 1
+
+
+@pytest.mark.parametrize("name", LONG)
+def test_long_choices_take_the_search_of_a_team(routes, name):
+    """The calls of test_gpu_paged_choice.py run the kernels that they are there for."""
+    c, (threads, seg, segs, join) = LONG[name]
+    hkv, t = c.get("hkv", 8), max(t for _, t in c["sizes"])
+    group = c.get("hq", 8) // hkv
+    tile = min(16 // min(1 << (group - 1).bit_length(), 16), t)
+    got = routes("choose", hq=c.get("hq", 8), hkv=hkv, hd=c.get("hd", 64), streams=len(c["sizes"]), nq=t, tokens=sum(t for _, t in c["sizes"]),
+                 page=4096, block=16, top=c["top"], window=c.get("window", 0), max_pages=-(-max(n for n, _ in c["sizes"]) // 4096),
+                 max_nkv=max(n for n, _ in c["sizes"]))
+    assert got[0][:2] == ("paged_select_blocks", (str(c.get("hd", 64)), str(threads // 64))) and got[0][3] == threads
+    assert got[0][4] == 4 * tile * seg and got[0][2] % (hkv * segs) == 0
+    assert seg > 512 and (join > 1 or hkv * got[0][2] >= 128)
+    if join:
+        assert [x[:2] for x in got[1:]] == [("paged_select_join", (str(join),))]
+        assert min(c["top"], seg) * segs > 1024 or join == 1
+    else:
+        assert len(got) == 1
+
+
+def test_four_heads_a_workgroup_with_and_without_options(routes):
+    """The calls of test_gpu_paged_q8_routes.py run the kernels that they are there for."""
+    for (hq, hkv, hd), streams in [((32, 8, 128), 12), ((8, 8, 128), 12), ((8, 4, 64), 24), ((24, 8, 64), 12)]:
+        for cap in (0, 30):
+            got = routes("attend", hq=hq, hkv=hkv, hd=hd, streams=streams, max_pages=128, cap=cap)
+            assert got[0][:2] == ("paged_walk_kernel", (str(hd), "true", "false", "4", "false" if cap else "true", "4"))
+    assert heads_of_a_workgroup(routes("attend", hq=64, hkv=64, hd=64, streams=8, max_pages=131)) == 4
