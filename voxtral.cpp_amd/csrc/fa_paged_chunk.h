@@ -43,8 +43,8 @@
 // KV8: pages of 8 bits, value = scale[granule] whole number. Whole numbers are exact
 // in f16, so the products stay those above, on whole numbers, and the scales are
 // applied in F32: K's multiplies the score; V's goes into the exponent, P' = 2^(x +
-// log2 s - m), so that f16 rounds P s as it rounds P whatever the granules' scales,
-// and the sum adds P' / s. A step's bytes come by global_load_lds a step ahead into a
+// log2 s - m), so that f16 rounds P s as it rounds P (by 2^-25 of the largest where
+// they lie more than 2^14 below it), and the sum adds P' / s. A step's bytes come by global_load_lds a step ahead into a
 // region of their own, and each is turned into f16 once, when the workgroup stores
 // the step to the ring (v_perm_b32, one f16 operation for two): in every wavefront's
 // fragments it would be done 8 times. The scales of 32 steps' granules lie in a table
@@ -454,7 +454,7 @@ static __global__ __launch_bounds__((PC<HD, KVGROUPS>::NT), 2) void paged_chunk_
     const float slope = MOD ? __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, paged_slope(a, h)))) : 0.f;
     float m = -INFINITY, l = 0.f;
     // KV8: the block's scales for the lane's granule: K's times c; log2 of V's, which is added to the
-    // scores (P are then the weights of whole numbers, and rounded as such whatever the scales);
+    // scores (P are then the weights of whole numbers, and rounded as such);
     // 1 / V's, which the sum of P takes back
     float cs = c, lsv = 0.f, isv = 1.f;
     auto scales_of = [&](int t) {

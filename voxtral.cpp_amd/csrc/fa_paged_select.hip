@@ -5,8 +5,9 @@
 // q is larger than sum_d max(q_d lo_d, q_d hi_d) = sum_d max(q_d, 0) hi_d + min(q_d, 0) lo_d.
 // With bounds and queries in 8 bits at scales that are powers of two that is one
 // product of whole numbers, of length 2 D, on v_mfma_i32_16x16x64_i8: exact, so the choice depends on
-// no order of sums. The choice is bound by the chain of its loads (sizes, pages, bounds), each of
-// about a microsecond, and the search: one stream of 128 blocks 8.7 us in a graph, of 512 12.9, 32 uneven ones of up
+// no order of sums. The choice is bound by a chain of loads (sizes, pages, queries, bounds), each of
+// about a microsecond, and the search; the first bounds are asked for after the queries are converted, which
+// each wavefront does for all columns (about 270 of its 661 VALU instructions), so the chain is longer than it has to be: one stream of 128 blocks 8.7 us in a graph, of 512 12.9, 32 uneven ones of up
 // to 512 18 (19 MB of bounds: 4 us at what a large copy reaches), of up to 2048 41 (76 MB). Bounds of
 // a token's block 4.3 us, of 8192 tokens' keys of 16 bits in blocks of 32 4.6 (17 MB: 3.4).
 #include <algorithm>
@@ -434,7 +435,7 @@ __global__ __launch_bounds__(64 * NW) void paged_select_blocks(SelectArgs sa) {
 }
 
 // Among the segments' best: a workgroup per token and kv head, of one wavefront (up to 1024 pairs) or 16
-// (up to 16384; beyond, one of them reads the pairs again and again).
+// (up to 16384; beyond, one of them reads the pairs again and again: 65536 blocks, top 1024 86 us, 69632 1.28 ms).
 template <int NW>
 __global__ __launch_bounds__(64 * NW) void paged_select_join(SelectArgs sa) {
     __shared__ ChooseRoom room;

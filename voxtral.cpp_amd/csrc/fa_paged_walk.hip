@@ -16,8 +16,8 @@
 //   bytes that the conversion makes anyway (v_perm_b32).
 //   8 bits: a whole number is exact in f16; K's scale multiplies the score, in F32. V's is
 //   taken into the exponent: with x' = x + log2(s) the weights P' = 2^(x' - max x') are those that
-//   multiply whole numbers, so f16 rounds them as it rounds P, however the scales of
-//   blocks differ; the sum of the softmax adds P' / s, in F32.
+//   multiply whole numbers, and f16 rounds them as it rounds P: by half a step, or, of rows whose P s
+//   lies more than 2^14 below the largest, by 2^-25 of that; the sum of the softmax adds P' / s, in F32.
 //   Chosen blocks: which tile is which row is read from the list, 32 steps at a time, a
 //   lane each, with the page and the scales. A call's tokens are cut into equal parts of
 //   their lists where they are few.
